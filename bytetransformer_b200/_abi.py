@@ -87,6 +87,11 @@ SIGNATURES = {
     "bt_add_bias_residual_layernorm_restore": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _f, _vp]),
     "bt_add_bias_gelu": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "bt_masked_softmax": (_i, [_vp, _vp, _i, _i, _i, _f, _vp]),
+    "bt_relative_position_bias": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),
+    "bt_relative_position_bias_grad_workspace": (_i, [_i, _i, _i, _i, _i, _i, C.POINTER(_sz)]),
+    "bt_relative_position_bias_grad": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
+    "bt_add_residual_rmsnorm": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _f, _vp]),
+    "bt_add_residual_rmsnorm_e4m3": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _vp]),
     "bt_profile_enable": (_i, [_vp, _i]),
     "bt_profile_read": (_i, [_vp, C.POINTER(C.c_double), C.POINTER(C.c_longlong)]),
 }

@@ -1,0 +1,450 @@
+// Learned relative position bias by buckets of distance, and its gradient.
+//
+//   bias[h, q, k] = table[bucket(k - (q + q_start)), h]
+//   grad_table[b, h] = sum of grad[i, h, q, k] over i, q, k with bucket(k - (q + q_start)) = b
+//
+// bucket(d), N buckets, largest distance told apart D: one-sided, the N buckets belong to n = max(-d, 0);
+// bidirectional, half of them to n = |d| at d <= 0 and half to n = d at d > 0.  Of a side's m buckets the first
+// e = m / 2 hold one distance each, the others grow with its logarithm:
+//   n < e: n,   else min(m - 1, e + floor((m - e) * log(n / e) / log(D / e))).
+// The borders are whole numbers, found on the host without rounding (see bucket_borders), so a distance on a border
+// falls on the same side for every caller and every device.
+//
+// What both kernels live on: a bias is constant along diagonals.
+#include <math.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "../../include/bt_b200.h"
+
+namespace bt {
+
+namespace {
+
+constexpr int kMaxBuckets = 256;
+constexpr int kMaxDistance = 1 << 20;
+
+// Smallest distance of each bucket of a side, rising: bucket(n) = the last i with first[i] <= n.
+struct Borders {
+  int first[kMaxBuckets];
+  int count;      // buckets of a side
+  int sides;      // 1 or 2
+  int exact;      // buckets of one distance each
+  float log_scale;  // (count - exact) / log2(D / exact): where to look first
+};
+
+// n^m * e^j against D^j * e^m in whole numbers of at most 4096 bits (20 bits * 128 + 7 bits * 128 at the limits above).
+struct Whole {
+  uint32_t limb[128];
+  int n = 1;
+  Whole() { limb[0] = 1; }
+  void times(uint32_t f, int power) {
+    while (power-- > 0) {
+      uint64_t carry = 0;
+      for (int i = 0; i < n; ++i) {
+        carry += static_cast<uint64_t>(limb[i]) * f;
+        limb[i] = static_cast<uint32_t>(carry);
+        carry >>= 32;
+      }
+      if (carry != 0 && n < 128) limb[n++] = static_cast<uint32_t>(carry);
+    }
+  }
+  bool less(const Whole& o) const {
+    if (n != o.n) return n < o.n;
+    for (int i = n - 1; i >= 0; --i)
+      if (limb[i] != o.limb[i]) return limb[i] < o.limb[i];
+    return false;
+  }
+};
+
+bool bucket_borders(Borders* b, int num_buckets, int max_distance, int bidirectional) {
+  b->sides = bidirectional ? 2 : 1;
+  b->count = num_buckets / b->sides;
+  b->exact = b->count / 2;
+  const int e = b->exact, m = b->count - e;
+  b->log_scale = static_cast<float>(m / log2(static_cast<double>(max_distance) / e));
+  for (int i = 0; i <= e; ++i) b->first[i] = i;
+  for (int j = 1; j < m; ++j) {
+    // Step j starts at the first whole n >= e * (D / e)^(j / m).  Double precision finds it unless that is a whole number
+    // itself, or so near one that rounding could tell them apart wrongly.
+    const double x = e * pow(static_cast<double>(max_distance) / e, static_cast<double>(j) / m);
+    const double near = nearbyint(x);
+    int n = static_cast<int>(ceil(x));
+    if (fabs(x - near) < 1e-9 * x) {
+      n = static_cast<int>(near);
+      Whole have, need;
+      have.times(static_cast<uint32_t>(n), m);
+      have.times(static_cast<uint32_t>(e), j);
+      need.times(static_cast<uint32_t>(max_distance), j);
+      need.times(static_cast<uint32_t>(e), m);
+      if (have.less(need)) ++n;
+    }
+    b->first[e + j] = n;
+  }
+  return true;
+}
+
+// Bucket of distance d by the borders in shared memory: the logarithm to a few bits, then the borders decide.
+__device__ __forceinline__ int bucket_of(int d, const Borders& b, const int* first) {
+  int n = d < 0 ? -d : (b.sides == 2 ? d : 0);
+  int i = n;
+  if (n >= b.exact) {
+    i = b.exact + static_cast<int>(__log2f(__fdividef(static_cast<float>(n), static_cast<float>(b.exact))) * b.log_scale);
+    i = min(i, b.count - 1);
+    while (i + 1 < b.count && first[i + 1] <= n) ++i;
+    while (first[i] > n) --i;
+  }
+  return (b.sides == 2 && d > 0) ? i + b.count : i;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+struct BiasArgs {
+  const void* table;  // [buckets, heads]
+  void* out;          // [heads, q_len, k_len]
+  int heads, q_len, k_len, q_start;
+  int rows, cols;     // of a CTA's tile
+  Borders borders;
+};
+
+constexpr int kBiasThreads = 256;
+
+// A CTA writes `rows` x `cols` of one head.  The tile holds rows + cols - 1 different values, one per diagonal; row r is
+// the slice of them that starts at rows - 1 - r.  So the CTA lays the values of its diagonals out in shared memory once,
+// 16 / sizeof(T) times, each copy an element further on: a slice then starts on a 16-byte boundary in one of the copies,
+// whichever boundary its place in global memory asks for, and leaves by one bulk copy.
+template <typename T, typename TableT>
+__global__ void __launch_bounds__(kBiasThreads) relative_bias_kernel(const __grid_constant__ BiasArgs a) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ T column[kMaxBuckets];
+  __shared__ int first[kMaxBuckets];
+  pdl_launch_dependents();
+  const int head = blockIdx.z;
+  const int q0 = blockIdx.y * a.rows;
+  const int k0 = blockIdx.x * a.cols;
+  const int rows = min(a.rows, a.q_len - q0);
+  const int cols = min(a.cols, a.k_len - k0);
+  const int diagonals = rows + cols - 1;
+  const int pitch = (a.rows + a.cols + V + V - 1) / V * V;  // elements of a copy, a multiple of 16 bytes
+  T* copies = reinterpret_cast<T*>(smem);
+  for (int i = threadIdx.x; i < a.borders.count; i += kBiasThreads) first[i] = a.borders.first[i];
+  pdl_wait();
+  for (int i = threadIdx.x; i < a.borders.count * a.borders.sides; i += kBiasThreads)
+    column[i] = static_cast<T>(static_cast<float>(reinterpret_cast<const TableT*>(a.table)[static_cast<size_t>(i) * a.heads + head]));
+  __syncthreads();
+  // diagonal x of the tile: distance of its last row's first element, plus x
+  const int d0 = k0 - (q0 + rows - 1) - a.q_start;
+  for (int x = threadIdx.x; x < diagonals; x += kBiasThreads) {
+    const T v = column[bucket_of(d0 + x, a.borders, first)];
+#pragma unroll
+    for (int p = 0; p < V; ++p)
+      if (x >= p) copies[p * pitch + x - p] = v;
+  }
+  fence_proxy_async_smem();
+  __syncthreads();
+  T* out = reinterpret_cast<T*>(a.out) + (static_cast<size_t>(head) * a.q_len + q0) * a.k_len + k0;
+  // elements of row r ahead of its first 16-byte boundary
+  auto head_of = [&](int r) {
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out + static_cast<size_t>(r) * a.k_len) / sizeof(T));
+    return min(static_cast<int>((V - at % V) % V), cols);
+  };
+  for (int r = threadIdx.x; r < rows; r += kBiasThreads) {
+    const int lead = head_of(r);
+    const int body = (cols - lead) / V * V;
+    const int x = rows - 1 - r + lead;
+    if (body > 0)
+      bulk_store(out + static_cast<size_t>(r) * a.k_len + lead, copies + (x % V) * pitch + x / V * V, static_cast<uint32_t>(body * sizeof(T)));
+  }
+  tma_store_commit();
+  // the ragged ends of the rows, 2 V - 2 elements at most: 2 V lanes for each row
+  for (int i = threadIdx.x; i < rows * 2 * V; i += kBiasThreads) {
+    const int r = i / (2 * V), s = i % (2 * V);
+    const int lead = head_of(r);
+    const int body = (cols - lead) / V * V;
+    const int c = s < V ? s : lead + body + s - V;
+    if (s < V ? c < lead : c < cols) out[static_cast<size_t>(r) * a.k_len + c] = copies[rows - 1 - r + c];
+  }
+  tma_store_wait_read();
+}
+
+// ------------------------------------------------------------------------------------------------ gradient
+struct GradArgs {
+  const void* grad;  // [batch, heads, q_len, k_len]
+  float* partial;    // [heads, buckets, parts]
+  int batch, heads, q_len, k_len, q_start;
+  int groups;  // CTAs side by side over a row chunk's diagonals
+  int chunks;  // row chunks
+  int parts;   // batch * chunks * groups
+  Borders borders;
+};
+
+constexpr int kGradThreads = 256;
+constexpr int kGradRows = 128;  // rows of a chunk: the longest chain of single-precision additions
+
+// A CTA sums the diagonals of `kGradRows` rows of one plane (sequence, head), over a range of diagonals, then the
+// diagonals of each bucket.  A thread holds 2 V - 1 diagonals (V = elements of 16 bytes) in registers and walks down them,
+// V rows and one aligned 16-byte load per row at a time: with every row the matrix's next aligned vector lies
+// k_len + 1 elements further on relative to the diagonals, so the vector of row r starts (-r * (k_len + 1)) mod V diagonals
+// into the thread's range, a number that only k_len mod V (M) decides and that repeats every V rows.  So every index of
+// a register is known at compile time, whatever the row length, and neighbouring threads load neighbouring vectors.
+template <typename T, int M>
+__global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const __grid_constant__ GradArgs a) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  constexpr int kSpan = kGradThreads * V;
+  __shared__ float low[kSpan + V], high[kSpan + V];
+  __shared__ int first[kMaxBuckets + 1];
+  pdl_launch_dependents();
+  const int t = threadIdx.x;
+  for (int i = t; i < a.borders.count; i += kGradThreads) first[i] = a.borders.first[i];
+  if (t == 0) first[a.borders.count] = 0x7fffffff;
+  const int group = blockIdx.x % a.groups;
+  const int chunk = blockIdx.x / a.groups;
+  const int head = blockIdx.y;
+  const int item = blockIdx.z;
+  const int q0 = chunk * kGradRows;
+  const int q1 = min(q0 + kGradRows, a.q_len);
+  const size_t plane = (static_cast<size_t>(item) * a.heads + head) * a.q_len * a.k_len;
+  const T* base = reinterpret_cast<const T*>(a.grad) + plane;
+  // The range's first diagonal, as column minus row: the chunk's leftmost one, -(q1 - 1), rounded down so that the vectors
+  // of the rows q0, q0 + V, ... are aligned in it (their columns are that diagonal plus the row).
+  const int phase = static_cast<int>((plane + static_cast<size_t>(q0) * a.k_len) % V);  // elements of row q0 past a boundary
+  const int leftmost = q0 - (q1 - 1);                                                   // as column, seen from row q0
+  int c0 = leftmost - (V - 1) + phase;  // (a row's vectors start up to V - 1 diagonals further on)
+  c0 = (c0 >= 0 ? c0 / V : -((-c0 + V - 1) / V)) * V - phase;                            // aligned column of row q0
+  c0 += group * kSpan + t * V;
+  float acc[2 * V - 1];
+#pragma unroll
+  for (int i = 0; i < 2 * V - 1; ++i) acc[i] = 0.f;
+  pdl_wait();
+#pragma unroll 1
+  for (int q = q0, c = c0; q < q1; q += V, c += V) {
+    if (c >= a.k_len || c + 3 * V - 2 <= 0) continue;  // the V vectors lie in columns c .. c + 3 V - 3
+    const bool inside = c >= 0 && c + 3 * V - 2 <= a.k_len && q + V <= q1;
+    uint4 v[V];
+    if (inside) {
+#pragma unroll
+      for (int r = 0; r < V; ++r) {
+        constexpr int kStep = M + 1;
+        const int shift = (V * kStep - r * kStep) % V;  // static: see above
+        v[r] = *reinterpret_cast<const uint4*>(base + static_cast<size_t>(q + r) * a.k_len + (c + r + shift));
+      }
+    } else {
+      for (int r = 0; r < V; ++r) {
+        constexpr int kStep = M + 1;
+        const int shift = (V * kStep - r * kStep) % V;
+        T e[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const int col = c + r + shift + i;
+          e[i] = (q + r < q1 && col >= 0 && col < a.k_len) ? base[static_cast<size_t>(q + r) * a.k_len + col] : static_cast<T>(0.f);
+        }
+        v[r] = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < V; ++r) {
+      constexpr int kStep = M + 1;
+      const int shift = (V * kStep - r * kStep) % V;
+      const uint32_t w[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (V == 8)
+          add_half2(acc[shift + 2 * i], acc[shift + 2 * i + 1], w[i]);
+        else
+          acc[shift + i] += __uint_as_float(w[i]);
+      }
+    }
+  }
+  // Diagonal t * V + i of the range: the thread's own first V in `low`, what it holds of its right neighbour's in `high`
+#pragma unroll
+  for (int i = 0; i < V; ++i) low[t * V + i] = acc[i];
+#pragma unroll
+  for (int i = V; i < 2 * V - 1; ++i) high[t * V + i] = acc[i];
+  high[t * V + 2 * V - 1] = 0.f;
+  if (t == 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      high[i] = 0.f;
+      low[kSpan + i] = 0.f;
+    }
+  }
+  __syncthreads();
+  // Distance of diagonal x: x + d_first.  A bucket is a run of distances; a warp sums a bucket's, in double precision: the
+  // runs are up to a range long.
+  const int d_first = c0 - t * V - q0 - a.q_start;
+  const int total = a.borders.count * a.borders.sides;
+  const int part = (item * a.chunks + chunk) * a.groups + group;
+  for (int b = t >> 5; b < total; b += kGradThreads / 32) {
+    const int i = b % a.borders.count;
+    long long lo, hi;  // distances of the bucket, inclusive
+    if (b >= a.borders.count) {
+      lo = max(first[i], 1);
+      hi = first[i + 1] - 1LL;
+    } else {
+      lo = i + 1 < a.borders.count ? 1LL - first[i + 1] : -0x7fffffffLL;
+      hi = (i == 0 && a.borders.sides == 1) ? 0x7fffffffLL : -static_cast<long long>(first[i]);
+    }
+    const int x0 = static_cast<int>(max(lo - d_first, 0LL));
+    const int x1 = static_cast<int>(min(hi - d_first, static_cast<long long>(kSpan + V - 1)));
+    double sum = 0.0;
+    for (int x = x0 + (t & 31); x <= x1; x += 32) sum += static_cast<double>(low[x]) + static_cast<double>(high[x]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((t & 31) == 0) a.partial[(static_cast<size_t>(head) * total + b) * a.parts + part] = static_cast<float>(sum);
+  }
+}
+
+// One warp per (head, bucket): the CTAs' sums, in a fixed order.
+__global__ void __launch_bounds__(256) relative_bias_grad_join_kernel(const float* __restrict__ partial, float* __restrict__ out,
+                                                                      int heads, int buckets, int parts) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int at = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (at >= heads * buckets) return;
+  double sum = 0.0;
+  for (int i = threadIdx.x & 31; i < parts; i += 32) sum += partial[static_cast<size_t>(at) * parts + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) out[static_cast<size_t>(at % buckets) * heads + at / buckets] = static_cast<float>(sum);
+}
+
+bool bias_shape_ok(int num_buckets, int max_distance, int bidirectional, int heads, int q_len, int k_len, int q_start) {
+  const int sides = bidirectional ? 2 : 1;
+  if (num_buckets < 2 * sides || num_buckets > kMaxBuckets || num_buckets % sides != 0) return false;
+  if (max_distance <= num_buckets / sides / 2 || max_distance > kMaxDistance) return false;
+  // distances stay far inside 32 bits
+  const int limit = 1 << 29;
+  return heads > 0 && heads <= 65535 && q_len > 0 && q_len <= limit && k_len > 0 && k_len <= limit && q_start >= -limit && q_start <= limit;
+}
+
+struct GradSplit {
+  int groups, chunks;
+  long long parts;
+};
+GradSplit grad_split(int batch, int q_len, int k_len, int elem_bytes) {
+  GradSplit s;
+  const int v = 16 / elem_bytes;
+  s.chunks = (q_len + kGradRows - 1) / kGradRows;
+  const long long diagonals = static_cast<long long>(k_len) + (q_len < kGradRows ? q_len : kGradRows) + 2 * v;
+  s.groups = static_cast<int>((diagonals + kGradThreads * v - 1) / (kGradThreads * v));
+  s.parts = static_cast<long long>(batch) * s.chunks * s.groups;
+  return s;
+}
+
+template <typename T, int M>
+cudaError_t launch_grad(const GradArgs& a, cudaStream_t stream) {
+  return launch_pdl(relative_bias_grad_kernel<T, M>, dim3(static_cast<unsigned>(a.groups) * a.chunks, a.heads, a.batch), dim3(kGradThreads),
+                    0, stream, a);
+}
+
+template <typename T, typename TableT>
+cudaError_t launch_bias(BiasArgs a, cudaStream_t stream) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  a.cols = a.k_len < 1024 ? a.k_len : 1024;
+  a.rows = a.q_len < 64 ? a.q_len : 64;
+  const size_t smem = static_cast<size_t>(V) * ((a.rows + a.cols + 2 * V - 1) / V * V) * sizeof(T);
+  const long long tiles_q = (a.q_len + a.rows - 1) / a.rows;
+  if (tiles_q > 65535) return cudaErrorInvalidValue;
+  return launch_pdl(relative_bias_kernel<T, TableT>, dim3((a.k_len + a.cols - 1) / a.cols, static_cast<unsigned>(tiles_q), a.heads),
+                    dim3(kBiasThreads), smem, stream, a);
+}
+
+}  // namespace
+
+}  // namespace bt
+
+using namespace bt;
+
+extern "C" {
+
+int bt_relative_position_bias(const void* table, int table_fp32, int num_buckets, int max_distance, int bidirectional,
+                              int head_num, int q_len, int k_len, int q_start, void* out, int out_fp32, void* stream) {
+  if (!table || !out || (reinterpret_cast<uintptr_t>(out) & 15u) != 0) return BT_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(table) & (table_fp32 ? 3u : 1u)) != 0) return BT_ERR_INVALID_ARG;
+  if (!bias_shape_ok(num_buckets, max_distance, bidirectional, head_num, q_len, k_len, q_start)) return BT_ERR_INVALID_ARG;
+  BiasArgs a;
+  a.table = table;
+  a.out = out;
+  a.heads = head_num;
+  a.q_len = q_len;
+  a.k_len = k_len;
+  a.q_start = q_start;
+  bucket_borders(&a.borders, num_buckets, max_distance, bidirectional);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (out_fp32)
+    e = table_fp32 ? launch_bias<float, float>(a, s) : launch_bias<float, __half>(a, s);
+  else
+    e = table_fp32 ? launch_bias<__half, float>(a, s) : launch_bias<__half, __half>(a, s);
+  if (e == cudaErrorInvalidValue) return BT_ERR_INVALID_ARG;
+  return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;
+}
+
+int bt_relative_position_bias_grad_workspace(int grad_fp32, int num_buckets, int batch, int head_num, int q_len, int k_len,
+                                             size_t* bytes) {
+  if (!bytes || batch <= 0 || batch > 65535) return BT_ERR_INVALID_ARG;
+  if (!bias_shape_ok(num_buckets, kMaxDistance, 0, head_num, q_len, k_len, 0)) return BT_ERR_INVALID_ARG;
+  const GradSplit s = grad_split(batch, q_len, k_len, grad_fp32 ? 4 : 2);
+  if (s.parts > 0x7fffffffLL) return BT_ERR_INVALID_ARG;
+  *bytes = static_cast<size_t>(s.parts) * head_num * num_buckets * 4;
+  return BT_OK;
+}
+
+int bt_relative_position_bias_grad(const void* grad, int grad_fp32, int num_buckets, int max_distance, int bidirectional,
+                                   int batch, int head_num, int q_len, int k_len, int q_start, float* grad_table,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (!grad || !grad_table || !workspace) return BT_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(grad) & 15u) != 0 || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0 ||
+      (reinterpret_cast<uintptr_t>(grad_table) & 3u) != 0)
+    return BT_ERR_INVALID_ARG;
+  if (!bias_shape_ok(num_buckets, max_distance, bidirectional, head_num, q_len, k_len, q_start)) return BT_ERR_INVALID_ARG;
+  size_t need = 0;
+  const int rc = bt_relative_position_bias_grad_workspace(grad_fp32, num_buckets, batch, head_num, q_len, k_len, &need);
+  if (rc != BT_OK) return rc;
+  if (workspace_bytes < need) return BT_ERR_WORKSPACE;
+  const GradSplit split = grad_split(batch, q_len, k_len, grad_fp32 ? 4 : 2);
+  GradArgs a;
+  a.grad = grad;
+  a.partial = reinterpret_cast<float*>(workspace);
+  a.batch = batch;
+  a.heads = head_num;
+  a.q_len = q_len;
+  a.k_len = k_len;
+  a.q_start = q_start;
+  a.groups = split.groups;
+  a.chunks = split.chunks;
+  a.parts = static_cast<int>(split.parts);
+  bucket_borders(&a.borders, num_buckets, max_distance, bidirectional);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaErrorInvalidValue;
+  if (grad_fp32) {
+    switch (k_len % 4) {
+      case 0: e = launch_grad<float, 0>(a, s); break;
+      case 1: e = launch_grad<float, 1>(a, s); break;
+      case 2: e = launch_grad<float, 2>(a, s); break;
+      case 3: e = launch_grad<float, 3>(a, s); break;
+    }
+  } else {
+    switch (k_len % 8) {
+      case 0: e = launch_grad<__half, 0>(a, s); break;
+      case 1: e = launch_grad<__half, 1>(a, s); break;
+      case 2: e = launch_grad<__half, 2>(a, s); break;
+      case 3: e = launch_grad<__half, 3>(a, s); break;
+      case 4: e = launch_grad<__half, 4>(a, s); break;
+      case 5: e = launch_grad<__half, 5>(a, s); break;
+      case 6: e = launch_grad<__half, 6>(a, s); break;
+      case 7: e = launch_grad<__half, 7>(a, s); break;
+    }
+  }
+  if (e == cudaSuccess)
+    e = launch_pdl(relative_bias_grad_join_kernel, dim3((head_num * num_buckets + 7) / 8), dim3(256), 0, s,
+                   static_cast<const float*>(a.partial), grad_table, head_num, num_buckets, a.parts);
+  return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;
+}
+
+}  // extern "C"

@@ -480,6 +480,130 @@ def masked_softmax_(logits, attr_mask, scale=1.0):
     return logits
 
 
+def _half_or_float(t: torch.Tensor, name: str, device=None) -> int:
+    """1 for fp32, 0 for fp16; anything else is refused.  `device`: where the call's other tensors are."""
+    _check(t, name)
+    if t.dtype not in (torch.float16, torch.float32):
+        raise RuntimeError(f"{name} must be fp16 or fp32")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, the other tensors are on {device}")
+    return int(t.dtype == torch.float32)
+
+
+def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_distance: int = 128,
+                           bidirectional: bool = True, q_start: int = 0,
+                           out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """[heads, q_len, k_len] = table[bucket(k - (q + q_start)), head]: the learned bias by buckets of distance, as
+    Encoder.forward_general takes it (fp16) or, with q_len = 1 and out_dtype float32, by distance as window_attention
+    does.  table [num_buckets, heads] fp16 or fp32; the buckets are those of bt_relative_position_bias."""
+    fp32 = _half_or_float(table, "table")
+    if table.dim() != 2:
+        raise RuntimeError("table must be [num_buckets, heads]")
+    if out_dtype not in (torch.float16, torch.float32):
+        raise RuntimeError("out_dtype must be torch.float16 or torch.float32")
+    buckets, heads = table.shape
+    if q_len == 0 or k_len == 0:
+        return torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
+    lib = _abi.load()
+    with torch.cuda.device(table.device):
+        out = torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
+        rc = lib.bt_relative_position_bias(table.data_ptr(), fp32, buckets, int(max_distance), int(bool(bidirectional)),
+                                           heads, q_len, k_len, int(q_start), out.data_ptr(),
+                                           int(out_dtype == torch.float32), _stream_ptr(table.device))
+    if rc != _abi.BT_OK:
+        raise _abi.BtError(rc, "bt_relative_position_bias")
+    return out
+
+
+def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_distance: int = 128,
+                                bidirectional: bool = True, q_start: int = 0) -> torch.Tensor:
+    """The gradient of relative_position_bias: [num_buckets, heads] fp32 from that of the bias, [heads, q, k], or of the
+    scores of several sequences that one bias was added to, [batch, heads, q, k]; fp16 or fp32."""
+    fp32 = _half_or_float(grad, "grad")
+    if grad.dim() not in (3, 4):
+        raise RuntimeError("grad must be [heads, q_len, k_len] or [batch, heads, q_len, k_len]")
+    batch = int(grad.shape[0]) if grad.dim() == 4 else 1
+    heads, q_len, k_len = grad.shape[-3:]
+    if grad.numel() == 0:
+        return torch.zeros(num_buckets, heads, dtype=torch.float32, device=grad.device)
+    lib = _abi.load()
+    with torch.cuda.device(grad.device):
+        n = C.c_size_t()
+        rc = lib.bt_relative_position_bias_grad_workspace(fp32, int(num_buckets), batch, heads, q_len, k_len, C.byref(n))
+        if rc != _abi.BT_OK:
+            raise _abi.BtError(rc, "bt_relative_position_bias_grad_workspace")
+        out = torch.empty(num_buckets, heads, dtype=torch.float32, device=grad.device)
+        ws = torch.empty(n.value, dtype=torch.int8, device=grad.device)
+        rc = lib.bt_relative_position_bias_grad(grad.data_ptr(), fp32, int(num_buckets), int(max_distance),
+                                                int(bool(bidirectional)), batch, heads, q_len, k_len, int(q_start),
+                                                out.data_ptr(), ws.data_ptr(), n.value, _stream_ptr(grad.device))
+    if rc != _abi.BT_OK:
+        raise _abi.BtError(rc, "bt_relative_position_bias_grad")
+    return out
+
+
+def _rmsnorm_args(x, residual, gamma, m_dev):
+    x_fp32 = _half_or_float(x, "x")
+    gamma_fp32 = _half_or_float(gamma, "gamma", x.device)
+    if x.dim() != 2 or gamma.dim() != 1 or gamma.shape[0] != x.shape[1]:
+        raise RuntimeError("x must be [rows, hidden] and gamma [hidden]")
+    if residual is not None:
+        _check(residual, "residual", torch.float16)
+        if residual.shape != x.shape or residual.device != x.device:
+            raise RuntimeError("residual must be fp16 of x's shape, on x's device")
+    if m_dev is not None:
+        _check(m_dev, "m_dev", torch.int32)
+        if m_dev.device != x.device or m_dev.numel() < 1:
+            raise RuntimeError("m_dev must be one int32 on x's device")
+    return x_fp32, gamma_fp32
+
+
+def add_residual_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], gamma: torch.Tensor, eps: float = 1e-6,
+                         m_dev: Optional[torch.Tensor] = None):
+    """(out, sum): sum = x + residual (fp16, the next residual; None without a residual), out = sum / rms(sum) * gamma,
+    fp16.  Rows from *m_dev on are left unwritten."""
+    x_fp32, gamma_fp32 = _rmsnorm_args(x, residual, gamma, m_dev)
+    rows, hidden = x.shape
+    lib = _abi.load()
+    with torch.cuda.device(x.device):
+        out = torch.empty(rows, hidden, dtype=torch.float16, device=x.device)
+        total = torch.empty_like(out) if residual is not None else None
+        if rows == 0:
+            return out, total
+        rc = lib.bt_add_residual_rmsnorm(x.data_ptr(), x_fp32, residual.data_ptr() if residual is not None else None,
+                                         gamma.data_ptr(), gamma_fp32, total.data_ptr() if total is not None else None,
+                                         out.data_ptr(), m_dev.data_ptr() if m_dev is not None else None, rows, hidden,
+                                         eps, _stream_ptr(x.device))
+    if rc != _abi.BT_OK:
+        raise _abi.BtError(rc, "bt_add_residual_rmsnorm")
+    return out, total
+
+
+def add_residual_rmsnorm_e4m3(x: torch.Tensor, residual: Optional[torch.Tensor], gamma: torch.Tensor, eps: float = 1e-6,
+                              group: int = 0, m_dev: Optional[torch.Tensor] = None):
+    """(out, scales, sum): add_residual_rmsnorm with the result in 8 bits, out float8_e4m3fn and fp32 scales with
+    out * scales = the norm: one to a row ([rows, 1], group = 0) or to 128 columns ([rows, ceil(hidden/128)], group = 128)."""
+    x_fp32, gamma_fp32 = _rmsnorm_args(x, residual, gamma, m_dev)
+    if group not in (0, 128):
+        raise RuntimeError("group must be 0 (a scale per row) or 128 (a scale per 128 columns)")
+    rows, hidden = x.shape
+    lib = _abi.load()
+    with torch.cuda.device(x.device):
+        out = torch.empty(rows, hidden, dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty(rows, (hidden + 127) // 128 if group else 1, dtype=torch.float32, device=x.device)
+        total = torch.empty(rows, hidden, dtype=torch.float16, device=x.device) if residual is not None else None
+        if rows == 0:
+            return out, scales, total
+        rc = lib.bt_add_residual_rmsnorm_e4m3(x.data_ptr(), x_fp32, residual.data_ptr() if residual is not None else None,
+                                              gamma.data_ptr(), gamma_fp32,
+                                              total.data_ptr() if total is not None else None, out.data_ptr(),
+                                              scales.data_ptr(), group, m_dev.data_ptr() if m_dev is not None else None,
+                                              rows, hidden, eps, _stream_ptr(x.device))
+    if rc != _abi.BT_OK:
+        raise _abi.BtError(rc, "bt_add_residual_rmsnorm_e4m3")
+    return out, scales, total
+
+
 def bert_transformer(head_num: int, head_size: int,
                      qkv_kernel, qkv_bias, attr_output_kernel, attr_output_bias,
                      attr_output_layernorm_gamma, attr_output_layernorm_beta,

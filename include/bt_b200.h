@@ -302,6 +302,47 @@ int bt_add_bias_gelu(void* x, const void* bias, const int* m_dev, int m_rows, in
 int bt_masked_softmax(void* logits, const void* attr_mask, int batch_size, int head_num, int seq_len,
                       float scale, void* stream);
 
+/* ---- relative positions, pre-norm, local attention ------------------------- */
+/* No counterpart in the reference, which takes a finished `attention_bias` only (bytetransformer/include/softmax.h:41-45).
+ * bt_relative_position_bias makes one from a learned table:
+ *     out[h,q,k] = table[bucket(k - (q + q_start)), h],   q < q_len, k < k_len
+ *   table [num_buckets, head_num] fp16 or fp32 (table_fp32), out [head_num, q_len, k_len] fp16 or fp32 (out_fp32), 16-byte
+ *   aligned.  fp16 with q_len = k_len = seq_len and q_start = 0 is the `attention_bias` of
+ *   bt_stack_forward_padded_general; q_len = 1 gives the row of a single token at position q_start, and q_len = 1,
+ *   k_len = left + 1 + right, q_start = left the values by distance that bt_window_attention takes (fp32 there).
+ *   Buckets of a distance d: bidirectional != 0: the first half of the buckets for n = -d >= 0, the second for n = d > 0;
+ *   else all of them for n = max(-d, 0).  Of a side's m buckets the first e = m / 2 hold one distance each; then
+ *   min(m - 1, e + floor((m - e) * log(n / e) / log(max_distance / e))), exact in whole numbers.
+ *   num_buckets <= 256, even if bidirectional, at least 2 to a side; e < max_distance <= 2^20; lengths and q_start
+ *   up to 2^29; q_len <= 64 * 65535.
+ * bt_relative_position_bias_grad is its gradient, also where one bias was added to the scores of `batch` sequences:
+ *     grad_table[b,h] = sum of grad[i,h,q,k] over i, q, k with bucket(k - (q + q_start)) = b
+ *   grad [batch, head_num, q_len, k_len] fp16 or fp32, 16-byte aligned; grad_table [num_buckets, head_num] fp32, every
+ *   element written.  Sums in single precision over at most 128 rows, in double beyond; the same bits every time (no
+ *   atomics).  batch <= 65535.  `workspace`: bt_relative_position_bias_grad_workspace() bytes, 16-byte aligned,
+ *   contents undefined before and after; calls that may overlap need one each. */
+int bt_relative_position_bias(const void* table, int table_fp32, int num_buckets, int max_distance, int bidirectional,
+                              int head_num, int q_len, int k_len, int q_start, void* out, int out_fp32, void* stream);
+int bt_relative_position_bias_grad_workspace(int grad_fp32, int num_buckets, int batch, int head_num, int q_len, int k_len,
+                                             size_t* bytes);
+int bt_relative_position_bias_grad(const void* grad, int grad_fp32, int num_buckets, int max_distance, int bidirectional,
+                                   int batch, int head_num, int q_len, int k_len, int q_start, float* grad_table,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm beside bt_add_bias_residual_layernorm():  s = x + residual,
+ *     out = s / sqrt(mean(s^2) + eps) * gamma    over rows [0, min(*m_dev, m_rows)); other rows are left as they are.
+ *   x fp16 or fp32 [m_rows, hidden] (x_fp32); residual fp16 or NULL; gamma fp16 or fp32; sum_out fp16 or NULL: s, the
+ *   next residual (the statistics are those of the unrounded s, whose squares must sum to a finite fp32).  out fp16, or e4m3 with
+ *     scale = max(max|y|, 2^-100) / 448,  out = y / scale (y: the fp16 form's result before rounding)
+ *   for each row (group = 0, scales float[m_rows]) or each 128 columns of a row, the last of which may be fewer (group =
+ *   128, scales float[m_rows, ceil(hidden / 128)]).  hidden % 8 == 0, <= 16384; pointers 16-byte aligned (m_dev, scales: 4).
+ *   sum_out may be x (fp16) or residual, and out may be x (fp16), element for element; m_dev may be NULL. */
+int bt_add_residual_rmsnorm(const void* x, int x_fp32, const void* residual, const void* gamma, int gamma_fp32, void* sum_out,
+                            void* out, const int* m_dev, int m_rows, int hidden, float eps, void* stream);
+int bt_add_residual_rmsnorm_e4m3(const void* x, int x_fp32, const void* residual, const void* gamma, int gamma_fp32,
+                                 void* sum_out, void* out, float* scales, int group, const int* m_dev, int m_rows, int hidden,
+                                 float eps, void* stream);
+
 /* ---- launch accounting and per-kernel timing ------------------------------ */
 /* Kernel kinds of the arrays below (one slot per kind, BT_PROF_KINDS slots). */
 #define BT_PROF_OFFSETS 0
