@@ -139,11 +139,23 @@ __global__ void __launch_bounds__(kBiasThreads) relative_bias_kernel(const __gri
   __syncthreads();
   // diagonal x of the tile: distance of its last row's first element, plus x
   const int d0 = k0 - (q0 + rows - 1) - a.q_start;
-  for (int x = threadIdx.x; x < diagonals; x += kBiasThreads) {
-    const T v = column[bucket_of(d0 + x, a.borders, first)];
+  for (int x = threadIdx.x; x < diagonals; x += kBiasThreads) copies[x] = column[bucket_of(d0 + x, a.borders, first)];
+  __syncthreads();
+  for (int y = threadIdx.x; y < pitch / V - 1; y += kBiasThreads) {  // the shifted copies, a vector at a time
+    const uint4 lo = reinterpret_cast<const uint4*>(copies)[y], hi = reinterpret_cast<const uint4*>(copies)[y + 1];
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-    for (int p = 0; p < V; ++p)
-      if (x >= p) copies[p * pitch + x - p] = v;
+    for (int p = 1; p < V; ++p) {
+      uint32_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 4)
+          o[i] = w[i + p < 8 ? i + p : 7];
+        else
+          o[i] = (p & 1) ? __funnelshift_r(w[i + p / 2], w[i + p / 2 + 1], 16) : w[i + p / 2];
+      }
+      reinterpret_cast<uint4*>(copies + p * pitch)[y] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
   }
   fence_proxy_async_smem();
   __syncthreads();
@@ -153,7 +165,8 @@ __global__ void __launch_bounds__(kBiasThreads) relative_bias_kernel(const __gri
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out + static_cast<size_t>(r) * a.k_len) / sizeof(T));
     return min(static_cast<int>((V - at % V) % V), cols);
   };
-  for (int r = threadIdx.x; r < rows; r += kBiasThreads) {
+  // (the lanes of a warp issue their copies one after the other: the rows go round the warps)
+  for (int r = (threadIdx.x & 31) * (kBiasThreads / 32) + (threadIdx.x >> 5); r < rows; r += kBiasThreads) {
     const int lead = head_of(r);
     const int body = (cols - lead) / V * V;
     const int x = rows - 1 - r + lead;
@@ -161,13 +174,15 @@ __global__ void __launch_bounds__(kBiasThreads) relative_bias_kernel(const __gri
       bulk_store(out + static_cast<size_t>(r) * a.k_len + lead, copies + (x % V) * pitch + x / V * V, static_cast<uint32_t>(body * sizeof(T)));
   }
   tma_store_commit();
-  // the ragged ends of the rows, 2 V - 2 elements at most: 2 V lanes for each row
-  for (int i = threadIdx.x; i < rows * 2 * V; i += kBiasThreads) {
-    const int r = i / (2 * V), s = i % (2 * V);
-    const int lead = head_of(r);
-    const int body = (cols - lead) / V * V;
-    const int c = s < V ? s : lead + body + s - V;
-    if (s < V ? c < lead : c < cols) out[static_cast<size_t>(r) * a.k_len + c] = copies[rows - 1 - r + c];
+  if (a.k_len % V != 0) {
+    // the ragged ends of the rows, 2 V - 2 elements at most: 2 V lanes for each row
+    for (int i = threadIdx.x; i < rows * 2 * V; i += kBiasThreads) {
+      const int r = i / (2 * V), s = i % (2 * V);
+      const int lead = head_of(r);
+      const int body = (cols - lead) / V * V;
+      const int c = s < V ? s : lead + body + s - V;
+      if (s < V ? c < lead : c < cols) out[static_cast<size_t>(r) * a.k_len + c] = copies[rows - 1 - r + c];
+    }
   }
   tma_store_wait_read();
 }
@@ -178,13 +193,13 @@ struct GradArgs {
   float* partial;    // [heads, buckets, parts]
   int batch, heads, q_len, k_len, q_start;
   int groups;  // CTAs side by side over a row chunk's diagonals
-  int chunks;  // row chunks
+  int chunks, chunk_rows;
   int parts;   // batch * chunks * groups
   Borders borders;
 };
 
 constexpr int kGradThreads = 256;
-constexpr int kGradRows = 128;  // rows of a chunk: the longest chain of single-precision additions
+constexpr int kGradRows = 128;  // rows of a chunk at most: the longest chain of single-precision additions
 
 // A CTA sums the diagonals of `kGradRows` rows of one plane (sequence, head), over a range of diagonals, then the
 // diagonals of each bucket.  A thread holds 2 V - 1 diagonals (V = elements of 16 bytes) in registers and walks down them,
@@ -195,28 +210,31 @@ constexpr int kGradRows = 128;  // rows of a chunk: the longest chain of single-
 template <typename T, int M>
 __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const __grid_constant__ GradArgs a) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  constexpr int kSpan = kGradThreads * V;
-  __shared__ float low[kSpan + V], high[kSpan + V];
-  __shared__ int first[kMaxBuckets + 1];
+  constexpr int kSpanMax = kGradThreads * V;
+  __shared__ float low[kSpanMax + V], high[kSpanMax + V];
+  __shared__ int first[kMaxBuckets];
   pdl_launch_dependents();
   const int t = threadIdx.x;
-  for (int i = t; i < a.borders.count; i += kGradThreads) first[i] = a.borders.first[i];
-  if (t == 0) first[a.borders.count] = 0x7fffffff;
+  const int span = blockDim.x * V;
+  for (int i = t; i < a.borders.count; i += blockDim.x) first[i] = a.borders.first[i];
   const int group = blockIdx.x % a.groups;
   const int chunk = blockIdx.x / a.groups;
   const int head = blockIdx.y;
   const int item = blockIdx.z;
-  const int q0 = chunk * kGradRows;
-  const int q1 = min(q0 + kGradRows, a.q_len);
-  const size_t plane = (static_cast<size_t>(item) * a.heads + head) * a.q_len * a.k_len;
+  const int q0 = chunk * a.chunk_rows;
+  const int q1 = min(q0 + a.chunk_rows, a.q_len);
+  const size_t plane_elems = static_cast<size_t>(a.q_len) * a.k_len;
+  const size_t plane = (static_cast<size_t>(item) * a.heads + head) * plane_elems;
+  const size_t left = (static_cast<size_t>(a.batch) * a.heads) * plane_elems - plane;  // elements from the plane on
   const T* base = reinterpret_cast<const T*>(a.grad) + plane;
+  const bool last = left == plane_elems && q0 + a.chunk_rows >= a.q_len;
   // The range's first diagonal, as column minus row: the chunk's leftmost one, -(q1 - 1), rounded down so that the vectors
   // of the rows q0, q0 + V, ... are aligned in it (their columns are that diagonal plus the row).
   const int phase = static_cast<int>((plane + static_cast<size_t>(q0) * a.k_len) % V);  // elements of row q0 past a boundary
   const int leftmost = q0 - (q1 - 1);                                                   // as column, seen from row q0
   int c0 = leftmost - (V - 1) + phase;  // (a row's vectors start up to V - 1 diagonals further on)
   c0 = (c0 >= 0 ? c0 / V : -((-c0 + V - 1) / V)) * V - phase;                            // aligned column of row q0
-  c0 += group * kSpan + t * V;
+  c0 += group * span + t * V;
   float acc[2 * V - 1];
 #pragma unroll
   for (int i = 0; i < 2 * V - 1; ++i) acc[i] = 0.f;
@@ -224,26 +242,45 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
 #pragma unroll 1
   for (int q = q0, c = c0; q < q1; q += V, c += V) {
     if (c >= a.k_len || c + 3 * V - 2 <= 0) continue;  // the V vectors lie in columns c .. c + 3 V - 3
-    const bool inside = c >= 0 && c + 3 * V - 2 <= a.k_len && q + V <= q1;
+    const T* row = base + static_cast<size_t>(q) * a.k_len + c;
     uint4 v[V];
-    if (inside) {
 #pragma unroll
-      for (int r = 0; r < V; ++r) {
-        constexpr int kStep = M + 1;
-        const int shift = (V * kStep - r * kStep) % V;  // static: see above
-        v[r] = *reinterpret_cast<const uint4*>(base + static_cast<size_t>(q + r) * a.k_len + (c + r + shift));
-      }
-    } else {
-      for (int r = 0; r < V; ++r) {
-        constexpr int kStep = M + 1;
-        const int shift = (V * kStep - r * kStep) % V;
-        T e[V];
+    for (int r = 0; r < V; ++r) {
+      constexpr int kStep = M + 1;
+      const int shift = (V * kStep - r * kStep) % V;  // static: see above
+      const int col = c + r + shift;
+      v[r] = make_uint4(0u, 0u, 0u, 0u);
+      // (a vector that starts in the row before or ends in the row behind: blanked below)
+      if (q + r < q1 && col < a.k_len && col + V > 0) {
+        const T* at = row + r * a.k_len + (r + shift);
+        if (M == 0 || !last || static_cast<size_t>(at - base) + V <= left) {
+          v[r] = *reinterpret_cast<const uint4*>(at);
+        } else {  // past the end of the buffer: element by element
+          T e[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int col = c + r + shift + i;
-          e[i] = (q + r < q1 && col >= 0 && col < a.k_len) ? base[static_cast<size_t>(q + r) * a.k_len + col] : static_cast<T>(0.f);
+          for (int i = 0; i < V; ++i) e[i] = (col + i >= 0 && col + i < a.k_len) ? at[i] : static_cast<T>(0.f);
+          v[r] = *reinterpret_cast<const uint4*>(e);
         }
-        v[r] = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+    if (M != 0 && (c < 0 || c + 3 * V - 2 > a.k_len)) {
+#pragma unroll
+      for (int r = 0; r < V; ++r) {
+        constexpr int kStep = M + 1;
+        const int col = c + r + (V * kStep - r * kStep) % V;
+        if (col < 0 || col + V > a.k_len) {
+          // bit i: element i is in the row
+          const uint32_t in = (0xffu << max(-col, 0)) & (0xffu >> max(min(col + 8 - a.k_len, 8), 0));
+          uint32_t w[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (V == 8)
+              w[i] &= ((in >> (2 * i)) & 1u) * 0xffffu + ((in >> (2 * i + 1)) & 1u) * 0xffff0000u;
+            else
+              w[i] = (col + i >= 0 && col + i < a.k_len) ? w[i] : 0u;
+          }
+          v[r] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
     }
 #pragma unroll
@@ -270,32 +307,31 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       high[i] = 0.f;
-      low[kSpan + i] = 0.f;
+      low[span + i] = 0.f;
     }
   }
   __syncthreads();
-  // Distance of diagonal x: x + d_first.  A bucket is a run of distances; a warp sums a bucket's, in double precision: the
-  // runs are up to a range long.
+  // Distance of diagonal x: x + d_first.  A bucket is a run of diagonals, summed by a warp.
   const int d_first = c0 - t * V - q0 - a.q_start;
   const int total = a.borders.count * a.borders.sides;
   const int part = (item * a.chunks + chunk) * a.groups + group;
-  for (int b = t >> 5; b < total; b += kGradThreads / 32) {
-    const int i = b % a.borders.count;
-    long long lo, hi;  // distances of the bucket, inclusive
-    if (b >= a.borders.count) {
-      lo = max(first[i], 1);
-      hi = first[i + 1] - 1LL;
+  for (int b = t >> 5; b < total; b += blockDim.x / 32) {
+    const bool right = b >= a.borders.count;
+    const int i = right ? b - a.borders.count : b;
+    const bool outermost = i + 1 == a.borders.count;
+    int x0 = 0, x1 = span + V - 1;  // the run, inclusive
+    if (right) {
+      x0 = max(x0, max(first[i], 1) - d_first);
+      if (!outermost) x1 = min(x1, first[i + 1] - 1 - d_first);
     } else {
-      lo = i + 1 < a.borders.count ? 1LL - first[i + 1] : -0x7fffffffLL;
-      hi = (i == 0 && a.borders.sides == 1) ? 0x7fffffffLL : -static_cast<long long>(first[i]);
+      if (!outermost) x0 = max(x0, 1 - first[i + 1] - d_first);
+      if (i > 0 || a.borders.sides == 2) x1 = min(x1, -first[i] - d_first);
     }
-    const int x0 = static_cast<int>(max(lo - d_first, 0LL));
-    const int x1 = static_cast<int>(min(hi - d_first, static_cast<long long>(kSpan + V - 1)));
-    double sum = 0.0;
-    for (int x = x0 + (t & 31); x <= x1; x += 32) sum += static_cast<double>(low[x]) + static_cast<double>(high[x]);
+    float sum = 0.f;
+    for (int x = x0 + (t & 31); x <= x1; x += 32) sum += low[x] + high[x];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((t & 31) == 0) a.partial[(static_cast<size_t>(head) * total + b) * a.parts + part] = static_cast<float>(sum);
+    if ((t & 31) == 0) a.partial[(static_cast<size_t>(head) * total + b) * a.parts + part] = sum;
   }
 }
 
@@ -323,22 +359,28 @@ bool bias_shape_ok(int num_buckets, int max_distance, int bidirectional, int hea
 }
 
 struct GradSplit {
-  int groups, chunks;
+  int groups, chunks, chunk_rows;
+  int threads;  // of a CTA: no more than the diagonals ask for
   long long parts;
 };
-GradSplit grad_split(int batch, int q_len, int k_len, int elem_bytes) {
+GradSplit grad_split(int batch, int heads, int q_len, int k_len, int elem_bytes) {
   GradSplit s;
   const int v = 16 / elem_bytes;
-  s.chunks = (q_len + kGradRows - 1) / kGradRows;
-  const long long diagonals = static_cast<long long>(k_len) + (q_len < kGradRows ? q_len : kGradRows) + 2 * v;
-  s.groups = static_cast<int>((diagonals + kGradThreads * v - 1) / (kGradThreads * v));
+  // Chunks of 128 rows waste least (a chunk of R rows walks R diagonals more than the matrix has columns), but every CTA
+  // walks its rows one after the other: calls of few rows take shorter ones.
+  s.chunk_rows = kGradRows;
+  while (s.chunk_rows > 16 && static_cast<long long>(batch) * heads * ((q_len + s.chunk_rows - 1) / s.chunk_rows) < 4 * 148) s.chunk_rows /= 2;
+  s.chunks = (q_len + s.chunk_rows - 1) / s.chunk_rows;
+  const long long vectors = (static_cast<long long>(k_len) + (q_len < s.chunk_rows ? q_len : s.chunk_rows) + 3 * v - 1) / v;
+  s.groups = static_cast<int>((vectors + kGradThreads - 1) / kGradThreads);
+  s.threads = static_cast<int>(((vectors + s.groups - 1) / s.groups + 31) / 32 * 32);
   s.parts = static_cast<long long>(batch) * s.chunks * s.groups;
   return s;
 }
 
 template <typename T, int M>
-cudaError_t launch_grad(const GradArgs& a, cudaStream_t stream) {
-  return launch_pdl(relative_bias_grad_kernel<T, M>, dim3(static_cast<unsigned>(a.groups) * a.chunks, a.heads, a.batch), dim3(kGradThreads),
+cudaError_t launch_grad(const GradArgs& a, int threads, cudaStream_t stream) {
+  return launch_pdl(relative_bias_grad_kernel<T, M>, dim3(static_cast<unsigned>(a.groups) * a.chunks, a.heads, a.batch), dim3(threads),
                     0, stream, a);
 }
 
@@ -389,7 +431,7 @@ int bt_relative_position_bias_grad_workspace(int grad_fp32, int num_buckets, int
                                              size_t* bytes) {
   if (!bytes || batch <= 0 || batch > 65535) return BT_ERR_INVALID_ARG;
   if (!bias_shape_ok(num_buckets, kMaxDistance, 0, head_num, q_len, k_len, 0)) return BT_ERR_INVALID_ARG;
-  const GradSplit s = grad_split(batch, q_len, k_len, grad_fp32 ? 4 : 2);
+  const GradSplit s = grad_split(batch, head_num, q_len, k_len, grad_fp32 ? 4 : 2);
   if (s.parts > 0x7fffffffLL) return BT_ERR_INVALID_ARG;
   *bytes = static_cast<size_t>(s.parts) * head_num * num_buckets * 4;
   return BT_OK;
@@ -407,7 +449,7 @@ int bt_relative_position_bias_grad(const void* grad, int grad_fp32, int num_buck
   const int rc = bt_relative_position_bias_grad_workspace(grad_fp32, num_buckets, batch, head_num, q_len, k_len, &need);
   if (rc != BT_OK) return rc;
   if (workspace_bytes < need) return BT_ERR_WORKSPACE;
-  const GradSplit split = grad_split(batch, q_len, k_len, grad_fp32 ? 4 : 2);
+  const GradSplit split = grad_split(batch, head_num, q_len, k_len, grad_fp32 ? 4 : 2);
   GradArgs a;
   a.grad = grad;
   a.partial = reinterpret_cast<float*>(workspace);
@@ -418,27 +460,28 @@ int bt_relative_position_bias_grad(const void* grad, int grad_fp32, int num_buck
   a.q_start = q_start;
   a.groups = split.groups;
   a.chunks = split.chunks;
+  a.chunk_rows = split.chunk_rows;
   a.parts = static_cast<int>(split.parts);
   bucket_borders(&a.borders, num_buckets, max_distance, bidirectional);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = cudaErrorInvalidValue;
   if (grad_fp32) {
     switch (k_len % 4) {
-      case 0: e = launch_grad<float, 0>(a, s); break;
-      case 1: e = launch_grad<float, 1>(a, s); break;
-      case 2: e = launch_grad<float, 2>(a, s); break;
-      case 3: e = launch_grad<float, 3>(a, s); break;
+      case 0: e = launch_grad<float, 0>(a, split.threads, s); break;
+      case 1: e = launch_grad<float, 1>(a, split.threads, s); break;
+      case 2: e = launch_grad<float, 2>(a, split.threads, s); break;
+      case 3: e = launch_grad<float, 3>(a, split.threads, s); break;
     }
   } else {
     switch (k_len % 8) {
-      case 0: e = launch_grad<__half, 0>(a, s); break;
-      case 1: e = launch_grad<__half, 1>(a, s); break;
-      case 2: e = launch_grad<__half, 2>(a, s); break;
-      case 3: e = launch_grad<__half, 3>(a, s); break;
-      case 4: e = launch_grad<__half, 4>(a, s); break;
-      case 5: e = launch_grad<__half, 5>(a, s); break;
-      case 6: e = launch_grad<__half, 6>(a, s); break;
-      case 7: e = launch_grad<__half, 7>(a, s); break;
+      case 0: e = launch_grad<__half, 0>(a, split.threads, s); break;
+      case 1: e = launch_grad<__half, 1>(a, split.threads, s); break;
+      case 2: e = launch_grad<__half, 2>(a, split.threads, s); break;
+      case 3: e = launch_grad<__half, 3>(a, split.threads, s); break;
+      case 4: e = launch_grad<__half, 4>(a, split.threads, s); break;
+      case 5: e = launch_grad<__half, 5>(a, split.threads, s); break;
+      case 6: e = launch_grad<__half, 6>(a, split.threads, s); break;
+      case 7: e = launch_grad<__half, 7>(a, split.threads, s); break;
     }
   }
   if (e == cudaSuccess)

@@ -154,13 +154,14 @@ __global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32) a
   if (OUT == kRmsRowScale) {
     top = row_reduce<WARPS, true>(top, scratch[1]);
     const float scale = fmaxf(top, 0x1p-100f) / 448.0f;
+    const float inv = 1.0f / scale;
     if (t == 0) a.scales[row] = scale;
 #pragma unroll
     for (int i = 0; i < NVEC; ++i) {
       const int v = i * kLanes + t;
       if (v < nvec) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] / scale;
+        for (int j = 0; j < 8; ++j) s[i][j] *= inv;
         reinterpret_cast<uint2*>(a.out)[at + v] = pack8_e4m3(s[i]);
       }
     }
@@ -176,10 +177,11 @@ __global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32) a
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float scale = fmaxf(m, 0x1p-100f) / 448.0f;
+      const float inv = 1.0f / scale;
       if (v < nvec) {
         if ((t & 15) == 0) a.scales[static_cast<size_t>(row) * groups + (v >> 4)] = scale;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] / scale;
+        for (int j = 0; j < 8; ++j) s[i][j] *= inv;
         reinterpret_cast<uint2*>(a.out)[at + v] = pack8_e4m3(s[i]);
       }
     }

@@ -28,6 +28,26 @@ def _stream_ptr(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+class _On:
+    """`with torch.cuda.device(device)` that gives the device's current stream, for calls that last microseconds: nothing
+    is switched where the device is current already."""
+    __slots__ = ("index", "guard")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.guard = None
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def _check(t: torch.Tensor, name: str, dtype=None):
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
@@ -505,11 +525,11 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_d
     if q_len == 0 or k_len == 0:
         return torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
     lib = _abi.load()
-    with torch.cuda.device(table.device):
+    with _On(table.device) as stream:
         out = torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
         rc = lib.bt_relative_position_bias(table.data_ptr(), fp32, buckets, int(max_distance), int(bool(bidirectional)),
                                            heads, q_len, k_len, int(q_start), out.data_ptr(),
-                                           int(out_dtype == torch.float32), _stream_ptr(table.device))
+                                           int(out_dtype == torch.float32), stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_relative_position_bias")
     return out
@@ -527,7 +547,7 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
     if grad.numel() == 0:
         return torch.zeros(num_buckets, heads, dtype=torch.float32, device=grad.device)
     lib = _abi.load()
-    with torch.cuda.device(grad.device):
+    with _On(grad.device) as stream:
         n = C.c_size_t()
         rc = lib.bt_relative_position_bias_grad_workspace(fp32, int(num_buckets), batch, heads, q_len, k_len, C.byref(n))
         if rc != _abi.BT_OK:
@@ -536,7 +556,7 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
         ws = torch.empty(n.value, dtype=torch.int8, device=grad.device)
         rc = lib.bt_relative_position_bias_grad(grad.data_ptr(), fp32, int(num_buckets), int(max_distance),
                                                 int(bool(bidirectional)), batch, heads, q_len, k_len, int(q_start),
-                                                out.data_ptr(), ws.data_ptr(), n.value, _stream_ptr(grad.device))
+                                                out.data_ptr(), ws.data_ptr(), n.value, stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_relative_position_bias_grad")
     return out
@@ -565,7 +585,7 @@ def add_residual_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], gamm
     x_fp32, gamma_fp32 = _rmsnorm_args(x, residual, gamma, m_dev)
     rows, hidden = x.shape
     lib = _abi.load()
-    with torch.cuda.device(x.device):
+    with _On(x.device) as stream:
         out = torch.empty(rows, hidden, dtype=torch.float16, device=x.device)
         total = torch.empty_like(out) if residual is not None else None
         if rows == 0:
@@ -573,7 +593,7 @@ def add_residual_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], gamm
         rc = lib.bt_add_residual_rmsnorm(x.data_ptr(), x_fp32, residual.data_ptr() if residual is not None else None,
                                          gamma.data_ptr(), gamma_fp32, total.data_ptr() if total is not None else None,
                                          out.data_ptr(), m_dev.data_ptr() if m_dev is not None else None, rows, hidden,
-                                         eps, _stream_ptr(x.device))
+                                         eps, stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_add_residual_rmsnorm")
     return out, total
@@ -588,7 +608,7 @@ def add_residual_rmsnorm_e4m3(x: torch.Tensor, residual: Optional[torch.Tensor],
         raise RuntimeError("group must be 0 (a scale per row) or 128 (a scale per 128 columns)")
     rows, hidden = x.shape
     lib = _abi.load()
-    with torch.cuda.device(x.device):
+    with _On(x.device) as stream:
         out = torch.empty(rows, hidden, dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty(rows, (hidden + 127) // 128 if group else 1, dtype=torch.float32, device=x.device)
         total = torch.empty(rows, hidden, dtype=torch.float16, device=x.device) if residual is not None else None
@@ -598,7 +618,7 @@ def add_residual_rmsnorm_e4m3(x: torch.Tensor, residual: Optional[torch.Tensor],
                                               gamma.data_ptr(), gamma_fp32,
                                               total.data_ptr() if total is not None else None, out.data_ptr(),
                                               scales.data_ptr(), group, m_dev.data_ptr() if m_dev is not None else None,
-                                              rows, hidden, eps, _stream_ptr(x.device))
+                                              rows, hidden, eps, stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_add_residual_rmsnorm_e4m3")
     return out, scales, total

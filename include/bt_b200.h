@@ -318,8 +318,8 @@ int bt_masked_softmax(void* logits, const void* attr_mask, int batch_size, int h
  * bt_relative_position_bias_grad is its gradient, also where one bias was added to the scores of `batch` sequences:
  *     grad_table[b,h] = sum of grad[i,h,q,k] over i, q, k with bucket(k - (q + q_start)) = b
  *   grad [batch, head_num, q_len, k_len] fp16 or fp32, 16-byte aligned; grad_table [num_buckets, head_num] fp32, every
- *   element written.  Sums in single precision over at most 128 rows, in double beyond; the same bits every time (no
- *   atomics).  batch <= 65535.  `workspace`: bt_relative_position_bias_grad_workspace() bytes, 16-byte aligned,
+ *   element written.  Sums in single precision within a block of at most 128 rows, in double beyond; the same bits every
+ *   time (no atomics).  batch <= 65535.  `workspace`: bt_relative_position_bias_grad_workspace() bytes, 16-byte aligned,
  *   contents undefined before and after; calls that may overlap need one each. */
 int bt_relative_position_bias(const void* table, int table_fp32, int num_buckets, int max_distance, int bidirectional,
                               int head_num, int q_len, int k_len, int q_start, void* out, int out_fp32, void* stream);
