@@ -201,17 +201,20 @@ struct GradArgs {
 constexpr int kGradThreads = 256;
 constexpr int kGradRows = 128;  // rows of a chunk at most: the longest chain of single-precision additions
 
-// A CTA sums the diagonals of `kGradRows` rows of one plane (sequence, head), over a range of diagonals, then the
+// A CTA sums the diagonals of up to `kGradRows` rows of one plane (sequence, head), over a range of diagonals, then the
 // diagonals of each bucket.  A thread holds 2 V - 1 diagonals (V = elements of 16 bytes) in registers and walks down them,
 // V rows and one aligned 16-byte load per row at a time: with every row the matrix's next aligned vector lies
 // k_len + 1 elements further on relative to the diagonals, so the vector of row r starts (-r * (k_len + 1)) mod V diagonals
 // into the thread's range, a number that only k_len mod V (M) decides and that repeats every V rows.  So every index of
 // a register is known at compile time, whatever the row length, and neighbouring threads load neighbouring vectors.
+// Rows that do not start on a 16-byte boundary have up to V - 1 elements ahead of their first whole vector and behind
+// their last; those are summed by diagonal, a thread each, ahead of the walk.
 template <typename T, int M>
 __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const __grid_constant__ GradArgs a) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   constexpr int kSpanMax = kGradThreads * V;
-  __shared__ float low[kSpanMax + V], high[kSpanMax + V];
+  constexpr int kEdge = kGradRows + V;
+  __shared__ float low[kSpanMax + V], high[kSpanMax + V], block[kGradThreads + 1], edge[M != 0 ? 2 : 1][M != 0 ? kEdge : 1];
   __shared__ int first[kMaxBuckets];
   pdl_launch_dependents();
   const int t = threadIdx.x;
@@ -222,67 +225,70 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
   const int head = blockIdx.y;
   const int item = blockIdx.z;
   const int q0 = chunk * a.chunk_rows;
-  const int q1 = min(q0 + a.chunk_rows, a.q_len);
-  const size_t plane_elems = static_cast<size_t>(a.q_len) * a.k_len;
-  const size_t plane = (static_cast<size_t>(item) * a.heads + head) * plane_elems;
-  const size_t left = (static_cast<size_t>(a.batch) * a.heads) * plane_elems - plane;  // elements from the plane on
-  const T* base = reinterpret_cast<const T*>(a.grad) + plane;
-  const bool last = left == plane_elems && q0 + a.chunk_rows >= a.q_len;
-  // The range's first diagonal, as column minus row: the chunk's leftmost one, -(q1 - 1), rounded down so that the vectors
-  // of the rows q0, q0 + V, ... are aligned in it (their columns are that diagonal plus the row).
-  const int phase = static_cast<int>((plane + static_cast<size_t>(q0) * a.k_len) % V);  // elements of row q0 past a boundary
-  const int leftmost = q0 - (q1 - 1);                                                   // as column, seen from row q0
-  int c0 = leftmost - (V - 1) + phase;  // (a row's vectors start up to V - 1 diagonals further on)
-  c0 = (c0 >= 0 ? c0 / V : -((-c0 + V - 1) / V)) * V - phase;                            // aligned column of row q0
-  c0 += group * span + t * V;
+  const int rows = min(a.chunk_rows, a.q_len - q0);
+  const int k_len = a.k_len;
+  const size_t start = ((static_cast<size_t>(item) * a.heads + head) * a.q_len + q0) * k_len;  // element of row q0
+  const T* base = reinterpret_cast<const T*>(a.grad) + start;
+  // Diagonals are counted as the column of row q0 that they pass.  The range's first one: the leftmost, -(rows - 1),
+  // rounded down so that the vectors of the rows q0, q0 + V, ... are aligned there (and V - 1 earlier: a row's vectors start up
+  // to that many diagonals further on).
+  const int phase = static_cast<int>(start % V);  // elements of row q0 past a boundary
+  const int leftmost = -(rows - 1) - (V - 1) + phase;
+  const int c_first = -((-leftmost + V - 1) / V) * V - phase + group * span;  // (leftmost <= 0)
+  const int c0 = c_first + t * V;
+  pdl_wait();
+  if constexpr (M != 0) {
+    // elements of row r (from q0) ahead of its first boundary
+    auto lead_of = [&](int r) { return min((V - static_cast<int>((phase + static_cast<unsigned>(r) * M) % V)) % V, k_len); };
+    for (int x = t; x < 2 * kEdge; x += blockDim.x) {
+      const bool right = x >= kEdge;
+      // diagonal -(rows - 1) + x on the left, k_len - V + 1 - (rows - 1) + x on the right
+      const int d = (right ? k_len - V + 1 + x - kEdge : x) - (rows - 1);
+      T e[V - 1];
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i) {
+        const int col = right ? k_len - 1 - i : i;
+        const int r = col - d;
+        bool take = r >= 0 && r < rows && col >= 0 && col < k_len;
+        if (take) {
+          const int lead = lead_of(r);
+          take = right ? col >= lead + (k_len - lead) / V * V : col < lead;
+        }
+        e[i] = take ? base[static_cast<size_t>(r) * k_len + col] : static_cast<T>(0.f);
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < V - 1; ++i) sum += static_cast<float>(e[i]);
+      edge[right][right ? x - kEdge : x] = sum;
+    }
+  }
   float acc[2 * V - 1];
 #pragma unroll
   for (int i = 0; i < 2 * V - 1; ++i) acc[i] = 0.f;
-  pdl_wait();
-#pragma unroll 1
-  for (int q = q0, c = c0; q < q1; q += V, c += V) {
-    if (c >= a.k_len || c + 3 * V - 2 <= 0) continue;  // the V vectors lie in columns c .. c + 3 V - 3
-    const T* row = base + static_cast<size_t>(q) * a.k_len + c;
-    uint4 v[V];
-#pragma unroll
-    for (int r = 0; r < V; ++r) {
-      constexpr int kStep = M + 1;
-      const int shift = (V * kStep - r * kStep) % V;  // static: see above
-      const int col = c + r + shift;
-      v[r] = make_uint4(0u, 0u, 0u, 0u);
-      // (a vector that starts in the row before or ends in the row behind: blanked below)
-      if (q + r < q1 && col < a.k_len && col + V > 0) {
-        const T* at = row + r * a.k_len + (r + shift);
-        if (M == 0 || !last || static_cast<size_t>(at - base) + V <= left) {
-          v[r] = *reinterpret_cast<const uint4*>(at);
-        } else {  // past the end of the buffer: element by element
-          T e[V];
-#pragma unroll
-          for (int i = 0; i < V; ++i) e[i] = (col + i >= 0 && col + i < a.k_len) ? at[i] : static_cast<T>(0.f);
-          v[r] = *reinterpret_cast<const uint4*>(e);
-        }
-      }
-    }
-    if (M != 0 && (c < 0 || c + 3 * V - 2 > a.k_len)) {
+  // One step: V rows, a whole vector of each.
+  auto load = [&](uint4 (&v)[V], int n) {
+    const int c = c0 + n * V;
+    const T* row = base + static_cast<size_t>(n * V) * k_len + c;
+    // the V vectors lie in columns c .. c + 3 V - 3
+    if (c >= 0 && c + 3 * V - 2 <= k_len && n * V + V <= rows) {
 #pragma unroll
       for (int r = 0; r < V; ++r) {
         constexpr int kStep = M + 1;
-        const int col = c + r + (V * kStep - r * kStep) % V;
-        if (col < 0 || col + V > a.k_len) {
-          // bit i: element i is in the row
-          const uint32_t in = (0xffu << max(-col, 0)) & (0xffu >> max(min(col + 8 - a.k_len, 8), 0));
-          uint32_t w[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+        v[r] = *reinterpret_cast<const uint4*>(row + r * static_cast<ptrdiff_t>(k_len) + (r + (V * kStep - r * kStep) % V));
+      }
+    } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (V == 8)
-              w[i] &= ((in >> (2 * i)) & 1u) * 0xffffu + ((in >> (2 * i + 1)) & 1u) * 0xffff0000u;
-            else
-              w[i] = (col + i >= 0 && col + i < a.k_len) ? w[i] : 0u;
-          }
-          v[r] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+      for (int r = 0; r < V; ++r) {
+        constexpr int kStep = M + 1;
+        const int shift = (V * kStep - r * kStep) % V;  // static: see above
+        const int col = c + r + shift;
+        v[r] = make_uint4(0u, 0u, 0u, 0u);
+        if (n * V + r < rows && col >= 0 && col + V <= k_len)
+          v[r] = *reinterpret_cast<const uint4*>(row + r * static_cast<ptrdiff_t>(k_len) + (r + shift));
       }
     }
+  };
+  auto add = [&](const uint4 (&v)[V]) {
 #pragma unroll
     for (int r = 0; r < V; ++r) {
       constexpr int kStep = M + 1;
@@ -295,6 +301,23 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
         else
           acc[shift + i] += __uint_as_float(w[i]);
       }
+    }
+  };
+  // The steps of this thread: those whose vectors have a column in the matrix.  The next one's loads are out before this
+  // one's values are added.
+  const int n0 = c0 + 3 * V - 2 > 0 ? 0 : (-(c0 + 3 * V - 2)) / V + 1;
+  const int n1 = min((rows + V - 1) / V, c0 < k_len ? (k_len - 1 - c0) / V + 1 : 0);
+  if (n0 < n1) {
+    uint4 v[V], w[V];
+    load(v, n0);
+#pragma unroll 1
+    for (int n = n0; n < n1; n += 2) {
+      const bool more = n + 1 < n1;
+      if (more) load(w, n + 1);
+      add(v);
+      if (!more) break;
+      if (n + 2 < n1) load(v, n + 2);
+      add(w);
     }
   }
   // Diagonal t * V + i of the range: the thread's own first V in `low`, what it holds of its right neighbour's in `high`
@@ -311,27 +334,59 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
     }
   }
   __syncthreads();
-  // Distance of diagonal x: x + d_first.  A bucket is a run of diagonals, summed by a warp.
-  const int d_first = c0 - t * V - q0 - a.q_start;
+  // The diagonals' sums, in `low`, and those of V diagonals each, which the long runs below take.
+  for (int g = t; g <= static_cast<int>(blockDim.x); g += blockDim.x) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int x = g * V + i;
+      float d = low[x] + high[x];
+      if constexpr (M != 0) {
+        if (x < span) {  // (the rest of the range is the next group's too)
+          const int l = c_first + x + (rows - 1), r = l - (k_len - V + 1);
+          if (l >= 0 && l < kEdge) d += edge[0][l];
+          if (r >= 0 && r < kEdge) d += edge[1][r];
+        }
+      }
+      low[x] = d;
+      sum += d;
+    }
+    block[g] = sum;
+  }
+  __syncthreads();
+  // Distance of diagonal x: x + d_first.  A bucket is a run of diagonals, summed by eight lanes.
+  const int d_first = c_first - q0 - a.q_start;
   const int total = a.borders.count * a.borders.sides;
   const int part = (item * a.chunks + chunk) * a.groups + group;
-  for (int b = t >> 5; b < total; b += blockDim.x / 32) {
-    const bool right = b >= a.borders.count;
-    const int i = right ? b - a.borders.count : b;
-    const bool outermost = i + 1 == a.borders.count;
-    int x0 = 0, x1 = span + V - 1;  // the run, inclusive
-    if (right) {
-      x0 = max(x0, max(first[i], 1) - d_first);
-      if (!outermost) x1 = min(x1, first[i + 1] - 1 - d_first);
-    } else {
-      if (!outermost) x0 = max(x0, 1 - first[i + 1] - d_first);
-      if (i > 0 || a.borders.sides == 2) x1 = min(x1, -first[i] - d_first);
-    }
+  const int sub = t & 7;
+  for (int b0 = (t >> 5) * 4; b0 < total; b0 += blockDim.x / 8) {
+    const int b = b0 + ((t >> 3) & 3);
     float sum = 0.f;
-    for (int x = x0 + (t & 31); x <= x1; x += 32) sum += low[x] + high[x];
+    if (b < total) {
+      const bool right = b >= a.borders.count;
+      const int i = right ? b - a.borders.count : b;
+      const bool outermost = i + 1 == a.borders.count;
+      int x0 = 0, x1 = span + V;  // the run: x0 <= x < x1
+      if (right) {
+        x0 = max(x0, max(first[i], 1) - d_first);
+        if (!outermost) x1 = min(x1, first[i + 1] - d_first);
+      } else {
+        if (!outermost) x0 = max(x0, 1 - first[i + 1] - d_first);
+        if (i > 0 || a.borders.sides == 2) x1 = min(x1, 1 - first[i] - d_first);
+      }
+      // ragged ends element by element, what lies between by blocks
+      const int g0 = (x0 + V - 1) / V, g1 = x1 / V;
+      if (x0 < x1 && g0 < g1) {
+        for (int x = x0 + sub; x < g0 * V; x += 8) sum += low[x];
+        for (int g = g0 + sub; g < g1; g += 8) sum += block[g];
+        for (int x = g1 * V + sub; x < x1; x += 8) sum += low[x];
+      } else {
+        for (int x = x0 + sub; x < x1; x += 8) sum += low[x];
+      }
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((t & 31) == 0) a.partial[(static_cast<size_t>(head) * total + b) * a.parts + part] = sum;
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (sub == 0 && b < total) a.partial[(static_cast<size_t>(head) * total + b) * a.parts + part] = sum;
   }
 }
 
@@ -369,7 +424,7 @@ GradSplit grad_split(int batch, int heads, int q_len, int k_len, int elem_bytes)
   // Chunks of 128 rows waste least (a chunk of R rows walks R diagonals more than the matrix has columns), but every CTA
   // walks its rows one after the other: calls of few rows take shorter ones.
   s.chunk_rows = kGradRows;
-  while (s.chunk_rows > 16 && static_cast<long long>(batch) * heads * ((q_len + s.chunk_rows - 1) / s.chunk_rows) < 4 * 148) s.chunk_rows /= 2;
+  while (s.chunk_rows > 16 && static_cast<long long>(batch) * heads * ((q_len + s.chunk_rows - 1) / s.chunk_rows) < 2 * 148) s.chunk_rows /= 2;
   s.chunks = (q_len + s.chunk_rows - 1) / s.chunk_rows;
   const long long vectors = (static_cast<long long>(k_len) + (q_len < s.chunk_rows ? q_len : s.chunk_rows) + 3 * v - 1) / v;
   s.groups = static_cast<int>((vectors + kGradThreads - 1) / kGradThreads);
@@ -387,7 +442,7 @@ cudaError_t launch_grad(const GradArgs& a, int threads, cudaStream_t stream) {
 template <typename T, typename TableT>
 cudaError_t launch_bias(BiasArgs a, cudaStream_t stream) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  a.cols = a.k_len < 1024 ? a.k_len : 1024;
+  a.cols = a.k_len < 256 ? a.k_len : 256;
   a.rows = a.q_len < 64 ? a.q_len : 64;
   const size_t smem = static_cast<size_t>(V) * ((a.rows + a.cols + 2 * V - 1) / V * V) * sizeof(T);
   const long long tiles_q = (a.q_len + a.rows - 1) / a.rows;

@@ -5,9 +5,10 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
-# Single-precision additions that a value goes through at most: 127 down a diagonal's 128 rows, 1 with the neighbouring thread's
-# share, 65 over a lane's share of a run of 2056 diagonals, 5 over the lanes; and the rounding of the result.
-ROUNDINGS = 199
+# Single-precision additions that a value goes through at most: 127 down a diagonal's 128 rows, 3 with the neighbouring thread's
+# share and the rows' ends (up to 7 of their own, instead of the 127), 8 within a block of 8 diagonals, 36 over a lane's
+# share of a run of 257 blocks and its ends, 3 over the lanes; and the rounding of the result.
+ROUNDINGS = 178
 
 
 def bucket(d, buckets, dist, both):
