@@ -52,6 +52,15 @@ class bt_embedding_weights(C.Structure):
                 ("max_positions", C.c_int), ("type_vocab_size", C.c_int), ("eps", C.c_float)]
 
 
+class bt_window_attention_args(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out")] + \
+               [(n, C.c_longlong) for n in ("q_row_stride", "k_row_stride", "v_row_stride", "out_row_stride")] + \
+               [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "k_lens")] + \
+               [(n, C.c_int) for n in ("batch", "head_num", "kv_head_num", "q_rows", "k_rows", "max_q_len", "max_k_len",
+                                       "left", "right", "sinks")] + \
+               [("scale", C.c_float), ("distance_bias", C.c_void_p), ("bias_len", C.c_int), ("bias_left", C.c_int)]
+
+
 _vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes); one entry per declaration in include/bt_b200.h
@@ -92,6 +101,7 @@ SIGNATURES = {
     "bt_relative_position_bias_grad": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "bt_add_residual_rmsnorm": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _f, _vp]),
     "bt_add_residual_rmsnorm_e4m3": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _vp]),
+    "bt_window_attention": (_i, [C.POINTER(bt_window_attention_args), _vp]),
     "bt_profile_enable": (_i, [_vp, _i]),
     "bt_profile_read": (_i, [_vp, C.POINTER(C.c_double), C.POINTER(C.c_longlong)]),
 }

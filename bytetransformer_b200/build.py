@@ -19,7 +19,7 @@ LIB_DIR = os.path.join(PKG_DIR, "lib")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 
 CU_SOURCES = ["offsets.cu", "eltwise.cu", "embed_pool.cu", "relative_bias.cu", "rmsnorm.cu", "gemm_sm100.cu", "mha_sm100.cu",
-              "encoder.cu"]
+              "window_mha.cu", "encoder.cu"]
 CORE_LIB = os.path.join(LIB_DIR, "libbt_b200.so")
 THS_LIB = os.path.join(LIB_DIR, "libths_bytetransformer.so")
 

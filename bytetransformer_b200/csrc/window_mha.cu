@@ -1,0 +1,939 @@
+// Attention over packed sequences with a sliding window and a few first tokens that stay visible, optionally with a bias
+// by distance (head size 64, fp16 in and out, heads that may share keys and values).
+//
+// Query i of a sequence of Lq queries over Lk keys stands at position p = i + Lk - Lq.  It sees key j < Lk if
+//   j <= p + right   and   (j >= p - left  or  j < sinks),
+//   out_i = sum_j softmax_j(scale * q_i . k_j + bias[h, j - p]) v_j     over the keys it sees, 0 where it sees none.
+//
+// window_mha_kernel: 128 query rows of a head at a time.  The keys that any of them sees are a run of the first keys
+// and a run around the tile; the two are laid end to end ("virtual" keys: the first run, in steps of 16, then the second) and
+// walked in tiles of 128, so a handful of first tokens does not cost a tile of its own and the window starts wherever
+// the first row's does, not at a multiple of 128.  The tile that holds the seam is fetched in boxes of 16 keys.
+// The pipeline is that of mha_persistent_kernel (mha_sm100.cu): CTAs of 256 threads, two to an SM, that take over waiting
+// blocks; one warp loads, one issues the MMAs, four own a query row per thread; S, P and O live in tensor memory.
+#include <math.h>
+
+#include <mutex>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "../../include/bt_b200.h"
+
+namespace bt {
+
+namespace {
+
+constexpr int kRows = 128;  // query rows of a block, keys of a tile
+constexpr int kHeadDim = 64;
+constexpr int kTile = 128 * kHeadDim * 2;  // 16 KiB
+constexpr int kThreads = 256;
+constexpr int kSlots = 4;  // items between the loader and the other roles
+constexpr int kSeam = 16;  // keys of a box of the tile with the seam
+
+struct WindowArgs {
+  __half* out;
+  long long out_stride;
+  const int *q_offsets, *k_offsets, *k_lens;
+  int batch, heads, group;  // group: heads that share a key/value head
+  int q_rows, k_rows, max_q, max_k;
+  int left, right, sinks;  // left, right < 0: no bound
+  float scale_log2e;
+  const float* bias;  // [heads, bias_n]: distances -bias_left ..., the outermost values beyond
+  int bias_n, bias_left;
+  int* status;
+  int tma_out;
+  int take_over;  // the grid has more blocks than are resident
+  int by_rows;    // the grid has blocks for as many items as offsets that rise can hold, which others may exceed
+};
+
+struct Item {
+  int q_row, rows;     // first row of the tile in q and out, rows that exist; 0 rows: no more items
+  int p0;              // position of the first
+  int head;
+  int k_row, k_len;    // the sequence's keys
+};
+
+// The virtual keys of an item.
+struct Keys {
+  int ns;     // keys of the first run, a multiple of kSeam, or 0: the second run starts at key 0 or there are none
+  int ws;     // first key of the second run
+  int total;  // virtual keys
+  int tiles;  // >= 1: an item that sees nothing walks one tile of masked keys
+};
+__device__ __forceinline__ Keys keys_of(const WindowArgs& a, const Item& it) {
+  Keys k;
+  const int last = it.p0 + it.rows - 1;
+  const int hi = a.right < 0 ? it.k_len : min(it.k_len, last + a.right + 1);
+  const int lo = a.left < 0 ? 0 : max(0, it.p0 - a.left);
+  const int first = (max(min(a.sinks, hi), 0) + kSeam - 1) & ~(kSeam - 1);
+  const bool apart = lo > first;
+  k.ns = apart ? first : 0;
+  k.ws = apart ? lo : 0;
+  k.total = max(k.ns + hi - k.ws, 0);
+  k.tiles = max(1, (k.total + kRows - 1) / kRows);
+  return k;
+}
+
+// Item n = (sequence, query tile, head), heads fastest; called by whole warps, 32 sequences at a time.  A sequence whose
+// offsets do not describe rows of the buffers is left out and reported.
+__device__ __forceinline__ bool find_item(const WindowArgs& a, int n, int& cur_b, int& cur_first, Item& it) {
+  const int lane = static_cast<int>(threadIdx.x & 31u);
+  if (n < cur_first) cur_b = cur_first = 0;
+  while (cur_b < a.batch) {
+    const int b = cur_b + lane;
+    int start = 0, len = 0, k_row = 0, k_len = 0;
+    if (b < a.batch) {
+      start = __ldg(a.q_offsets + b);
+      len = __ldg(a.q_offsets + b + 1) - start;
+      k_row = __ldg(a.k_offsets + b);
+      const int room = __ldg(a.k_offsets + b + 1) - k_row;
+      k_len = a.k_lens != nullptr ? __ldg(a.k_lens + b) : room;
+      if (start < 0 || len < 0 || len > a.max_q || start > a.q_rows - len || k_row < 0 || k_len < 0 || k_len > a.max_k ||
+          k_len > room || k_row > a.k_rows - room) {
+        if (a.status != nullptr) atomicCAS(a.status, 0, kStatusBadOffsets);
+        len = 0;
+      }
+    }
+    const int items = ((len + kRows - 1) / kRows) * a.heads;
+    int incl = items;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    const unsigned found = __ballot_sync(0xffffffffu, b < a.batch && n < cur_first + incl);
+    if (found != 0u) {
+      const int src = __ffs(found) - 1;
+      start = __shfl_sync(0xffffffffu, start, src);
+      len = __shfl_sync(0xffffffffu, len, src);
+      it.k_row = uniform_int(__shfl_sync(0xffffffffu, k_row, src));
+      it.k_len = uniform_int(__shfl_sync(0xffffffffu, k_len, src));
+      cur_first += __shfl_sync(0xffffffffu, incl - items, src);
+      cur_b += src;
+      const int r = n - cur_first;
+      const int qt = r / a.heads;
+      if (qt < 0 || qt > (len - 1) / kRows) break;  // (offsets so wrong that the count of items passed 32 bits)
+      it.head = uniform_int(r - qt * a.heads);
+      it.q_row = uniform_int(start + qt * kRows);
+      it.rows = uniform_int(min(kRows, len - qt * kRows));
+      it.p0 = uniform_int(qt * kRows + it.k_len - len);
+      return true;
+    }
+    cur_first += __shfl_sync(0xffffffffu, incl, 31);
+    cur_b += 32;
+  }
+  it.rows = 0;
+  return false;
+}
+
+// Wait of the roles that one warp walks: between polls it sleeps, the softmax warps need the issue slots.
+__device__ __forceinline__ bool wait_role(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const long long t0 = clock64();
+  uint32_t polls = 0;
+  while (true) {
+    __nanosleep(40);
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((++polls & 63u) == 0u) {
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+      if (__any_sync(0xffffffffu, clock64() - t0 > (1ll << 31))) {
+        *abort_flag = 1;
+        if (status != nullptr) atomicCAS(status, 0, code);
+        return false;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// S = Q K^T of a 128 x 128 tile and the commit to `bar`; called by a whole warp.
+__device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint64_t* bar) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred q, f, t;\n\t"
+      ".reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "add.u64 a1, %1, 2;\n\t"
+      "add.u64 a2, %1, 4;\n\t"
+      "add.u64 a3, %1, 6;\n\t"
+      "add.u64 b1, %2, 2;\n\t"
+      "add.u64 b2, %2, 4;\n\t"
+      "add.u64 b3, %2, 6;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.u32 f, 0, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, f;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t"
+      "}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(smem_u32(bar))
+      : "memory");
+}
+// O (+)= P V over the first `steps` groups of 16 keys, P from tensor memory; called by a whole warp.
+__device__ __forceinline__ void mma_values(uint32_t d_tmem, uint32_t p_tmem, uint64_t vdesc, uint32_t idesc, uint32_t accumulate,
+                                           uint32_t steps) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred q, p, t;\n\t"
+      ".reg .b64 b;\n\t"
+      ".reg .b32 a;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.u32 p, %4, 0;\n\t"
+      "setp.eq.u32 t, 0, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+#define BT_STEP(I, A, B)                        \
+  "add.u32 a, %1, " A ";\n\t"                   \
+  "add.u64 b, %2, " B ";\n\t"                   \
+  "setp.gt.and.u32 p, %5, " I ", q;\n\t"        \
+  "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
+      BT_STEP("1", "8", "128") BT_STEP("2", "16", "256") BT_STEP("3", "24", "384") BT_STEP("4", "32", "512")
+      BT_STEP("5", "40", "640") BT_STEP("6", "48", "768") BT_STEP("7", "56", "896")
+#undef BT_STEP
+      "}\n" ::"r"(d_tmem),
+      "r"(p_tmem), "l"(vdesc), "r"(idesc), "r"(accumulate), "r"(steps)
+      : "memory");
+}
+template <int B>
+__device__ __forceinline__ void store_p(uint32_t taddr, const uint32_t (&r)[64]) {
+  uint32_t v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = r[B + i];
+  tmem_st_32x16(taddr, v);
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Bits lo .. hi - 1 of a word.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
+  const uint32_t below_hi = hi >= 32 ? 0xffffffffu : (hi > 0 ? (1u << hi) - 1u : 0u);
+  const uint32_t below_lo = lo >= 32 ? 0xffffffffu : (lo > 0 ? (1u << lo) - 1u : 0u);
+  return below_hi & ~below_lo;
+}
+
+// The bias of a tile, for all its rows: value of (column c, row r) at [c - r + 127], in log2 units.  `first`: the columns of
+// the first run of keys, `second` the others.  flat != 0: every value of the tile is second[0].
+struct BiasSlice {
+  float first[256], second[256];
+};
+
+template <bool BIAS>
+struct Layout {
+  static constexpr int kStages = 2;             // K and V tiles each
+  static constexpr int kQStages = BIAS ? 1 : 2;  // (the bias takes the place of the second Q tile)
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + kQStages * kTile;
+  static constexpr int kV = kK + kStages * kTile;
+  static constexpr int kOut = kV + kStages * kTile;
+  static constexpr int kBias = kOut + kTile;
+  static constexpr int kBar = kBias + (BIAS ? kStages * static_cast<int>(sizeof(BiasSlice)) : 0);
+  static constexpr int kBytes = kBar + 512;
+};
+
+template <bool BIAS>
+__global__ void __launch_bounds__(kThreads, 2)
+window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k16,
+                  const __grid_constant__ CUtensorMap tm_v16, const __grid_constant__ CUtensorMap tm_out, const WindowArgs args) {
+  using L = Layout<BIAS>;
+  constexpr int kStages = L::kStages, kQStages = L::kQStages;
+  constexpr uint32_t kTmemS = 0, kTmemO = 128, kTmemP = 192;
+  constexpr int kLoadTimeout = kStatusMhaLoadTimeout, kMmaTimeout = kStatusMhaMmaTimeout, kSoftmaxTimeout = kStatusMhaSoftmaxTimeout;
+  extern __shared__ __align__(1024) uint8_t smem[];
+
+  pdl_launch_dependents();
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* q_full = bars;                    // [2] by item
+  uint64_t* q_empty = bars + 2;               // [2]
+  uint64_t* k_full = bars + 4;                // [kStages] by tile
+  uint64_t* k_empty = bars + 6;
+  uint64_t* v_full = bars + 8;
+  uint64_t* v_empty = bars + 10;
+  uint64_t* s_full = bars + 12;
+  uint64_t* s_free = bars + 13;
+  uint64_t* p_full = bars + 14;
+  uint64_t* pv_done = bars + 15;
+  uint64_t* o_done = bars + 16;
+  uint64_t* item_full = bars + 17;            // [kSlots]
+  uint64_t* item_empty = bars + 21;           // [kSlots]
+  uint64_t* taken_full = bars + 25;
+  uint64_t* bias_full = bars + 26;            // [kStages] by tile
+  uint64_t* bias_empty = bars + 28;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* taken = smem + L::kBar + 256;       // 16 bytes
+  Item* items = reinterpret_cast<Item*>(smem + L::kBar + 272);
+  volatile int* flat = reinterpret_cast<volatile int*>(smem + L::kBar + 272 + kSlots * sizeof(Item));  // [kStages]
+  static_assert(272 + kSlots * sizeof(Item) + kStages * 4 <= 512, "barriers and items");
+
+  const int warp = uniform_int(static_cast<int>(threadIdx.x >> 5));
+  const int lane = threadIdx.x & 31;
+  const bool smem_ok = (smem_u32(smem) & 1023u) == 0u;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 1);
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+      mbar_init(&bias_full[s], 1);
+      mbar_init(&bias_empty[s], 4);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 4);
+    mbar_init(p_full, 4);
+    mbar_init(pv_done, 1);
+    mbar_init(o_done, 1);
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&item_full[s], 1);
+      mbar_init(&item_empty[s], BIAS ? 6 : 5);
+    }
+    mbar_init(taken_full, 1);
+    *abort_flag = smem_ok ? 0 : 1;
+    fence_mbar_init();
+    if (!smem_ok && args.status != nullptr) atomicCAS(args.status, 0, kLoadTimeout + 0x10);
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = uniform_u32(*tmem_slot);
+  pdl_wait();
+
+  // Each role finds the block's own item by itself; the n-th taken over comes through slot n % kSlots.
+  Item it;
+  auto own_item = [&]() {
+    int b = 0, f = 0;
+    return find_item(args, static_cast<int>(blockIdx.x), b, f, it);
+  };
+  auto parity = [](uint32_t n) { return (n / kSlots) & 1u; };
+  auto read_item = [&](uint32_t n) {  // (once item_full has completed)
+    const Item* s = &items[n % kSlots];
+    it.q_row = uniform_int(s->q_row);
+    it.rows = uniform_int(s->rows);
+    it.p0 = uniform_int(s->p0);
+    it.head = uniform_int(s->head);
+    it.k_row = uniform_int(s->k_row);
+    it.k_len = uniform_int(s->k_len);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[n % kSlots]);
+  };
+
+  if (warp >= 4) {
+    regs_dec<40>();
+    if (!smem_ok) {
+      // straight to the teardown
+    } else if (warp == 4) {
+      // ------------------------------------------------------------------ loads
+      int cur_b = 0, cur_first = 0;
+      bool have = find_item(args, static_cast<int>(blockIdx.x), cur_b, cur_first, it);
+      uint32_t asked = 0;
+      int beyond = args.by_rows && blockIdx.x == 0 ? static_cast<int>(gridDim.x) : -1;
+      // The next block that has not started, or, behind the last one, items that the grid's bound did not foresee: offsets
+      // that fall can hold more than it does, so the first block's CTA looks there once (which reports such offsets too).
+      auto take_next = [&]() {
+        have = false;
+        if (args.take_over && asked != 0xffffffffu) {
+          while (true) {
+            if (elect_one()) launch_control_ask(taken, taken_full);
+            if (!wait_role(taken_full, asked & 1u, abort_flag, args.status, kLoadTimeout)) return;
+            ++asked;
+            const int block = uniform_int(launch_control_answer(taken));
+            if (block < 0) break;
+            have = find_item(args, block, cur_b, cur_first, it);
+            if (have) return;
+          }
+          asked = 0xffffffffu;
+        }
+        if (beyond >= 0) have = find_item(args, beyond++, cur_b, cur_first, it);
+        if (!have) beyond = -1;
+      };
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (uint32_t n = 0; have; ++n) {
+        const Keys keys = keys_of(args, it);
+        const int qb = static_cast<int>(n % kQStages);
+        const int kv_col = it.head / args.group * kHeadDim;
+        ok = wait_role(&q_empty[qb], ((n / kQStages) & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&q_full[qb], kTile);
+          tma_load_2d(smem + L::kQ + qb * kTile, &tm_q, &q_full[qb], it.head * kHeadDim, it.q_row);
+        }
+        for (int j = 0; j < keys.tiles; ++j) {
+          const int u0 = j * kRows;
+          const bool seam = u0 < keys.ns && u0 + kRows > keys.ns;
+          const int row = it.k_row + (u0 < keys.ns ? u0 : keys.ws + u0 - keys.ns);
+          ok = wait_role(&k_empty[stage], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
+          if (!ok) break;
+          uint8_t* k_dst = smem + L::kK + stage * kTile;
+          uint8_t* v_dst = smem + L::kV + stage * kTile;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&k_full[stage], kTile);
+            if (!seam) {
+              tma_load_2d(k_dst, &tm_k, &k_full[stage], kv_col, row);
+            } else {
+              for (int s = 0; s < kRows; s += kSeam) {
+                const int u = u0 + s;
+                tma_load_2d(k_dst + s * 128, &tm_k16, &k_full[stage], kv_col, it.k_row + (u < keys.ns ? u : keys.ws + u - keys.ns));
+              }
+            }
+          }
+          __syncwarp();
+          ok = wait_role(&v_empty[stage], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
+          if (!ok) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&v_full[stage], kTile);
+            if (!seam) {
+              tma_load_2d(v_dst, &tm_v, &v_full[stage], kv_col, row);
+            } else {
+              for (int s = 0; s < kRows; s += kSeam) {
+                const int u = u0 + s;
+                tma_load_2d(v_dst + s * 128, &tm_v16, &v_full[stage], kv_col, it.k_row + (u < keys.ns ? u : keys.ws + u - keys.ns));
+              }
+            }
+          }
+          __syncwarp();
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        take_next();
+        const uint32_t slot = n % kSlots;
+        if (!wait_role(&item_empty[slot], parity(n) ^ 1u, abort_flag, args.status, kLoadTimeout)) break;
+        if (lane == 0) {
+          Item w = it;
+          if (!have) w.rows = 0;
+          items[slot] = w;
+          mbar_arrive(&item_full[slot]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 5) {
+      // -------------------------------------------------------------- MMA issue
+      constexpr uint64_t kDescK = make_smem_desc_hi(16, 1024);
+      constexpr uint64_t kDescV = make_smem_desc_hi(kTile, 1024);
+      constexpr uint32_t kIdescS = make_idesc_f16(128, 128, 0, 0);
+      constexpr uint32_t kIdescO = make_idesc_f16(128, 64, 0, 1);
+      const uint32_t s_q = smem_u32(smem + L::kQ), s_k = smem_u32(smem + L::kK), s_v = smem_u32(smem + L::kV);
+      int st = 0;
+      uint32_t ph = 0, step = 0;
+      auto q_ready = [&](uint32_t n) { return (n / kQStages) & 1u; };
+      auto issue_s = [&](uint32_t n, int stage, bool last) {
+        tc_fence_after();
+        mma_scores(tmem_base + kTmemS, smem_desc(kDescK, s_q + (n % kQStages) * kTile), smem_desc(kDescK, s_k + stage * kTile), kIdescS,
+                   s_full);
+        if (elect_one()) umma_commit(&k_empty[stage]);
+        if (last && elect_one()) umma_commit(&q_empty[n % kQStages]);  // the item's last product with Q
+      };
+      bool have = own_item();
+      Keys keys{};
+      if (have) keys = keys_of(args, it);
+      bool s_issued = false;  // the first S of the item about to start
+      for (uint32_t n = 0; have; ++n) {
+        if (!s_issued) {
+          // S overwrites its columns: the softmax warps must hold the last one in registers
+          if (step > 0 && !wait_role(s_free, (step - 1u) & 1u, abort_flag, args.status, kMmaTimeout)) break;
+          if (!wait_role(&q_full[n % kQStages], q_ready(n), abort_flag, args.status, kMmaTimeout)) break;
+          if (!wait_role(&k_full[st], ph, abort_flag, args.status, kMmaTimeout)) break;
+          issue_s(n, st, keys.tiles == 1);
+        }
+        s_issued = false;
+        bool next_known = false, next_have = false, ok = true;
+        Keys next{};
+        const int tiles = keys.tiles, total = keys.total;
+        for (int j = 0; j < tiles; ++j, ++step) {
+          const int st_n = st + 1 == kStages ? 0 : st + 1;
+          const uint32_t ph_n = st + 1 == kStages ? ph ^ 1u : ph;
+          // The next S - of this item, or of the next one if that is known and its tiles have landed - goes as soon as the
+          // softmax warps hold the present one
+          ok = wait_role(s_free, step & 1u, abort_flag, args.status, kMmaTimeout);
+          if (!ok) break;
+          if (j + 1 < tiles) {
+            ok = wait_role(&k_full[st_n], ph_n, abort_flag, args.status, kMmaTimeout);
+            if (!ok) break;
+            issue_s(n, st_n, j + 2 == tiles);
+          } else {
+            if (__all_sync(0xffffffffu, mbar_test_wait(&item_full[n % kSlots], parity(n)))) {
+              read_item(n);
+              next_known = true;
+              next_have = it.rows > 0;
+              if (next_have) next = keys_of(args, it);
+            }
+            if (next_have && __all_sync(0xffffffffu, mbar_test_wait(&q_full[(n + 1) % kQStages], q_ready(n + 1)) &&
+                                                         mbar_test_wait(&k_full[st_n], ph_n))) {
+              issue_s(n + 1, st_n, next.tiles == 1);
+              s_issued = true;
+            }
+          }
+          ok = wait_role(p_full, step & 1u, abort_flag, args.status, kMmaTimeout) &&
+               wait_role(&v_full[st], ph, abort_flag, args.status, kMmaTimeout);
+          if (!ok) break;
+          tc_fence_after();
+          const int valid = max(1, min(kRows, total - j * kRows));
+          mma_values(tmem_base + kTmemO, tmem_base + kTmemP, smem_desc(kDescV, s_v + st * kTile), kIdescO, j > 0 ? 1u : 0u,
+                     static_cast<uint32_t>((valid + 15) >> 4));
+          if (elect_one()) umma_commit(pv_done);
+          if (elect_one()) umma_commit(&v_empty[st]);
+          st = st_n;
+          ph = ph_n;
+        }
+        if (!ok) break;
+        if (elect_one()) umma_commit(o_done);
+        if (!next_known) {
+          if (!wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kMmaTimeout)) break;
+          read_item(n);
+          next_have = it.rows > 0;
+          if (next_have) next = keys_of(args, it);
+        }
+        have = next_have;
+        keys = next;
+      }
+    } else if (BIAS && warp == 6) {
+      // ------------------------------------------------------------------- bias
+      bool have = own_item(), ok = true;
+      uint32_t step = 0;
+      for (uint32_t n = 0; have && ok; ++n) {
+        const Keys keys = keys_of(args, it);
+        const float* bias = args.bias + static_cast<long long>(it.head) * args.bias_n;
+        const int top = args.bias_n - 1;
+        for (int j = 0; j < keys.tiles; ++j, ++step) {
+          const int stage = static_cast<int>(step % kStages);
+          ok = wait_role(&bias_empty[stage], ((step / kStages) & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
+          if (!ok) break;
+          BiasSlice* slice = reinterpret_cast<BiasSlice*>(smem + L::kBias) + stage;
+          const int u0 = j * kRows;
+          // index of the value at [0]: distance of column 0 and row 127
+          const int at2 = keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left;
+          const int at1 = u0 - it.p0 - 127 + args.bias_left;
+          const bool has_first = u0 < keys.ns;
+          const bool is_flat = !has_first && (at2 >= top || at2 + 254 <= 0);
+          if (lane == 0) flat[stage] = is_flat;
+          if (is_flat) {
+            if (lane == 0) slice->second[0] = __ldg(bias + (at2 >= top ? top : 0)) * 1.4426950408889634f;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              slice->second[i * 32 + lane] = __ldg(bias + min(max(at2 + i * 32 + lane, 0), top)) * 1.4426950408889634f;
+            if (has_first) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                slice->first[i * 32 + lane] = __ldg(bias + min(max(at1 + i * 32 + lane, 0), top)) * 1.4426950408889634f;
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bias_full[stage]);
+        }
+        if (!ok || !wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kLoadTimeout)) break;
+        read_item(n);
+        have = it.rows > 0;
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax (warps 0..3)
+    regs_inc<216>();
+    const int r = warp * 32 + lane;  // query row inside the tile == tensor-memory lane
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t t_s = t_lane + kTmemS, t_o = t_lane + kTmemO, t_p = t_lane + kTmemP;
+    const float c = args.scale_log2e;
+    int stage = 0;
+    uint32_t phase = 0, step = 0;
+    bool have = smem_ok && own_item();
+    for (uint32_t n = 0; have; ++n) {
+      const Keys keys = keys_of(args, it);
+      const bool exists = r < it.rows;
+      const bool idle = warp * 32 >= it.rows;  // no row of this warp exists
+      // virtual keys that this row sees: [0, a_hi) and [b_lo, b_hi)
+      const int p = it.p0 + r;
+      const int hi = args.right < 0 ? it.k_len : min(it.k_len, p + args.right + 1);
+      const int a_hi = args.left < 0 ? 0 : min(args.sinks, hi);
+      const int b_lo = keys.ns + max((args.left < 0 ? 0 : p - args.left) - keys.ws, 0);
+      const int b_hi = keys.ns + hi - keys.ws;
+      // The exponent reference of a row may lag its maximum by 2^8 (then the warp's rows move theirs and rescale O); rows that
+      // do not exist have no say, so results are a function of the inputs alone
+      const float max_lag = exists ? 8.0f : INFINITY;
+      float m_ref = -INFINITY, l_run = 0.f;
+      for (int j = 0; j < keys.tiles; ++j, ++step) {
+        const int u0 = j * kRows;
+        mbar_wait_anyway_lane(s_full, step & 1u, abort_flag, args.status, kSoftmaxTimeout);
+        tc_fence_after();
+        bool pv_waited = j == 0;  // (an item's first tile: the wait for the previous item's O covered it)
+        auto wait_pv = [&]() {  // P and O belong to the previous tile's MMAs until those have retired
+          mbar_wait_anyway_lane(pv_done, (step - 1u) & 1u, abort_flag, args.status, kSoftmaxTimeout);
+          tc_fence_after();
+          pv_waited = true;
+        };
+        auto move_reference = [&](float m_new) {
+          if (j == 0) {
+            m_ref = m_new;
+          } else if (__any_sync(0xffffffffu, (m_new - m_ref) > max_lag)) {
+            if (!pv_waited) wait_pv();
+            const float f = m_new == m_ref ? 1.0f : ex2(m_ref - m_new);
+#pragma unroll
+            for (int cb = 0; cb < kHeadDim; cb += 32) {
+              uint32_t v[32];
+              tmem_ld_32x32(t_o + cb, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+              tmem_st_32x32(t_o + cb, v);
+            }
+            l_run *= f;
+            m_ref = m_new;
+          }
+        };
+        // what the exponent subtracts: a row that has seen nothing yet keeps its masked scores at 2^-inf
+        auto reference = [&]() { return m_ref == -INFINITY ? 0.f : m_ref; };
+        const float* slice = nullptr;
+        bool is_flat = true;
+        float flat_bias = 0.f;
+        if (BIAS) {
+          const int bs = static_cast<int>(step % kStages);
+          mbar_wait_anyway_lane(&bias_full[bs], (step / kStages) & 1u, abort_flag, args.status, kSoftmaxTimeout);
+          slice = reinterpret_cast<const float*>(smem + L::kBias + bs * sizeof(BiasSlice)) + 127 - r;
+          is_flat = flat[bs] != 0;
+          if (is_flat) flat_bias = slice[256 - 127 + r];
+        }
+        const bool whole = __all_sync(0xffffffffu, !exists || (b_lo <= u0 && b_hi >= u0 + kRows));
+        if (idle) {
+          if (lane == 0) mbar_arrive(s_free);
+          if (!pv_waited) wait_pv();  // (or this warp's next p_full would count for the tile that the others are still at)
+        } else if (whole) {
+          // every row of the warp sees every key of the tile
+          uint32_t s[128];
+          tmem_ld_32x32_at<0>(t_s, s);
+          tmem_ld_32x32_at<32>(t_s + 32, s);
+          tmem_ld_32x32_at<64>(t_s + 64, s);
+          tmem_ld_32x32_at<96>(t_s + 96, s);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free);
+          float scale = c, shift = flat_bias;
+          if (BIAS && !is_flat) {  // (whole tiles lie in the second run)
+            const float* b = slice + 256;
+#pragma unroll
+            for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b[i]));
+            scale = 1.0f;
+          }
+          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 128; i += 8) {
+            mx0 = max3(mx0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            mx1 = max3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+            mx2 = max3(mx2, __uint_as_float(s[i + 4]), __uint_as_float(s[i + 5]));
+            mx3 = max3(mx3, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
+          }
+          move_reference(fmaxf(m_ref, fmaf(scale, max3(mx0, mx1, fmaxf(mx2, mx3)), shift)));
+          const float minus = shift - reference();
+          unsigned long long l0 = pack_f32x2(0.f, 0.f), l1 = l0;
+          const unsigned long long sc2 = pack_f32x2(scale, scale), mi2 = pack_f32x2(minus, minus);
+          uint32_t pk[64];
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            float t0, t1;
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, mi2), t0, t1);
+            const float p0 = ex2(t0), p1 = ex2(t1);
+            if (i & 1) l1 = add_f32x2(l1, pack_f32x2(p0, p1)); else l0 = add_f32x2(l0, pack_f32x2(p0, p1));
+            pk[i] = pack_half2(p0, p1);
+          }
+          float la, lb;
+          unpack_f32x2(add_f32x2(l0, l1), la, lb);
+          l_run += la + lb;
+          if (!pv_waited) wait_pv();
+          store_p<0>(t_p, pk);
+          store_p<16>(t_p + 16, pk);
+          store_p<32>(t_p + 32, pk);
+          store_p<48>(t_p + 48, pk);
+        } else {
+          // Some keys are masked for some row: by chunks of 32 keys, those that any row of the warp sees, in two passes over S.
+          auto seen = [&](int c0) { return bits_between(0, a_hi - u0 - c0) | bits_between(b_lo - u0 - c0, b_hi - u0 - c0); };
+          auto scores = [&](int c0, uint32_t w, float (&v)[32]) {
+            uint32_t raw[32];
+            tmem_ld_32x32(t_s + c0, raw);
+            tmem_ld_wait();
+            if (BIAS && !is_flat) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float* b = slice + (u0 + c0 + 16 * h < keys.ns ? 0 : 256) + c0;
+#pragma unroll
+                for (int i = 16 * h; i < 16 * h + 16; ++i) v[i] = fmaf(__uint_as_float(raw[i]), c, b[i]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = BIAS ? fmaf(__uint_as_float(raw[i]), c, flat_bias) : __uint_as_float(raw[i]) * c;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = ((w >> i) & 1u) ? v[i] : -INFINITY;
+          };
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c0 = 0; c0 < kRows; c0 += 32) {
+            const uint32_t w = seen(c0);
+            if (!__any_sync(0xffffffffu, exists && w != 0u)) continue;
+            float v[32];
+            scores(c0, w, v);
+            float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              m0 = max3(m0, v[i], v[i + 1]);
+              m1 = max3(m1, v[i + 2], v[i + 3]);
+            }
+            mx = fmaxf(mx, fmaxf(m0, m1));
+          }
+          move_reference(fmaxf(m_ref, mx));
+          if (!pv_waited) wait_pv();
+          const float m = reference();
+          const int used = (min(kRows, keys.total - u0) + 15) & ~15;  // keys that are multiplied
+#pragma unroll 1
+          for (int c0 = 0; c0 < max(used, 16); c0 += 32) {
+            const uint32_t w = seen(c0);
+            uint32_t pk[16];
+            if (__any_sync(0xffffffffu, exists && w != 0u)) {
+              float v[32];
+              scores(c0, w, v);
+              float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float p0 = ex2(v[2 * i] - m), p1 = ex2(v[2 * i + 1] - m);
+                l0 += p0;
+                l1 += p1;
+                pk[i] = pack_half2(p0, p1);
+              }
+              l_run += l0 + l1;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[i] = 0u;
+            }
+            tmem_st_32x16(t_p + (c0 >> 1), pk);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free);
+        }
+        if (BIAS) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bias_empty[step % kStages]);
+        }
+        const int valid = min(kRows, keys.total - u0);
+        if (valid < kRows) {
+          // blank the V rows behind the last key (as far as they are multiplied): they may be anybody's
+          mbar_wait_anyway_lane(&v_full[stage], phase, abort_flag, args.status, kSoftmaxTimeout);
+          if (r >= valid && r < max(16, (valid + 15) & ~15)) {
+            uint4* vr = reinterpret_cast<uint4*>(smem + L::kV + stage * kTile + r * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) vr[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!mbar_wait_warp(o_done, n & 1u, abort_flag, args.status, kSoftmaxTimeout)) break;
+      tc_fence_after();
+      // O / row sum -> fp16 -> this warp's staging rows -> global memory: a slab of 32 rows that all exist by one bulk
+      // store, others by the threads, eight to a row
+      const float inv = 1.0f / l_run;
+      const bool some = l_run != 0.f;  // (a row that sees no key is 0; a NaN stays one)
+      if (lane == 0) tma_store_wait_read();
+      __syncwarp();
+      uint8_t* stage_out = smem + L::kOut + warp * (32 * 128);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[32];
+        tmem_ld_32x32(t_o + 32 * h, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint4 w;
+          auto pair = [&](int i) {
+            return some ? pack_half2(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv) : 0u;
+          };
+          w.x = pair(u * 8);
+          w.y = pair(u * 8 + 2);
+          w.z = pair(u * 8 + 4);
+          w.w = pair(u * 8 + 6);
+          *reinterpret_cast<uint4*>(stage_out + lane * 128 + (((4 * h + u) ^ (lane & 7)) << 4)) = w;
+        }
+      }
+      const bool whole_slab = args.tma_out != 0 && warp * 32 + 32 <= it.rows;
+      if (whole_slab) fence_proxy_async_smem();
+      __syncwarp();
+      if (whole_slab) {
+        if (lane == 0) {
+          tma_store_2d(&tm_out, stage_out, it.head * kHeadDim, it.q_row + warp * 32);
+          tma_store_commit();
+        }
+      } else {
+        const int sub = lane >> 3, unit = lane & 7;
+        __half* out = args.out + static_cast<long long>(it.q_row + warp * 32) * args.out_stride + it.head * kHeadDim + unit * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int row = 4 * k + sub;
+          const uint4 w = *reinterpret_cast<const uint4*>(stage_out + row * 128 + ((unit ^ (row & 7)) << 4));
+          if (warp * 32 + row < it.rows) *reinterpret_cast<uint4*>(out + row * args.out_stride) = w;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (!mbar_wait_warp(&item_full[n % kSlots], parity(n), abort_flag, args.status, kSoftmaxTimeout)) break;
+      read_item(n);
+      have = it.rows > 0;
+    }
+    if (lane == 0) tma_store_wait_all();  // the staging rows must outlive the last bulk store
+    tc_fence_before();
+  }
+
+  __syncthreads();
+  if (*abort_flag != 0) {  // copies in flight land before the block's memory goes to another
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
+  }
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 256);
+  }
+}
+
+template <bool BIAS>
+cudaError_t launch_window(const CUtensorMap (&tm)[6], WindowArgs a, int sms, cudaStream_t stream) {
+  auto kern = window_mha_kernel<BIAS>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<BIAS>::kBytes);
+  if (e != cudaSuccess) return e;
+  // A block per item, by an upper bound: tiles of sequences of max_q queries, or of sequences that share q_rows rows
+  long long tiles = static_cast<long long>(a.batch) * ((a.max_q + kRows - 1) / kRows);
+  const long long by_rows = (a.q_rows + static_cast<long long>(a.batch) * (kRows - 1)) / kRows;
+  a.by_rows = tiles > by_rows ? 1 : 0;
+  if (a.by_rows) tiles = by_rows;
+  const long long grid = tiles * a.heads;
+  if (grid > 0x7fffffffLL - 0x10000) return cudaErrorInvalidValue;
+  a.take_over = grid > 2LL * sms ? 1 : 0;
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Layout<BIAS>::kBytes, stream, tm[0], tm[1], tm[2], tm[3],
+                    tm[4], tm[5], a);
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+struct DeviceFacts {
+  int sms = 0, major = 0;
+  int* status = nullptr;
+};
+// What a call needs to know of the current device; looked up once (outside a capture, see bt_b200.h).
+cudaError_t device_facts(DeviceFacts* f) {
+  static std::mutex mu;
+  static DeviceFacts known[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(mu);
+  if (known[dev].status == nullptr) {
+    DeviceFacts n;
+    e = cudaDeviceGetAttribute(&n.sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&n.major, cudaDevAttrComputeCapabilityMajor, dev);
+    if (e != cudaSuccess) return e;
+    n.status = device_status_word();
+    if (n.status == nullptr) return cudaErrorUnknown;
+    known[dev] = n;
+  }
+  *f = known[dev];
+  return cudaSuccess;
+}
+
+// Lengths, windows and positions stay below this, so that none of their sums passes 32 bits.
+constexpr int kMaxLength = (1 << 30) - 1;
+
+}  // namespace
+
+}  // namespace bt
+
+using namespace bt;
+
+extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stream_v) {
+  if (a == nullptr || !a->q || !a->out || !a->q_offsets || !a->k_offsets) return BT_ERR_INVALID_ARG;
+  if (a->k_rows > 0 && (!a->k || !a->v)) return BT_ERR_INVALID_ARG;
+  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->out, 16)) return BT_ERR_INVALID_ARG;
+  if (!aligned(a->q_offsets, 4) || !aligned(a->k_offsets, 4) || !aligned(a->k_lens, 4) || !aligned(a->distance_bias, 4)) return BT_ERR_INVALID_ARG;
+  if (a->head_num <= 0 || a->head_num > 1024 || a->kv_head_num <= 0 || a->head_num % a->kv_head_num != 0) return BT_ERR_INVALID_ARG;
+  if (a->batch <= 0 || a->q_rows <= 0 || a->k_rows < 0 || a->max_q_len <= 0 || a->max_q_len > kMaxLength || a->max_k_len < 0 ||
+      a->max_k_len > kMaxLength || a->sinks < 0 || !(a->scale > 0.f) || !(a->scale < INFINITY))
+    return BT_ERR_INVALID_ARG;
+  const long long q_cols = 64LL * a->head_num, kv_cols = 64LL * a->kv_head_num, max_stride = 1LL << 32;
+  const long long strides[4] = {a->q_row_stride, a->k_row_stride, a->v_row_stride, a->out_row_stride};
+  for (int i = 0; i < 4; ++i)
+    if (strides[i] % 8 != 0 || strides[i] < (i == 0 || i == 3 ? q_cols : kv_cols) || strides[i] > max_stride) return BT_ERR_INVALID_ARG;
+  if (a->distance_bias != nullptr && (a->bias_len <= 0 || a->bias_len > kMaxLength / 2 || a->bias_left < 0 || a->bias_left >= a->bias_len))
+    return BT_ERR_INVALID_ARG;
+  DeviceFacts dev;
+  if (device_facts(&dev) != cudaSuccess) return BT_ERR_CUDA;
+  if (dev.major != 10) return BT_ERR_UNSUPPORTED;
+  WindowArgs w;
+  w.out = static_cast<__half*>(a->out);
+  w.out_stride = a->out_row_stride;
+  w.q_offsets = a->q_offsets;
+  w.k_offsets = a->k_offsets;
+  w.k_lens = a->k_lens;
+  w.batch = a->batch;
+  w.heads = a->head_num;
+  w.group = a->head_num / a->kv_head_num;
+  w.q_rows = a->q_rows;
+  w.k_rows = a->k_rows;
+  w.max_q = a->max_q_len;
+  w.max_k = a->max_k_len;
+  // a bound that no distance reaches is none
+  w.left = a->left >= a->max_k_len ? -1 : a->left;
+  w.right = a->right >= kMaxLength ? -1 : a->right;
+  w.sinks = a->sinks < a->max_k_len ? a->sinks : a->max_k_len;
+  w.scale_log2e = a->scale * 1.4426950408889634f;
+  w.bias = a->distance_bias;
+  w.bias_n = a->bias_len;
+  w.bias_left = a->bias_left;
+  w.status = dev.status;
+  // Without any key rows the loads of the one masked tile that an item walks need some rows: those of q do.
+  const bool none = a->k_rows == 0;
+  const void *k = none ? a->q : a->k, *v = none ? a->q : a->v;
+  const uint64_t k_rows = none ? a->q_rows : a->k_rows;
+  const long long k_ld = none ? a->q_row_stride : a->k_row_stride, v_ld = none ? a->q_row_stride : a->v_row_stride;
+  CUtensorMap tm[6];
+  const bool ok = make_tmap_2d(&tm[0], a->q, a->q_rows, q_cols, a->q_row_stride, 64, 128) &&
+                  make_tmap_2d(&tm[1], k, k_rows, kv_cols, k_ld, 64, 128) && make_tmap_2d(&tm[2], v, k_rows, kv_cols, v_ld, 64, 128) &&
+                  make_tmap_2d(&tm[3], k, k_rows, kv_cols, k_ld, 64, kSeam) && make_tmap_2d(&tm[4], v, k_rows, kv_cols, v_ld, 64, kSeam) &&
+                  make_tmap_2d(&tm[5], a->out, a->q_rows, q_cols, a->out_row_stride, 64, 32);
+  if (!ok) return BT_ERR_CUDA;
+  w.tma_out = 1;
+  const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+  const cudaError_t e = w.bias != nullptr ? launch_window<true>(tm, w, dev.sms, stream) : launch_window<false>(tm, w, dev.sms, stream);
+  if (e == cudaErrorInvalidValue) return BT_ERR_INVALID_ARG;
+  return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;
+}

@@ -624,6 +624,70 @@ def add_residual_rmsnorm_e4m3(x: torch.Tensor, residual: Optional[torch.Tensor],
     return out, scales, total
 
 
+def _rows(t: torch.Tensor, name: str, device, heads_of: int = 64) -> int:
+    """Heads of a matrix [rows, heads * 64] whose rows may be further apart than they are long."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dtype != torch.float16:
+        raise RuntimeError(f"Inconsistency of Tensor type: {name}")
+    if t.dim() != 2 or t.shape[1] == 0 or t.shape[1] % heads_of != 0 or t.stride(1) != 1:
+        raise RuntimeError(f"{name} must be [rows, heads*64] with contiguous rows")
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, the other tensors are on {device}")
+    return t.shape[1] // heads_of
+
+
+def _ints(t: torch.Tensor, name: str, device) -> int:
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.device != device:
+        raise RuntimeError(f"{name} must be a contiguous int32 vector on the device of the other tensors")
+    return t.shape[0]
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
+                     max_q_len: int, max_k_len: int, *, left: int = -1, right: int = -1, sinks: int = 0,
+                     k_lens: Optional[torch.Tensor] = None, distance_bias: Optional[torch.Tensor] = None,
+                     bias_left: int = 0, scale: float = 0.125, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """[rows, heads*64]: packed attention in which a query sees `left` keys before it, `right` behind it and the first
+    `sinks` ones of its sequence (bt_window_attention has the definition).  q [rows, heads*64], k and v
+    [k_rows, kv_heads*64], fp16, views into a packed QKV product among them; queries are the last ones of their
+    sequence's keys, so a single new token over a cache is a sequence of one query (k_lens: how much of each
+    sequence's place in the cache is filled).  distance_bias [heads, n] fp32, value of distance j - p at bias_left + j - p.
+    Rows that belong to no sequence are left as `out` has them (undefined without `out`)."""
+    device = q.device
+    heads, kv_heads = _rows(q, "q", device), _rows(k, "k", device)
+    if _rows(v, "v", device) != kv_heads or v.shape[0] != k.shape[0]:
+        raise RuntimeError("k and v must have the same shape")
+    batch = _ints(q_offsets, "q_offsets", device) - 1
+    if _ints(k_offsets, "k_offsets", device) != batch + 1 or batch < 0:
+        raise RuntimeError("q_offsets and k_offsets must have batch + 1 elements")
+    if k_lens is not None and _ints(k_lens, "k_lens", device) != batch:
+        raise RuntimeError("k_lens must have batch elements")
+    n_bias = 0
+    if distance_bias is not None:
+        _check(distance_bias, "distance_bias", torch.float32)
+        if distance_bias.dim() != 2 or distance_bias.shape[0] != heads or distance_bias.device != device:
+            raise RuntimeError("distance_bias must be [heads, n] on the device of the other tensors")
+        n_bias = distance_bias.shape[1]
+    if out is not None and (_rows(out, "out", device) != heads or out.shape[0] != q.shape[0]):
+        raise RuntimeError("out must have q's shape")
+    lib = _abi.load()
+    with _On(device) as stream:
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.float16, device=device)
+        rows, k_rows = q.shape[0], k.shape[0]
+        if rows == 0 or batch == 0:
+            return out
+        a = _abi.bt_window_attention_args(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
+            out.stride(0), q_offsets.data_ptr(), k_offsets.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
+            batch, heads, kv_heads, rows, k_rows, max_q_len, max_k_len, left, right, sinks, scale,
+            distance_bias.data_ptr() if distance_bias is not None else None, n_bias, bias_left)
+        rc = lib.bt_window_attention(C.byref(a), stream)
+    if rc != _abi.BT_OK:
+        raise _abi.BtError(rc, "bt_window_attention")
+    return out
+
+
 def bert_transformer(head_num: int, head_size: int,
                      qkv_kernel, qkv_bias, attr_output_kernel, attr_output_bias,
                      attr_output_layernorm_gamma, attr_output_layernorm_beta,

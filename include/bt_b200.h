@@ -343,6 +343,39 @@ int bt_add_residual_rmsnorm_e4m3(const void* x, int x_fp32, const void* residual
                                  void* sum_out, void* out, float* scales, int group, const int* m_dev, int m_rows, int hidden,
                                  float eps, void* stream);
 
+/* Attention beside bt_attention() with a sliding window and a few first tokens that stay visible (no counterpart in the
+ * reference): heads of 64, fp16, packed sequences of any length, queries and keys each with rows of their own.
+ *   Query i of sequence b (rows q_offsets[b] .. q_offsets[b+1] - 1 of q and out, Lq of them) stands at position p = i + Lk - Lq
+ *   of its Lk keys: the last query sees the last key.  Key j is visible to it if
+ *       j <= p + right   and   (j >= p - left  or  j < sinks);        left < 0, right < 0: no such bound
+ *       out = sum over visible j of softmax(scale * q.k_j + distance_bias[h, bias_left + (j - p)]) * v_j,
+ *   and zeros where no key is visible (Lk = 0, p + right < 0).  Distances outside the table take its outermost values;
+ *   distance_bias (fp32 [head_num, bias_len], or NULL) is what bt_relative_position_bias makes of a learned table with
+ *   q_len = 1, q_start = bias_left.
+ *   Lk: k_offsets[b+1] - k_offsets[b] rows from k_offsets[b] of k and v, or k_lens[b] of them (k_lens not NULL): a cache
+ *   with room to grow.  Query head h reads key/value head h / (head_num / kv_head_num).  Row strides in halves, multiples of 8;
+ *   data pointers 16-byte aligned; q_offsets, k_offsets int32[batch+1], k_lens int32[batch], on the device.  max_q_len,
+ *   max_k_len: upper bounds of Lq and Lk.  Rows of q and out from q_offsets[batch] on are neither read into a result nor written.
+ *   The values in a sequence's own rows of k and v must be finite where any of 128 neighbouring queries sees them; what
+ *   other rows hold does not matter.  out may not overlap q, k or v.
+ *   Offsets or lengths that do not describe rows of the buffers make the sequence a no-op and set the device's status
+ *   word, as in bt_attention (bt_device_status of any handle of the device).
+ *   The current device is the one used; the first call on it looks its properties up and must be outside a stream capture. */
+typedef struct bt_window_attention_args {
+  const void *q, *k, *v; /* [q_rows, head_num * 64], [k_rows, kv_head_num * 64] twice */
+  void* out;             /* [q_rows, head_num * 64] */
+  long long q_row_stride, k_row_stride, v_row_stride, out_row_stride;
+  const int *q_offsets, *k_offsets, *k_lens;
+  int batch, head_num, kv_head_num;
+  int q_rows, k_rows; /* rows allocated */
+  int max_q_len, max_k_len;
+  int left, right, sinks;
+  float scale; /* > 0; 1 / sqrt(64) is the usual one */
+  const float* distance_bias;
+  int bias_len, bias_left;
+} bt_window_attention_args;
+int bt_window_attention(const bt_window_attention_args* args, void* stream);
+
 /* ---- launch accounting and per-kernel timing ------------------------------ */
 /* Kernel kinds of the arrays below (one slot per kind, BT_PROF_KINDS slots). */
 #define BT_PROF_OFFSETS 0
