@@ -150,6 +150,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^x of a pair on the FMA pipe: whole part by the rounding of x + 1.5 * 2^23, the rest, f in [-1/2, 1/2], by the polynomial of
+// degree 4 with the least relative error there (2.6e-6; Remez exchange).  Below 2^-126 it stays at that.
+__device__ __forceinline__ void ex2_pair_fma(float& x0, float& x1) {
+  const unsigned long long magic = pack_f32x2(12582912.f, 12582912.f), less = pack_f32x2(-12582912.f, -12582912.f);
+  const unsigned long long x = pack_f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const unsigned long long r = add_f32x2(x, magic);
+  const unsigned long long f = fma_f32x2(add_f32x2(r, less), pack_f32x2(-1.f, -1.f), x);
+  unsigned long long p = fma_f32x2(f, pack_f32x2(0.00957010221f, 0.00957010221f), pack_f32x2(0.0559178591f, 0.0559178591f));
+  p = fma_f32x2(p, f, pack_f32x2(0.240247443f, 0.240247443f));
+  p = fma_f32x2(p, f, pack_f32x2(0.693121791f, 0.693121791f));
+  p = fma_f32x2(p, f, pack_f32x2(0.999999285f, 0.999999285f));
+  float r0, r1, p0, p1;
+  unpack_f32x2(r, r0, r1);
+  unpack_f32x2(p, p0, p1);
+  x0 = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
+  x1 = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -204,13 +221,6 @@ __device__ __forceinline__ void mma_values(uint32_t d_tmem, uint32_t p_tmem, uin
       "r"(p_tmem), "l"(vdesc), "r"(idesc), "r"(accumulate), "r"(steps)
       : "memory");
 }
-template <int B>
-__device__ __forceinline__ void store_p(uint32_t taddr, const uint32_t (&r)[64]) {
-  uint32_t v[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = r[B + i];
-  tmem_st_32x16(taddr, v);
-}
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -219,6 +229,11 @@ template <int N>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
 
 // Bits lo .. hi - 1 of a word.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
@@ -575,25 +590,116 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int a_hi = args.left < 0 ? 0 : min(args.sinks, hi);
       const int b_lo = keys.ns + max((args.left < 0 ? 0 : p - args.left) - keys.ws, 0);
       const int b_hi = keys.ns + hi - keys.ws;
-      // The exponent reference of a row may lag its maximum by 2^8 (then the warp's rows move theirs and rescale O); rows that
-      // do not exist have no say, so results are a function of the inputs alone
-      const float max_lag = exists ? 8.0f : INFINITY;
+      // A tile's weights are 2^(score - m_ref) with the reference of the tiles before, so that they need not wait for the tile's
+      // own maximum.  Where that turns out to be more than 2^kLag above a row's reference (fp16 holds the weights up to
+      // there) the warp's rows move theirs to their maxima, rescale O, and the tile's weights are formed again.  Rows that do
+      // not exist have no say, so results are a function of the inputs alone.
+      constexpr float kLag = 12.0f;
       float m_ref = -INFINITY, l_run = 0.f;
       for (int j = 0; j < keys.tiles; ++j, ++step) {
         const int u0 = j * kRows;
         mbar_wait_anyway_lane(s_full, step & 1u, abort_flag, args.status, kSoftmaxTimeout);
         tc_fence_after();
-        bool pv_waited = j == 0;  // (an item's first tile: the wait for the previous item's O covered it)
         auto wait_pv = [&]() {  // P and O belong to the previous tile's MMAs until those have retired
+          if (j == 0) return;   // (an item's first tile: the wait for the previous item's O covered it)
           mbar_wait_anyway_lane(pv_done, (step - 1u) & 1u, abort_flag, args.status, kSoftmaxTimeout);
           tc_fence_after();
-          pv_waited = true;
         };
-        auto move_reference = [&](float m_new) {
+        const float* slice = nullptr;
+        bool is_flat = true;
+        float scale = c, shift = 0.f;  // log2 units of what `s` holds below
+        if (BIAS) {
+          const int bs = static_cast<int>(step % kStages);
+          mbar_wait_anyway_lane(&bias_full[bs], (step / kStages) & 1u, abort_flag, args.status, kSoftmaxTimeout);
+          slice = reinterpret_cast<const float*>(smem + L::kBias + bs * sizeof(BiasSlice)) + 127 - r;
+          is_flat = flat[bs] != 0;
+          if (is_flat) shift = slice[256 - 127 + r]; else scale = 1.0f;
+        }
+        if (idle) {
+          if (lane == 0) mbar_arrive(s_free);
+          wait_pv();  // (or this warp's next p_full would count for the tile that the others are still at)
+        } else {
+          const bool whole = __all_sync(0xffffffffu, !exists || (b_lo <= u0 && b_hi >= u0 + kRows));
+          uint32_t s[128];
+          float mx0 = -INFINITY, mx1 = -INFINITY;
+          unsigned some = 0xfu;  // chunks of 32 keys that any row of the warp sees
+          // scores of chunk CH: the bias added, masked keys out; the row's maximum
+          auto fix = [&](auto chunk) {
+            constexpr int B = decltype(chunk)::value * 32;
+            if (BIAS && !is_flat) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float* b = slice + (u0 + B + 16 * h < keys.ns ? 0 : 256);
+#pragma unroll
+                for (int i = B + 16 * h; i < B + 16 * h + 16; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b[i]));
+              }
+            }
+            if (!whole) {
+              const uint32_t w = bits_between(0, a_hi - u0 - B) | bits_between(b_lo - u0 - B, b_hi - u0 - B);
+              if (!__any_sync(0xffffffffu, exists && w != 0u)) {
+                some &= ~(1u << (B / 32));
+                return;
+              }
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[B + i] = ((w >> i) & 1u) ? s[B + i] : 0xff800000u;
+            }
+#pragma unroll
+            for (int i = B; i < B + 32; i += 4) {
+              mx0 = max3(mx0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+              mx1 = max3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
+            }
+          };
+          float minus = 0.f;
+          unsigned long long l0 = 0ull, l1 = 0ull;  // pairs of zeros
+          // weights of chunk CH: fp16 pairs, fp32 sums
+          uint32_t pk[64];
+          auto weigh = [&](auto chunk) {
+            constexpr int B = decltype(chunk)::value * 32;
+            if (some & (1u << (B / 32))) {
+              const unsigned long long sc2 = pack_f32x2(scale, scale), mi2 = pack_f32x2(minus, minus);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float t0, t1;
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[B + 2 * i]), __uint_as_float(s[B + 2 * i + 1])), sc2, mi2), t0, t1);
+                if (i % 8 == 7) {  // one pair in eight goes round the special-function unit
+                  ex2_pair_fma(t0, t1);
+                } else {
+                  t0 = ex2(t0);
+                  t1 = ex2(t1);
+                }
+                const float p0 = t0, p1 = t1;
+                if (i & 1) l1 = add_f32x2(l1, pack_f32x2(p0, p1)); else l0 = add_f32x2(l0, pack_f32x2(p0, p1));
+                pk[B / 2 + i] = pack_half2(p0, p1);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pk[B / 2 + i] = 0u;
+            }
+          };
+          auto store = [&](auto chunk) {
+            constexpr int B = decltype(chunk)::value * 16;
+            uint32_t v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = pk[B + i];
+            tmem_st_32x16(t_p + B, v);
+          };
+          tmem_ld_32x32_at<0>(t_s, s);
+          tmem_ld_32x32_at<32>(t_s + 32, s);
+          tmem_ld_32x32_at<64>(t_s + 64, s);
+          tmem_ld_32x32_at<96>(t_s + 96, s);
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free);
+          fix(Int<0>());
+          fix(Int<1>());
+          fix(Int<2>());
+          fix(Int<3>());
+          const float m_new = fmaxf(m_ref, fmaf(scale, fmaxf(mx0, mx1), shift));
           if (j == 0) {
             m_ref = m_new;
-          } else if (__any_sync(0xffffffffu, (m_new - m_ref) > max_lag)) {
-            if (!pv_waited) wait_pv();
+          } else if (__any_sync(0xffffffffu, exists && m_new - m_ref > kLag)) {
+            wait_pv();
             const float f = m_new == m_ref ? 1.0f : ex2(m_ref - m_new);
 #pragma unroll
             for (int cb = 0; cb < kHeadDim; cb += 32) {
@@ -607,135 +713,19 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             l_run *= f;
             m_ref = m_new;
           }
-        };
-        // what the exponent subtracts: a row that has seen nothing yet keeps its masked scores at 2^-inf
-        auto reference = [&]() { return m_ref == -INFINITY ? 0.f : m_ref; };
-        const float* slice = nullptr;
-        bool is_flat = true;
-        float flat_bias = 0.f;
-        if (BIAS) {
-          const int bs = static_cast<int>(step % kStages);
-          mbar_wait_anyway_lane(&bias_full[bs], (step / kStages) & 1u, abort_flag, args.status, kSoftmaxTimeout);
-          slice = reinterpret_cast<const float*>(smem + L::kBias + bs * sizeof(BiasSlice)) + 127 - r;
-          is_flat = flat[bs] != 0;
-          if (is_flat) flat_bias = slice[256 - 127 + r];
-        }
-        const bool whole = __all_sync(0xffffffffu, !exists || (b_lo <= u0 && b_hi >= u0 + kRows));
-        if (idle) {
-          if (lane == 0) mbar_arrive(s_free);
-          if (!pv_waited) wait_pv();  // (or this warp's next p_full would count for the tile that the others are still at)
-        } else if (whole) {
-          // every row of the warp sees every key of the tile
-          uint32_t s[128];
-          tmem_ld_32x32_at<0>(t_s, s);
-          tmem_ld_32x32_at<32>(t_s + 32, s);
-          tmem_ld_32x32_at<64>(t_s + 64, s);
-          tmem_ld_32x32_at<96>(t_s + 96, s);
-          tmem_ld_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_free);
-          float scale = c, shift = flat_bias;
-          if (BIAS && !is_flat) {  // (whole tiles lie in the second run)
-            const float* b = slice + 256;
-#pragma unroll
-            for (int i = 0; i < 128; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b[i]));
-            scale = 1.0f;
-          }
-          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 128; i += 8) {
-            mx0 = max3(mx0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-            mx1 = max3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-            mx2 = max3(mx2, __uint_as_float(s[i + 4]), __uint_as_float(s[i + 5]));
-            mx3 = max3(mx3, __uint_as_float(s[i + 6]), __uint_as_float(s[i + 7]));
-          }
-          move_reference(fmaxf(m_ref, fmaf(scale, max3(mx0, mx1, fmaxf(mx2, mx3)), shift)));
-          const float minus = shift - reference();
-          unsigned long long l0 = pack_f32x2(0.f, 0.f), l1 = l0;
-          const unsigned long long sc2 = pack_f32x2(scale, scale), mi2 = pack_f32x2(minus, minus);
-          uint32_t pk[64];
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            float t0, t1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc2, mi2), t0, t1);
-            const float p0 = ex2(t0), p1 = ex2(t1);
-            if (i & 1) l1 = add_f32x2(l1, pack_f32x2(p0, p1)); else l0 = add_f32x2(l0, pack_f32x2(p0, p1));
-            pk[i] = pack_half2(p0, p1);
-          }
+          minus = shift - (m_ref == -INFINITY ? 0.f : m_ref);  // (a row that has seen nothing yet keeps its masked scores at 2^-inf)
+          weigh(Int<0>());
+          weigh(Int<1>());
+          wait_pv();
+          store(Int<0>());
+          store(Int<1>());
+          weigh(Int<2>());
+          store(Int<2>());
+          weigh(Int<3>());
+          store(Int<3>());
           float la, lb;
           unpack_f32x2(add_f32x2(l0, l1), la, lb);
           l_run += la + lb;
-          if (!pv_waited) wait_pv();
-          store_p<0>(t_p, pk);
-          store_p<16>(t_p + 16, pk);
-          store_p<32>(t_p + 32, pk);
-          store_p<48>(t_p + 48, pk);
-        } else {
-          // Some keys are masked for some row: by chunks of 32 keys, those that any row of the warp sees, in two passes over S.
-          auto seen = [&](int c0) { return bits_between(0, a_hi - u0 - c0) | bits_between(b_lo - u0 - c0, b_hi - u0 - c0); };
-          auto scores = [&](int c0, uint32_t w, float (&v)[32]) {
-            uint32_t raw[32];
-            tmem_ld_32x32(t_s + c0, raw);
-            tmem_ld_wait();
-            if (BIAS && !is_flat) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float* b = slice + (u0 + c0 + 16 * h < keys.ns ? 0 : 256) + c0;
-#pragma unroll
-                for (int i = 16 * h; i < 16 * h + 16; ++i) v[i] = fmaf(__uint_as_float(raw[i]), c, b[i]);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = BIAS ? fmaf(__uint_as_float(raw[i]), c, flat_bias) : __uint_as_float(raw[i]) * c;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = ((w >> i) & 1u) ? v[i] : -INFINITY;
-          };
-          float mx = -INFINITY;
-#pragma unroll 1
-          for (int c0 = 0; c0 < kRows; c0 += 32) {
-            const uint32_t w = seen(c0);
-            if (!__any_sync(0xffffffffu, exists && w != 0u)) continue;
-            float v[32];
-            scores(c0, w, v);
-            float m0 = -INFINITY, m1 = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              m0 = max3(m0, v[i], v[i + 1]);
-              m1 = max3(m1, v[i + 2], v[i + 3]);
-            }
-            mx = fmaxf(mx, fmaxf(m0, m1));
-          }
-          move_reference(fmaxf(m_ref, mx));
-          if (!pv_waited) wait_pv();
-          const float m = reference();
-          const int used = (min(kRows, keys.total - u0) + 15) & ~15;  // keys that are multiplied
-#pragma unroll 1
-          for (int c0 = 0; c0 < max(used, 16); c0 += 32) {
-            const uint32_t w = seen(c0);
-            uint32_t pk[16];
-            if (__any_sync(0xffffffffu, exists && w != 0u)) {
-              float v[32];
-              scores(c0, w, v);
-              float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float p0 = ex2(v[2 * i] - m), p1 = ex2(v[2 * i + 1] - m);
-                l0 += p0;
-                l1 += p1;
-                pk[i] = pack_half2(p0, p1);
-              }
-              l_run += l0 + l1;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) pk[i] = 0u;
-            }
-            tmem_st_32x16(t_p + (c0 >> 1), pk);
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_free);
         }
         if (BIAS) {
           __syncwarp();
