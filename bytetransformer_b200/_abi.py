@@ -58,7 +58,8 @@ class bt_window_attention_args(C.Structure):
                [(n, C.c_void_p) for n in ("q_offsets", "k_offsets", "k_lens")] + \
                [(n, C.c_int) for n in ("batch", "head_num", "kv_head_num", "q_rows", "k_rows", "max_q_len", "max_k_len",
                                        "left", "right", "sinks")] + \
-               [("scale", C.c_float), ("distance_bias", C.c_void_p), ("bias_len", C.c_int), ("bias_left", C.c_int)]
+               [("scale", C.c_float), ("distance_bias", C.c_void_p), ("bias_len", C.c_int), ("bias_left", C.c_int),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 _vp, _i, _f, _sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
@@ -101,6 +102,7 @@ SIGNATURES = {
     "bt_relative_position_bias_grad": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
     "bt_add_residual_rmsnorm": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _f, _vp]),
     "bt_add_residual_rmsnorm_e4m3": (_i, [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _f, _vp]),
+    "bt_window_attention_workspace": (_i, [_i, _i, _i, _i, _i, _i, _i, C.POINTER(_sz)]),
     "bt_window_attention": (_i, [C.POINTER(bt_window_attention_args), _vp]),
     "bt_profile_enable": (_i, [_vp, _i]),
     "bt_profile_read": (_i, [_vp, C.POINTER(C.c_double), C.POINTER(C.c_longlong)]),

@@ -9,7 +9,8 @@
 // and a run around the tile; the two are laid end to end ("virtual" keys: the first run, in steps of 16, then the second) and
 // walked in tiles of 128, so a handful of first tokens does not cost a tile of its own and the window starts wherever
 // the first row's does, not at a multiple of 128.  The tile that holds the seam is fetched in boxes of 16 keys.
-// The pipeline is that of mha_persistent_kernel (mha_sm100.cu): CTAs of 256 threads, two to an SM, that take over waiting
+// window_few_kernel: calls of few queries (single tokens), see there.
+// The pipeline of the first is that of mha_persistent_kernel (mha_sm100.cu): CTAs of 256 threads, two to an SM, that take over waiting
 // blocks; one warp loads, one issues the MMAs, four own a query row per thread; S, P and O live in tensor memory.
 #include <math.h>
 
@@ -41,8 +42,7 @@ struct WindowArgs {
   const float* bias;  // [heads, bias_n]: distances -bias_left ..., the outermost values beyond
   int bias_n, bias_left;
   int* status;
-  int tma_out;
-  int take_over;  // the grid has more blocks than are resident
+    int take_over;  // the grid has more blocks than are resident
   int by_rows;    // the grid has blocks for as many items as offsets that rise can hold, which others may exceed
 };
 
@@ -778,7 +778,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           *reinterpret_cast<uint4*>(stage_out + lane * 128 + (((4 * h + u) ^ (lane & 7)) << 4)) = w;
         }
       }
-      const bool whole_slab = args.tma_out != 0 && warp * 32 + 32 <= it.rows;
+      const bool whole_slab = warp * 32 + 32 <= it.rows;
       if (whole_slab) fence_proxy_async_smem();
       __syncwarp();
       if (whole_slab) {
@@ -833,6 +833,301 @@ cudaError_t launch_window(const CUtensorMap (&tm)[6], WindowArgs a, int sms, cud
                     tm[4], tm[5], a);
 }
 
+// -------------------------------------------------------------------------------------------- few queries
+// The queries of a sequence times the heads that share a key/value head are at most 16 rows: what a step of generation
+// asks for.  The keys are read once and that is the time it takes, so a CTA belongs to a (sequence, key/value head, range of
+// its virtual keys) and all rows that need them; each of its four warps walks every fourth 32 keys with a softmax of its
+// own, on mma.sync (16 x 8 x 16: a tcgen05 tile would be one eighth full at best, and its operands would pass through shared
+// memory).  K and V go from global memory straight into the operands' registers: the order of the 64 dimensions in q.k and of
+// the output columns in p.v is free, and is chosen so that a thread's registers are 16 contiguous bytes of a row.
+// The next keys are requested as soon as a product has taken the last ones.
+constexpr int kFewRows = 16;
+constexpr int kFewWarps = 4;
+constexpr int kFewKeys = 32;  // of a step
+
+struct FewArgs {
+  WindowArgs w;
+  const __half *q, *k, *v;
+  long long q_stride, k_stride, v_stride;
+  int splits;
+  float* partial_o;  // [batch, kv_heads, splits, 16, 64]
+  float2* partial_ml;  // [batch, kv_heads, splits, 16]: reference and sum
+};
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load16(const __half* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// The sequence of a CTA: rows of its queries, position of the first, its keys.  false: nothing to do.
+__device__ __forceinline__ bool few_item(const WindowArgs& a, int b, Item& it) {
+  const int start = a.q_offsets[b], len = a.q_offsets[b + 1] - start;
+  const int k_row = a.k_offsets[b], room = a.k_offsets[b + 1] - k_row;
+  const int k_len = a.k_lens != nullptr ? a.k_lens[b] : room;
+  if (start < 0 || len < 0 || len > a.max_q || start > a.q_rows - len || k_row < 0 || k_len < 0 || k_len > a.max_k || k_len > room ||
+      k_row > a.k_rows - room) {
+    if (threadIdx.x == 0 && a.status != nullptr) atomicCAS(a.status, 0, kStatusBadOffsets);
+    return false;
+  }
+  it.q_row = start;
+  it.rows = len;
+  it.p0 = k_len - len;
+  it.k_row = k_row;
+  it.k_len = k_len;
+  return len > 0;
+}
+
+template <bool BIAS>
+__global__ void __launch_bounds__(kFewWarps * 32) window_few_kernel(const __grid_constant__ FewArgs a) {
+  __shared__ float o_all[kFewWarps][kFewRows][kHeadDim + 4];
+  __shared__ float2 ml_all[kFewWarps][kFewRows];
+  pdl_launch_dependents();
+  const WindowArgs& w = a.w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int split = blockIdx.x, kv = blockIdx.y, b = blockIdx.z;
+  pdl_wait();
+  Item it;
+  if (!few_item(w, b, it)) return;
+  const Keys keys = keys_of(w, it);
+  const int rows = it.rows * w.group;
+  // this CTA's virtual keys, in whole steps
+  const int steps = (keys.total + kFewKeys - 1) / kFewKeys;
+  const int first = static_cast<int>(static_cast<long long>(steps) * split / a.splits);
+  const int last = static_cast<int>(static_cast<long long>(steps) * (split + 1) / a.splits);
+
+  // Queries: row r is query r / group, head r % group.  Dimensions 32 i + 8 c + 4 s + {0, 1} and + {2, 3} stand at the places 2c,
+  // 2c + 1 and 2c + 8, 2c + 9 of the product's step 2 i + s.
+  uint32_t qa[2][2][4];  // [row half][i][register]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = g + 8 * h;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows)
+        v = load16(a.q + static_cast<long long>(it.q_row + r / w.group) * a.q_stride + (kv * w.group + r % w.group) * kHeadDim + i * 32 + c * 8);
+      qa[h][i][0] = v.x;
+      qa[h][i][1] = v.y;
+      qa[h][i][2] = v.z;
+      qa[h][i][3] = v.w;
+    }
+  }
+  // virtual keys that the thread's two rows see: [0, a_hi) and [b_lo, b_hi); their bias rows
+  int a_hi[2], b_lo[2], b_hi[2], pos[2];
+  const float* bias[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = min(g + 8 * h, rows - 1);
+    pos[h] = it.p0 + r / w.group;
+    const int hi = w.right < 0 ? it.k_len : min(it.k_len, pos[h] + w.right + 1);
+    a_hi[h] = w.left < 0 ? 0 : min(w.sinks, hi);
+    b_lo[h] = keys.ns + max((w.left < 0 ? 0 : pos[h] - w.left) - keys.ws, 0);
+    b_hi[h] = keys.ns + hi - keys.ws;
+    bias[h] = BIAS ? w.bias + static_cast<long long>(kv * w.group + r % w.group) * w.bias_n : nullptr;
+  }
+  const __half* kb = a.k + static_cast<long long>(it.k_row) * a.k_stride + kv * kHeadDim;
+  const __half* vb = a.v + static_cast<long long>(it.k_row) * a.v_stride + kv * kHeadDim;
+  auto key_of = [&](int u) {  // (keys behind the last one: the last one's row, with a weight of 0)
+    u = min(u, keys.total - 1);
+    return u < keys.ns ? u : keys.ws + u - keys.ns;
+  };
+  uint4 kr[4][2], vr[2][4];  // K: keys 8 n + g, dimensions 32 i + 8 c ..; V: keys 16 s + {2c, 2c + 1, 2c + 8, 2c + 9}, dimensions 8 g ..
+  auto load_k = [&](int u0) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const __half* p = kb + static_cast<long long>(key_of(u0 + 8 * n + g)) * a.k_stride + c * 8;
+      kr[n][0] = load16(p);
+      kr[n][1] = load16(p + 32);
+    }
+  };
+  auto load_v = [&](int u0) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        vr[s][x] = load16(vb + static_cast<long long>(key_of(u0 + 16 * s + 2 * c + (x & 1) + (x >> 1) * 8)) * a.v_stride + g * 8);
+  };
+  float o[8][4];
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[t][i] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  if (first + warp < last) {
+    load_k((first + warp) * kFewKeys);
+    load_v((first + warp) * kFewKeys);
+  }
+#pragma unroll 1
+  for (int step = first + warp; step < last; step += kFewWarps) {
+    const int u0 = step * kFewKeys;
+    const bool more = step + kFewWarps < last;
+    float s[4][4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mma_16816(s[n], qa[0][i][0], qa[1][i][0], qa[0][i][1], qa[1][i][1], kr[n][i].x, kr[n][i].y);
+        mma_16816(s[n], qa[0][i][2], qa[1][i][2], qa[0][i][3], qa[1][i][3], kr[n][i].z, kr[n][i].w);
+      }
+    }
+    if (more) load_k(u0 + kFewWarps * kFewKeys);
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // row g + 8 (i / 2), key 8 n + 2 c + i % 2
+        const int h = i >> 1, u = u0 + 8 * n + 2 * c + (i & 1);
+        const bool seen = u < a_hi[h] || (u >= b_lo[h] && u < b_hi[h]);
+        float x = s[n][i] * w.scale_log2e;
+        if (BIAS) x = fmaf(__ldg(bias[h] + min(max(key_of(u) - pos[h] + w.bias_left, 0), w.bias_n - 1)), 1.4426950408889634f, x);
+        s[n][i] = seen ? x : -INFINITY;
+        top[h] = fmaxf(top[h], s[n][i]);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      const float m_new = fmaxf(m[h], top[h]);
+      const float f = m_new == m[h] ? 1.0f : ex2(m[h] - m_new);
+      m[h] = m_new;
+      l[h] *= f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        o[t][2 * h] *= f;
+        o[t][2 * h + 1] *= f;
+      }
+    }
+    uint32_t p[4][2];  // [n][row half]
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float ref = m[h] == -INFINITY ? 0.f : m[h];
+        const float p0 = ex2(s[n][2 * h] - ref), p1 = ex2(s[n][2 * h + 1] - ref);
+        l[h] += p0 + p1;
+        p[n][h] = pack_half2(p0, p1);
+      }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const uint32_t v0[4] = {vr[st][0].x, vr[st][0].y, vr[st][0].z, vr[st][0].w}, v1[4] = {vr[st][1].x, vr[st][1].y, vr[st][1].z, vr[st][1].w};
+      const uint32_t v2[4] = {vr[st][2].x, vr[st][2].y, vr[st][2].z, vr[st][2].w}, v3[4] = {vr[st][3].x, vr[st][3].y, vr[st][3].z, vr[st][3].w};
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {  // output column n of the product t is dimension 8 n + t: t picks a half of the registers
+        const uint32_t sel = (t & 1) ? 0x7632u : 0x5410u;
+        mma_16816(o[t], p[2 * st][0], p[2 * st][1], p[2 * st + 1][0], p[2 * st + 1][1], __byte_perm(v0[t >> 1], v1[t >> 1], sel),
+                  __byte_perm(v2[t >> 1], v3[t >> 1], sel));
+      }
+    }
+    if (more) load_v(u0 + kFewWarps * kFewKeys);
+  }
+  // The warps' results: O, reference and sum of each row
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (c == 0) ml_all[warp][g + 8 * h] = make_float2(m[h], l[h]);
+    float* dst = &o_all[warp][g + 8 * h][16 * c];
+#pragma unroll
+    for (int t = 0; t < 8; t += 4) {
+      *reinterpret_cast<float4*>(dst + t) = make_float4(o[t][2 * h], o[t + 1][2 * h], o[t + 2][2 * h], o[t + 3][2 * h]);
+      *reinterpret_cast<float4*>(dst + 8 + t) = make_float4(o[t][2 * h + 1], o[t + 1][2 * h + 1], o[t + 2][2 * h + 1], o[t + 3][2 * h + 1]);
+    }
+  }
+  __syncthreads();
+  // eight columns of a row to a thread
+  const int r = threadIdx.x >> 3, col = (threadIdx.x & 7) * 8;
+  if (r >= rows) return;
+  float top = -INFINITY, sum = 0.f, acc[8];
+#pragma unroll
+  for (int i = 0; i < kFewWarps; ++i) top = fmaxf(top, ml_all[i][r].x);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFewWarps; ++i) {
+    const float2 ml = ml_all[i][r];
+    if (ml.x == -INFINITY) continue;  // this warp has seen no key of the row
+    const float f = ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) acc[x] = fmaf(o_all[i][r][col + x], f, acc[x]);
+  }
+  if (a.splits == 1) {
+    const float inv = 1.0f / sum;
+    uint4 out = make_uint4(0u, 0u, 0u, 0u);
+    if (sum != 0.f)
+      out = make_uint4(pack_half2(acc[0] * inv, acc[1] * inv), pack_half2(acc[2] * inv, acc[3] * inv), pack_half2(acc[4] * inv, acc[5] * inv),
+                       pack_half2(acc[6] * inv, acc[7] * inv));
+    *reinterpret_cast<uint4*>(w.out + static_cast<long long>(it.q_row + r / w.group) * w.out_stride + (kv * w.group + r % w.group) * kHeadDim +
+                              col) = out;
+  } else {
+    const long long at = ((static_cast<long long>(b) * gridDim.y + kv) * a.splits + split) * kFewRows + r;
+    if (col == 0) a.partial_ml[at] = make_float2(top, sum);
+    float4* dst = reinterpret_cast<float4*>(a.partial_o + at * kHeadDim + col);
+    dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  }
+}
+
+// The splits of a (sequence, key/value head) put together: four columns of a row to a thread.
+__global__ void __launch_bounds__(kFewRows * 16) window_few_join_kernel(const __grid_constant__ FewArgs a) {
+  pdl_launch_dependents();
+  const WindowArgs& w = a.w;
+  const int kv = blockIdx.x, b = blockIdx.y, r = threadIdx.x >> 4, col = (threadIdx.x & 15) * 4;
+  pdl_wait();
+  Item it;
+  if (!few_item(w, b, it) || r >= it.rows * w.group) return;
+  const long long at = (static_cast<long long>(b) * gridDim.x + kv) * a.splits * kFewRows + r;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.partial_ml[at + s * kFewRows].x);
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.partial_ml[at + s * kFewRows];
+    const float4 o = *reinterpret_cast<const float4*>(a.partial_o + (at + s * kFewRows) * kHeadDim + col);
+    if (ml.x == -INFINITY) continue;
+    const float f = ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    acc.x = fmaf(o.x, f, acc.x);
+    acc.y = fmaf(o.y, f, acc.y);
+    acc.z = fmaf(o.z, f, acc.z);
+    acc.w = fmaf(o.w, f, acc.w);
+  }
+  const float inv = 1.0f / sum;
+  uint2 out = make_uint2(0u, 0u);
+  if (sum != 0.f) out = make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
+  *reinterpret_cast<uint2*>(w.out + static_cast<long long>(it.q_row + r / w.group) * w.out_stride + (kv * w.group + r % w.group) * kHeadDim +
+                            col) = out;
+}
+
+// Whether a call takes the kernel for few queries, and into how many ranges it cuts a sequence's keys (0: the other kernel).
+// Enough CTAs that every SM holds four of them, as long as a range keeps 128 keys.
+int few_splits(int batch, int kv_heads, int group, int max_q, int max_k, int left, int sinks) {
+  if (static_cast<long long>(max_q) * group > kFewRows || batch > 65535 || kv_heads > 65535) return 0;
+  long long keys = max_k;
+  if (left >= 0) keys = static_cast<long long>(left) + max_q + sinks + kSeam < keys ? static_cast<long long>(left) + max_q + sinks + kSeam : keys;
+  const long long items = static_cast<long long>(batch) * kv_heads;
+  long long splits = (4 * 148 + items - 1) / items;
+  const long long most = (keys + 127) / 128;
+  if (splits > most) splits = most;
+  if (splits > 148) splits = 148;
+  return splits < 1 ? 1 : static_cast<int>(splits);
+}
+size_t few_workspace(long long items, int splits) {
+  return splits <= 1 ? 0 : static_cast<size_t>(items) * splits * kFewRows * (kHeadDim * 4 + 8);
+}
+
+template <bool BIAS>
+cudaError_t launch_few(const FewArgs& a, int kv_heads, cudaStream_t stream) {
+  cudaError_t e = launch_pdl(window_few_kernel<BIAS>, dim3(a.splits, kv_heads, a.w.batch), dim3(kFewWarps * 32), 0, stream, a);
+  if (e == cudaSuccess && a.splits > 1) e = launch_pdl(window_few_join_kernel, dim3(kv_heads, a.w.batch), dim3(kFewRows * 16), 0, stream, a);
+  return e;
+}
+
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 struct DeviceFacts {
@@ -869,6 +1164,16 @@ constexpr int kMaxLength = (1 << 30) - 1;
 }  // namespace bt
 
 using namespace bt;
+
+extern "C" int bt_window_attention_workspace(int batch, int head_num, int kv_head_num, int max_q_len, int max_k_len, int left, int sinks,
+                                             size_t* bytes) {
+  if (!bytes || batch <= 0 || head_num <= 0 || head_num > 1024 || kv_head_num <= 0 || head_num % kv_head_num != 0 || max_q_len <= 0 ||
+      max_q_len > kMaxLength || max_k_len < 0 || max_k_len > kMaxLength || sinks < 0)
+    return BT_ERR_INVALID_ARG;
+  *bytes = few_workspace(static_cast<long long>(batch) * kv_head_num,
+                         few_splits(batch, kv_head_num, head_num / kv_head_num, max_q_len, max_k_len, left, sinks));
+  return BT_OK;
+}
 
 extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stream_v) {
   if (a == nullptr || !a->q || !a->out || !a->q_offsets || !a->k_offsets) return BT_ERR_INVALID_ARG;
@@ -910,6 +1215,20 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
   w.bias_n = a->bias_len;
   w.bias_left = a->bias_left;
   w.status = dev.status;
+  const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+  cudaError_t e;
+  const int splits = few_splits(a->batch, a->kv_head_num, w.group, a->max_q_len, a->max_k_len, a->left, a->sinks);
+  if (splits > 0) {
+    const long long items = static_cast<long long>(a->batch) * a->kv_head_num;
+    const size_t need = few_workspace(items, splits);
+    if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return BT_ERR_WORKSPACE;
+    if (!aligned(a->workspace, 16)) return BT_ERR_INVALID_ARG;
+    FewArgs f{w, static_cast<const __half*>(a->q), static_cast<const __half*>(a->k), static_cast<const __half*>(a->v),
+              a->q_row_stride, a->k_row_stride, a->v_row_stride, splits, static_cast<float*>(a->workspace), nullptr};
+    f.partial_ml = reinterpret_cast<float2*>(f.partial_o + items * splits * kFewRows * kHeadDim);
+    e = w.bias != nullptr ? launch_few<true>(f, a->kv_head_num, stream) : launch_few<false>(f, a->kv_head_num, stream);
+    return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;
+  }
   // Without any key rows the loads of the one masked tile that an item walks need some rows: those of q do.
   const bool none = a->k_rows == 0;
   const void *k = none ? a->q : a->k, *v = none ? a->q : a->v;
@@ -921,9 +1240,7 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
                   make_tmap_2d(&tm[3], k, k_rows, kv_cols, k_ld, 64, kSeam) && make_tmap_2d(&tm[4], v, k_rows, kv_cols, v_ld, 64, kSeam) &&
                   make_tmap_2d(&tm[5], a->out, a->q_rows, q_cols, a->out_row_stride, 64, 32);
   if (!ok) return BT_ERR_CUDA;
-  w.tma_out = 1;
-  const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  const cudaError_t e = w.bias != nullptr ? launch_window<true>(tm, w, dev.sms, stream) : launch_window<false>(tm, w, dev.sms, stream);
+  e = w.bias != nullptr ? launch_window<true>(tm, w, dev.sms, stream) : launch_window<false>(tm, w, dev.sms, stream);
   if (e == cudaErrorInvalidValue) return BT_ERR_INVALID_ARG;
   return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;
 }

@@ -677,11 +677,19 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
         rows, k_rows = q.shape[0], k.shape[0]
         if rows == 0 or batch == 0:
             return out
+        ws, n = None, 0
+        if max_q_len * heads <= 16 * kv_heads:  # few queries: the keys may be cut into ranges
+            size = C.c_size_t()
+            if lib.bt_window_attention_workspace(batch, heads, kv_heads, max_q_len, max_k_len, left, sinks,
+                                                 C.byref(size)) == _abi.BT_OK and size.value:
+                n = size.value
+                ws = torch.empty(n, dtype=torch.int8, device=device)
         a = _abi.bt_window_attention_args(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
             out.stride(0), q_offsets.data_ptr(), k_offsets.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
             batch, heads, kv_heads, rows, k_rows, max_q_len, max_k_len, left, right, sinks, scale,
-            distance_bias.data_ptr() if distance_bias is not None else None, n_bias, bias_left)
+            distance_bias.data_ptr() if distance_bias is not None else None, n_bias, bias_left,
+            ws.data_ptr() if n else None, n)
         rc = lib.bt_window_attention(C.byref(a), stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_window_attention")

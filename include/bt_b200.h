@@ -373,7 +373,13 @@ typedef struct bt_window_attention_args {
   float scale; /* > 0; 1 / sqrt(64) is the usual one */
   const float* distance_bias;
   int bias_len, bias_left;
+  void* workspace; /* bt_window_attention_workspace() bytes, 16-byte aligned (0 bytes: may be NULL); calls that may overlap */
+  size_t workspace_bytes; /* need one each, contents undefined before and after */
 } bt_window_attention_args;
+/* Bytes for the partial results of calls of few queries (max_q_len * head_num / kv_head_num <= 16), whose keys are cut into
+ * ranges where there are few sequences; 0 for all others.  The same values as in the call. */
+int bt_window_attention_workspace(int batch, int head_num, int kv_head_num, int max_q_len, int max_k_len, int left, int sinks,
+                                  size_t* bytes);
 int bt_window_attention(const bt_window_attention_args* args, void* stream);
 
 /* ---- launch accounting and per-kernel timing ------------------------------ */

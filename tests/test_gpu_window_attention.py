@@ -148,6 +148,36 @@ def test_single_tokens(cuda_device, left, heads, kv, with_bias):
           bias, 64)
 
 
+@pytest.mark.parametrize("left,right,sinks", [(-1, -1, 0), (-1, 0, 0), (40, 0, 20), (3, 2, 1), (700, 9, 100), (0, 0, 0)])
+@pytest.mark.parametrize("q_len,heads,kv", [(16, 3, 3), (4, 8, 2), (5, 9, 3), (2, 8, 1)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_few_queries(cuda_device, left, right, sinks, q_len, heads, kv, with_bias):
+    """Drafted tokens and the like: up to q_len queries for each sequence, one range of keys or several."""
+    q_lens, k_lens, room = [q_len, 1, 0, q_len, min(3, q_len), q_len], [900, 70, 5, 2, 0, 2500], 2500
+    g = torch.Generator().manual_seed(q_len + heads)
+    q = torch.randn(sum(q_lens), heads * D, generator=g).half().to(cuda_device)
+    cache = torch.full((len(k_lens), room, 2 * kv * D), float("nan")).half()
+    for b, n in enumerate(k_lens):
+        cache[b, :n] = torch.randn(n, 2 * kv * D, generator=g).half()
+    cache = cache.view(-1, 2 * kv * D).to(cuda_device)
+    q_off = torch.tensor([0] + q_lens).cumsum(0).int().to(cuda_device)
+    k_off = (torch.arange(len(k_lens) + 1) * room).int().to(cuda_device)
+    bias = torch.randn(heads, 65, device=cuda_device) if with_bias else None
+    check(q, cache[:, :kv * D], cache[:, kv * D:], q_off, k_off, q_len, room, torch.tensor(k_lens).int().to(cuda_device), left, right,
+          sinks, bias, 32)
+
+
+def test_single_tokens_of_many_sequences(cuda_device):
+    """More sequences than there are ranges to cut: the result is written without the second kernel."""
+    lens = [(i * 97) % 300 for i in range(700)]
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(700, 2 * D, generator=g).half().to(cuda_device)
+    kv = torch.randn(sum(lens), 2 * D, generator=g).half().to(cuda_device)
+    q_off = torch.arange(701, dtype=torch.int32, device=cuda_device)
+    k_off = torch.tensor([0] + lens).cumsum(0).int().to(cuda_device)
+    check(q, kv[:, :D], kv[:, D:], q_off, k_off, 1, 300, None, 200, 0, 4)
+
+
 def test_large_scores(cuda_device):
     """References that move in every tile, weights that all but one vanish."""
     q, k, v, off = packed([900, 130], 2, 2, cuda_device, seed=5)

@@ -72,3 +72,36 @@ def test_python_refuses_host_tensors(lib):
         E.relative_position_bias_grad(torch.zeros(2, 8, 8), 32)
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         E.add_residual_rmsnorm(t, None, t[0])
+
+
+def window(lib, **change):
+    f = dict(q=P, k=P, v=P, out=P, q_row_stride=768, k_row_stride=768, v_row_stride=768, out_row_stride=768, q_offsets=P,
+             k_offsets=P, k_lens=None, batch=2, head_num=12, kv_head_num=12, q_rows=100, k_rows=100, max_q_len=60, max_k_len=60,
+             left=-1, right=-1, sinks=0, scale=0.125, distance_bias=None, bias_len=0, bias_left=0, workspace=None, workspace_bytes=0)
+    f.update(change)
+    return lib.bt_window_attention(C.byref(_abi.bt_window_attention_args(**f)), None)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q_offsets=None), dict(k_offsets=None), dict(q=P + 8),
+    dict(k=P + 2), dict(v=P + 4), dict(out=P + 8), dict(q_offsets=P + 2), dict(k_lens=P + 1), dict(distance_bias=P + 2, bias_len=9),
+    dict(q_row_stride=760), dict(k_row_stride=767), dict(v_row_stride=772), dict(out_row_stride=0), dict(q_row_stride=(1 << 32) + 8),
+    dict(head_num=0), dict(head_num=1025), dict(kv_head_num=0), dict(kv_head_num=5), dict(batch=0), dict(q_rows=0), dict(k_rows=-1),
+    dict(max_q_len=0), dict(max_q_len=1 << 30), dict(max_k_len=-1), dict(max_k_len=1 << 30), dict(sinks=-1), dict(scale=0.0),
+    dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(distance_bias=P, bias_len=0),
+    dict(distance_bias=P, bias_len=5, bias_left=5), dict(distance_bias=P, bias_len=5, bias_left=-1)])
+def test_window(lib, change):
+    assert window(lib, **change) == _abi.BT_ERR_INVALID_ARG
+    assert lib.bt_window_attention(None, None) == _abi.BT_ERR_INVALID_ARG
+
+
+def test_window_workspace(lib):
+    n = C.c_size_t(7)
+    ask = lib.bt_window_attention_workspace
+    assert ask(2, 12, 12, 17, 100, -1, 0, C.byref(n)) == _abi.BT_OK and n.value == 0  # not few queries
+    assert ask(2, 12, 12, 1, 100, -1, 0, C.byref(n)) == _abi.BT_OK and n.value == 0  # 100 keys are one range
+    assert ask(1, 8, 2, 1, 1 << 20, -1, 0, C.byref(n)) == _abi.BT_OK and n.value == 2 * 148 * 16 * (64 * 4 + 8)
+    assert ask(1, 8, 2, 1, 1 << 20, 500, 4, C.byref(n)) == _abi.BT_OK and n.value == 2 * 5 * 16 * (64 * 4 + 8)
+    for bad in [(0, 8, 2, 1, 9, -1, 0), (1, 8, 3, 1, 9, -1, 0), (1, 8, 2, 0, 9, -1, 0), (1, 8, 2, 1, -1, -1, 0), (1, 8, 2, 1, 9, -1, -1)]:
+        assert ask(*bad, C.byref(n)) == _abi.BT_ERR_INVALID_ARG
+    assert ask(1, 8, 2, 1, 9, -1, 0, None) == _abi.BT_ERR_INVALID_ARG
