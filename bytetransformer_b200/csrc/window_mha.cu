@@ -880,7 +880,7 @@ __device__ __forceinline__ bool few_item(const WindowArgs& a, int b, Item& it) {
 }
 
 template <bool BIAS>
-__global__ void __launch_bounds__(kFewWarps * 32) window_few_kernel(const __grid_constant__ FewArgs a) {
+__global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __grid_constant__ FewArgs a) {
   __shared__ float o_all[kFewWarps][kFewRows][kHeadDim + 4];
   __shared__ float2 ml_all[kFewWarps][kFewRows];
   pdl_launch_dependents();
@@ -1073,35 +1073,44 @@ __global__ void __launch_bounds__(kFewWarps * 32) window_few_kernel(const __grid
   }
 }
 
-// The splits of a (sequence, key/value head) put together: four columns of a row to a thread.
-__global__ void __launch_bounds__(kFewRows * 16) window_few_join_kernel(const __grid_constant__ FewArgs a) {
+// The ranges of a row put together: sixteen threads by four columns, each of sixteen groups takes every sixteenth range.
+__global__ void __launch_bounds__(256) window_few_join_kernel(const __grid_constant__ FewArgs a) {
+  __shared__ float4 o_all[16][16];
+  __shared__ float2 ml_all[16];
   pdl_launch_dependents();
   const WindowArgs& w = a.w;
-  const int kv = blockIdx.x, b = blockIdx.y, r = threadIdx.x >> 4, col = (threadIdx.x & 15) * 4;
+  const int r = blockIdx.x, kv = blockIdx.y, b = blockIdx.z, part = threadIdx.x >> 4, x = threadIdx.x & 15;
   pdl_wait();
   Item it;
   if (!few_item(w, b, it) || r >= it.rows * w.group) return;
-  const long long at = (static_cast<long long>(b) * gridDim.x + kv) * a.splits * kFewRows + r;
+  const long long at = (static_cast<long long>(b) * gridDim.y + kv) * a.splits * kFewRows + r;
   float top = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.partial_ml[at + s * kFewRows].x);
+  auto take = [&](float2 ml, float4 o) {
+    if (ml.x == -INFINITY) return;  // no key of the range is seen
+    const float next = fmaxf(top, ml.x), f0 = ex2(top - next), f1 = ex2(ml.x - next);
+    top = next;
+    sum = fmaf(ml.y, f1, sum * f0);
+    acc.x = fmaf(o.x, f1, acc.x * f0);
+    acc.y = fmaf(o.y, f1, acc.y * f0);
+    acc.z = fmaf(o.z, f1, acc.z * f0);
+    acc.w = fmaf(o.w, f1, acc.w * f0);
+  };
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.partial_ml[at + s * kFewRows];
-    const float4 o = *reinterpret_cast<const float4*>(a.partial_o + (at + s * kFewRows) * kHeadDim + col);
-    if (ml.x == -INFINITY) continue;
-    const float f = ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    acc.x = fmaf(o.x, f, acc.x);
-    acc.y = fmaf(o.y, f, acc.y);
-    acc.z = fmaf(o.z, f, acc.z);
-    acc.w = fmaf(o.w, f, acc.w);
+  for (int s = part; s < a.splits; s += 16) {
+    const long long i = at + static_cast<long long>(s) * kFewRows;
+    take(a.partial_ml[i], *reinterpret_cast<const float4*>(a.partial_o + i * kHeadDim + 4 * x));
   }
+  o_all[part][x] = acc;
+  if (x == 0) ml_all[part] = make_float2(top, sum);
+  __syncthreads();
+  if (part != 0) return;
+  for (int i = 1; i < min(16, a.splits); ++i) take(ml_all[i], o_all[i][x]);
   const float inv = 1.0f / sum;
   uint2 out = make_uint2(0u, 0u);
   if (sum != 0.f) out = make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
   *reinterpret_cast<uint2*>(w.out + static_cast<long long>(it.q_row + r / w.group) * w.out_stride + (kv * w.group + r % w.group) * kHeadDim +
-                            col) = out;
+                            4 * x) = out;
 }
 
 // Whether a call takes the kernel for few queries, and into how many ranges it cuts a sequence's keys (0: the other kernel).
@@ -1124,7 +1133,7 @@ size_t few_workspace(long long items, int splits) {
 template <bool BIAS>
 cudaError_t launch_few(const FewArgs& a, int kv_heads, cudaStream_t stream) {
   cudaError_t e = launch_pdl(window_few_kernel<BIAS>, dim3(a.splits, kv_heads, a.w.batch), dim3(kFewWarps * 32), 0, stream, a);
-  if (e == cudaSuccess && a.splits > 1) e = launch_pdl(window_few_join_kernel, dim3(kv_heads, a.w.batch), dim3(kFewRows * 16), 0, stream, a);
+  if (e == cudaSuccess && a.splits > 1) e = launch_pdl(window_few_join_kernel, dim3(a.w.max_q * a.w.group, kv_heads, a.w.batch), dim3(256), 0, stream, a);
   return e;
 }
 
