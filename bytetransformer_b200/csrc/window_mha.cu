@@ -1114,17 +1114,26 @@ __global__ void __launch_bounds__(256) window_few_join_kernel(const __grid_const
 }
 
 // Whether a call takes the kernel for few queries, and into how many ranges it cuts a sequence's keys (0: the other kernel).
-// Enough CTAs that every SM holds four of them, as long as a range keeps 128 keys.
+// 444 CTAs are resident (three to an SM).  A CTA's time goes with its keys and something like 200 more (its first loads wait for
+// one another, its results are put together), so of the numbers of ranges that leave a range 128 keys the one with the
+// shortest sum over the waves is taken.  us per call, 64 sequences of 4100 keys, 16 heads over 4, by ranges:
+// 1 66, 2 68, 3 56, 6 61; 8 of 4096, 12 heads, 4 ranges (one wave) 23.9, 5 31.6, 7 29.5; 2 of 30000, 12 heads, 18 38.0, 24 46.9.
 int few_splits(int batch, int kv_heads, int group, int max_q, int max_k, int left, int sinks) {
   if (static_cast<long long>(max_q) * group > kFewRows || batch > 65535 || kv_heads > 65535) return 0;
+  constexpr long long kResident = 3 * 148, kOverhead = 200;
   long long keys = max_k;
   if (left >= 0) keys = static_cast<long long>(left) + max_q + sinks + kSeam < keys ? static_cast<long long>(left) + max_q + sinks + kSeam : keys;
   const long long items = static_cast<long long>(batch) * kv_heads;
-  long long splits = (4 * 148 + items - 1) / items;
-  const long long most = (keys + 127) / 128;
-  if (splits > most) splits = most;
-  if (splits > 148) splits = 148;
-  return splits < 1 ? 1 : static_cast<int>(splits);
+  int best = 1;
+  long long best_cost = 0x7fffffffffffffffLL;
+  for (int s = 1; s <= 148 && (s == 1 || s * 128LL <= keys); ++s) {
+    const long long cost = (items * s + kResident - 1) / kResident * (keys / s + kOverhead);
+    if (cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
 }
 size_t few_workspace(long long items, int splits) {
   return splits <= 1 ? 0 : static_cast<size_t>(items) * splits * kFewRows * (kHeadDim * 4 + 8);
