@@ -7,11 +7,17 @@
 //
 // window_mha_kernel: 128 query rows of a head at a time.  The keys that any of them sees are a run of the first keys
 // and a run around the tile; the two are laid end to end ("virtual" keys: the first run, in steps of 16, then the second) and
-// walked in tiles of 128, so a handful of first tokens does not cost a tile of its own and the window starts wherever
-// the first row's does, not at a multiple of 128.  The tile that holds the seam is fetched in boxes of 16 keys.
+// walked in tiles of 64, so a handful of first tokens does not cost a tile of its own and the window starts wherever
+// the first row's does.  The tile that holds the seam is fetched in boxes of 16 keys.
+//   What bounds it is the chain of a softmax (scores from tensor memory, maximum, exponentials, weights back), not the tensor
+//   core: a warp by itself leaves the special-function unit idle more than half of the time.  So two groups of four warps
+//   share the 128 rows, one takes the even tiles, the other the odd ones, each with scores, weights, reference, sum and O of
+//   its own; the two results are put together when the item ends (the groups take turns in that).  With two CTAs to an SM
+//   four warps take turns on each scheduler.
+//   S = Q K^T (128 x 64 x 64) lands in 64 columns of tensor memory; the weights go back over them as fp16 pairs, from where
+//   O += P V takes them; the next S of a group is issued right behind that product.  One thread issues a group's MMAs and
+//   they execute in order, so no barrier stands between P V and the S that overwrites P.
 // window_few_kernel: calls of few queries (single tokens), see there.
-// The pipeline of the first is that of mha_persistent_kernel (mha_sm100.cu): CTAs of 256 threads, two to an SM, that take over waiting
-// blocks; one warp loads, one issues the MMAs, four own a query row per thread; S, P and O live in tensor memory.
 #include <math.h>
 
 #include <mutex>
@@ -24,10 +30,12 @@ namespace bt {
 
 namespace {
 
-constexpr int kRows = 128;  // query rows of a block, keys of a tile
+constexpr int kRows = 128;  // query rows of a block
+constexpr int kKeys = 64;   // keys of a tile
 constexpr int kHeadDim = 64;
-constexpr int kTile = 128 * kHeadDim * 2;  // 16 KiB
-constexpr int kThreads = 256;
+constexpr int kQTile = kRows * kHeadDim * 2;   // 16 KiB
+constexpr int kKvTile = kKeys * kHeadDim * 2;  // 8 KiB
+constexpr int kThreads = 384;  // two groups of four softmax warps; loads, MMAs of either group, bias
 constexpr int kSlots = 4;  // items between the loader and the other roles
 constexpr int kSeam = 16;  // keys of a box of the tile with the seam
 
@@ -70,7 +78,7 @@ __device__ __forceinline__ Keys keys_of(const WindowArgs& a, const Item& it) {
   k.ns = apart ? first : 0;
   k.ws = apart ? lo : 0;
   k.total = max(k.ns + hi - k.ws, 0);
-  k.tiles = max(1, (k.total + kRows - 1) / kRows);
+  k.tiles = max(1, (k.total + kKeys - 1) / kKeys);
   return k;
 }
 
@@ -173,7 +181,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// S = Q K^T of a 128 x 128 tile and the commit to `bar`; called by a whole warp.
+// S = Q K^T of a 128 x 64 tile and the commit to `bar`; called by a whole warp.
 __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint64_t* bar) {
   asm volatile(
       "{\n\t"
@@ -197,7 +205,7 @@ __device__ __forceinline__ void mma_scores(uint32_t d_tmem, uint64_t adesc, uint
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(smem_u32(bar))
       : "memory");
 }
-// O (+)= P V over the first `steps` groups of 16 keys, P from tensor memory; called by a whole warp.
+// O (+)= P V over the first `steps` <= 4 groups of 16 keys, P from tensor memory; called by a whole warp.
 __device__ __forceinline__ void mma_values(uint32_t d_tmem, uint32_t p_tmem, uint64_t vdesc, uint32_t idesc, uint32_t accumulate,
                                            uint32_t steps) {
   asm volatile(
@@ -214,8 +222,7 @@ __device__ __forceinline__ void mma_values(uint32_t d_tmem, uint32_t p_tmem, uin
   "add.u64 b, %2, " B ";\n\t"                   \
   "setp.gt.and.u32 p, %5, " I ", q;\n\t"        \
   "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, t;\n\t"
-      BT_STEP("1", "8", "128") BT_STEP("2", "16", "256") BT_STEP("3", "24", "384") BT_STEP("4", "32", "512")
-      BT_STEP("5", "40", "640") BT_STEP("6", "48", "768") BT_STEP("7", "56", "896")
+      BT_STEP("1", "8", "128") BT_STEP("2", "16", "256") BT_STEP("3", "24", "384")
 #undef BT_STEP
       "}\n" ::"r"(d_tmem),
       "r"(p_tmem), "l"(vdesc), "r"(idesc), "r"(accumulate), "r"(steps)
@@ -242,60 +249,61 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return below_hi & ~below_lo;
 }
 
-// The bias of a tile, for all its rows: value of (column c, row r) at [c - r + 127], in log2 units.  `first`: the columns of
-// the first run of keys, `second` the others.  flat != 0: every value of the tile is second[0].
+// The bias of a tile's second run of keys, for all its rows: value of (column c, row r) at c - r + 127, in log2 units.  Four
+// copies, each an element further on, so that a thread reads its row's values four at a time wherever they start; the pitch
+// keeps the copies that neighbouring rows read in different banks.
+constexpr int kBiasPitch = 200;
 struct BiasSlice {
-  float first[256], second[256];
+  float copy[4][kBiasPitch];
 };
 
 template <bool BIAS>
 struct Layout {
-  static constexpr int kStages = 2;             // K and V tiles each
+  static constexpr int kStages = 2;              // K and V tiles, for each group
   static constexpr int kQStages = BIAS ? 1 : 2;  // (the bias takes the place of the second Q tile)
   static constexpr int kQ = 0;
-  static constexpr int kK = kQ + kQStages * kTile;
-  static constexpr int kV = kK + kStages * kTile;
-  static constexpr int kOut = kV + kStages * kTile;
-  static constexpr int kBias = kOut + kTile;
-  static constexpr int kBar = kBias + (BIAS ? kStages * static_cast<int>(sizeof(BiasSlice)) : 0);
-  static constexpr int kBytes = kBar + 512;
+  static constexpr int kK = kQ + kQStages * kQTile;
+  static constexpr int kV = kK + 2 * kStages * kKvTile;
+  static constexpr int kOut = kV + 2 * kStages * kKvTile;  // 32 rows x 64 bytes for each of the eight warps
+  static constexpr int kBias = kOut + 8 * 32 * 64;
+  static constexpr int kBar = kBias + (BIAS ? 2 * kStages * static_cast<int>(sizeof(BiasSlice)) : 0);
+  static constexpr int kBytes = kBar + 1024;
 };
 
 template <bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
 window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k16,
-                  const __grid_constant__ CUtensorMap tm_v16, const __grid_constant__ CUtensorMap tm_out, const WindowArgs args) {
+                  const __grid_constant__ CUtensorMap tm_v16, const WindowArgs args) {
   using L = Layout<BIAS>;
   constexpr int kStages = L::kStages, kQStages = L::kQStages;
-  constexpr uint32_t kTmemS = 0, kTmemO = 128, kTmemP = 192;
   constexpr int kLoadTimeout = kStatusMhaLoadTimeout, kMmaTimeout = kStatusMhaMmaTimeout, kSoftmaxTimeout = kStatusMhaSoftmaxTimeout;
   extern __shared__ __align__(1024) uint8_t smem[];
 
   pdl_launch_dependents();
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* q_full = bars;                    // [2] by item
-  uint64_t* q_empty = bars + 2;               // [2]
-  uint64_t* k_full = bars + 4;                // [kStages] by tile
-  uint64_t* k_empty = bars + 6;
-  uint64_t* v_full = bars + 8;
-  uint64_t* v_empty = bars + 10;
-  uint64_t* s_full = bars + 12;
-  uint64_t* s_free = bars + 13;
-  uint64_t* p_full = bars + 14;
-  uint64_t* pv_done = bars + 15;
-  uint64_t* o_done = bars + 16;
-  uint64_t* item_full = bars + 17;            // [kSlots]
-  uint64_t* item_empty = bars + 21;           // [kSlots]
-  uint64_t* taken_full = bars + 25;
-  uint64_t* bias_full = bars + 26;            // [kStages] by tile
-  uint64_t* bias_empty = bars + 28;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 30);
+  uint64_t* q_empty = bars + 2;               // [2] both groups' last products with Q
+  uint64_t* k_full = bars + 4;                // [group][kStages] by the group's tiles
+  uint64_t* k_empty = bars + 8;
+  uint64_t* v_full = bars + 12;
+  uint64_t* v_empty = bars + 16;
+  uint64_t* s_full = bars + 20;               // [group] S is there, and the P V before it has retired
+  uint64_t* p_full = bars + 22;               // [group] P is there, V rows blanked
+  uint64_t* o_done = bars + 24;               // [group] the item's last P V has retired
+  uint64_t* merge_full = bars + 26;           // [group][warp] this group's O, reference and sum may be read by the other group
+  uint64_t* merge_empty = bars + 34;          // [group][warp] they have been
+  uint64_t* item_full = bars + 42;            // [kSlots]
+  uint64_t* item_empty = bars + 46;           // [kSlots]
+  uint64_t* taken_full = bars + 50;
+  uint64_t* bias_full = bars + 51;            // [group][kStages] by the group's tiles
+  uint64_t* bias_empty = bars + 55;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 59);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  uint8_t* taken = smem + L::kBar + 256;       // 16 bytes
-  Item* items = reinterpret_cast<Item*>(smem + L::kBar + 272);
-  volatile int* flat = reinterpret_cast<volatile int*>(smem + L::kBar + 272 + kSlots * sizeof(Item));  // [kStages]
-  static_assert(272 + kSlots * sizeof(Item) + kStages * 4 <= 512, "barriers and items");
+  uint8_t* taken = smem + L::kBar + 480;       // 16 bytes
+  Item* items = reinterpret_cast<Item*>(smem + L::kBar + 496);
+  volatile int* flat = reinterpret_cast<volatile int*>(smem + L::kBar + 496 + kSlots * sizeof(Item));  // [group][kStages]
+  static_assert(496 + kSlots * sizeof(Item) + 2 * kStages * 4 <= 1024, "barriers and items");
 
   const int warp = uniform_int(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
@@ -303,7 +311,12 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 1);
+      mbar_init(&q_empty[s], 2);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_done[s], 1);
+    }
+    for (int s = 0; s < 2 * kStages; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 1);
@@ -311,14 +324,13 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(&bias_full[s], 1);
       mbar_init(&bias_empty[s], 4);
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_free, 4);
-    mbar_init(p_full, 4);
-    mbar_init(pv_done, 1);
-    mbar_init(o_done, 1);
+    for (int s = 0; s < 8; ++s) {
+      mbar_init(&merge_full[s], 1);
+      mbar_init(&merge_empty[s], 1);
+    }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&item_full[s], 1);
-      mbar_init(&item_empty[s], BIAS ? 6 : 5);
+      mbar_init(&item_empty[s], BIAS ? 11 : 10);
     }
     mbar_init(taken_full, 1);
     *abort_flag = smem_ok ? 0 : 1;
@@ -328,7 +340,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  if (warp == 5) {
+  if (warp == 8) {
     tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
@@ -337,6 +349,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = uniform_u32(*tmem_slot);
   pdl_wait();
+  // tensor memory of group g: S (and P over it) at 64 g, O at 128 + 64 g
 
   // Each role finds the block's own item by itself; the n-th taken over comes through slot n % kSlots.
   Item it;
@@ -356,12 +369,13 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     __syncwarp();
     if (lane == 0) mbar_arrive(&item_empty[n % kSlots]);
   };
+  // Tile j of item n belongs to group (j + n) & 1, so the group that had one tile more has one less next time.
 
-  if (warp >= 4) {
-    regs_dec<40>();
+  if (warp >= 8) {
+    regs_dec<48>();
     if (!smem_ok) {
       // straight to the teardown
-    } else if (warp == 4) {
+    } else if (warp == 8) {
       // ------------------------------------------------------------------ loads
       int cur_b = 0, cur_first = 0;
       bool have = find_item(args, static_cast<int>(blockIdx.x), cur_b, cur_first, it);
@@ -386,8 +400,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (beyond >= 0) have = find_item(args, beyond++, cur_b, cur_first, it);
         if (!have) beyond = -1;
       };
-      int stage = 0;
-      uint32_t phase = 0;
+      uint32_t count[2] = {0, 0};  // tiles of the groups so far
       bool ok = true;
       for (uint32_t n = 0; have; ++n) {
         const Keys keys = keys_of(args, it);
@@ -396,47 +409,36 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         ok = wait_role(&q_empty[qb], ((n / kQStages) & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
         if (!ok) break;
         if (elect_one()) {
-          mbar_arrive_expect_tx(&q_full[qb], kTile);
-          tma_load_2d(smem + L::kQ + qb * kTile, &tm_q, &q_full[qb], it.head * kHeadDim, it.q_row);
+          mbar_arrive_expect_tx(&q_full[qb], kQTile);
+          tma_load_2d(smem + L::kQ + qb * kQTile, &tm_q, &q_full[qb], it.head * kHeadDim, it.q_row);
         }
         for (int j = 0; j < keys.tiles; ++j) {
-          const int u0 = j * kRows;
-          const bool seam = u0 < keys.ns && u0 + kRows > keys.ns;
+          const int g = (j + static_cast<int>(n)) & 1;
+          const uint32_t cnt = g ? count[1]++ : count[0]++;
+          const int slot = g * kStages + static_cast<int>(cnt % kStages);
+          const uint32_t phase = (cnt / kStages) & 1u;
+          const int u0 = j * kKeys;
+          const bool seam = u0 < keys.ns && u0 + kKeys > keys.ns;
           const int row = it.k_row + (u0 < keys.ns ? u0 : keys.ws + u0 - keys.ns);
-          ok = wait_role(&k_empty[stage], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
-          if (!ok) break;
-          uint8_t* k_dst = smem + L::kK + stage * kTile;
-          uint8_t* v_dst = smem + L::kV + stage * kTile;
-          if (elect_one()) {
-            mbar_arrive_expect_tx(&k_full[stage], kTile);
+          auto fetch = [&](uint8_t* dst, const CUtensorMap* whole, const CUtensorMap* box, uint64_t* bar) {
+            mbar_arrive_expect_tx(bar, kKvTile);
             if (!seam) {
-              tma_load_2d(k_dst, &tm_k, &k_full[stage], kv_col, row);
+              tma_load_2d(dst, whole, bar, kv_col, row);
             } else {
-              for (int s = 0; s < kRows; s += kSeam) {
+              for (int s = 0; s < kKeys; s += kSeam) {
                 const int u = u0 + s;
-                tma_load_2d(k_dst + s * 128, &tm_k16, &k_full[stage], kv_col, it.k_row + (u < keys.ns ? u : keys.ws + u - keys.ns));
+                tma_load_2d(dst + s * 128, box, bar, kv_col, it.k_row + (u < keys.ns ? u : keys.ws + u - keys.ns));
               }
             }
-          }
-          __syncwarp();
-          ok = wait_role(&v_empty[stage], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
+          };
+          ok = wait_role(&k_empty[slot], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
           if (!ok) break;
-          if (elect_one()) {
-            mbar_arrive_expect_tx(&v_full[stage], kTile);
-            if (!seam) {
-              tma_load_2d(v_dst, &tm_v, &v_full[stage], kv_col, row);
-            } else {
-              for (int s = 0; s < kRows; s += kSeam) {
-                const int u = u0 + s;
-                tma_load_2d(v_dst + s * 128, &tm_v16, &v_full[stage], kv_col, it.k_row + (u < keys.ns ? u : keys.ws + u - keys.ns));
-              }
-            }
-          }
+          if (elect_one()) fetch(smem + L::kK + slot * kKvTile, &tm_k, &tm_k16, &k_full[slot]);
           __syncwarp();
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          ok = wait_role(&v_empty[slot], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
+          if (!ok) break;
+          if (elect_one()) fetch(smem + L::kV + slot * kKvTile, &tm_v, &tm_v16, &v_full[slot]);
+          __syncwarp();
         }
         if (!ok) break;
         take_next();
@@ -450,120 +452,87 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         __syncwarp();
       }
-    } else if (warp == 5) {
-      // -------------------------------------------------------------- MMA issue
+    } else if (warp <= 10) {
+      // -------------------------------------------------------------- MMA issue, warp 9 + g for group g
       constexpr uint64_t kDescK = make_smem_desc_hi(16, 1024);
-      constexpr uint64_t kDescV = make_smem_desc_hi(kTile, 1024);
-      constexpr uint32_t kIdescS = make_idesc_f16(128, 128, 0, 0);
-      constexpr uint32_t kIdescO = make_idesc_f16(128, 64, 0, 1);
-      const uint32_t s_q = smem_u32(smem + L::kQ), s_k = smem_u32(smem + L::kK), s_v = smem_u32(smem + L::kV);
-      int st = 0;
-      uint32_t ph = 0, step = 0;
-      auto q_ready = [&](uint32_t n) { return (n / kQStages) & 1u; };
-      auto issue_s = [&](uint32_t n, int stage, bool last) {
-        tc_fence_after();
-        mma_scores(tmem_base + kTmemS, smem_desc(kDescK, s_q + (n % kQStages) * kTile), smem_desc(kDescK, s_k + stage * kTile), kIdescS,
-                   s_full);
-        if (elect_one()) umma_commit(&k_empty[stage]);
-        if (last && elect_one()) umma_commit(&q_empty[n % kQStages]);  // the item's last product with Q
-      };
+      constexpr uint64_t kDescV = make_smem_desc_hi(kKvTile, 1024);
+      constexpr uint32_t kIdescS = make_idesc_f16(128, kKeys, 0, 0);
+      constexpr uint32_t kIdescO = make_idesc_f16(128, kHeadDim, 0, 1);
+      const int g = warp - 9;
+      const uint32_t t_s = tmem_base + 64u * g, t_o = tmem_base + 128u + 64u * g;
+      const uint32_t s_q = smem_u32(smem + L::kQ);
+      const uint32_t s_k = smem_u32(smem + L::kK + g * kStages * kKvTile), s_v = smem_u32(smem + L::kV + g * kStages * kKvTile);
+      uint64_t *kf = k_full + g * kStages, *ke = k_empty + g * kStages, *vf = v_full + g * kStages, *ve = v_empty + g * kStages;
+      uint32_t cnt = 0;  // the group's tiles so far
       bool have = own_item();
-      Keys keys{};
-      if (have) keys = keys_of(args, it);
-      bool s_issued = false;  // the first S of the item about to start
       for (uint32_t n = 0; have; ++n) {
-        if (!s_issued) {
-          // S overwrites its columns: the softmax warps must hold the last one in registers
-          if (step > 0 && !wait_role(s_free, (step - 1u) & 1u, abort_flag, args.status, kMmaTimeout)) break;
-          if (!wait_role(&q_full[n % kQStages], q_ready(n), abort_flag, args.status, kMmaTimeout)) break;
-          if (!wait_role(&k_full[st], ph, abort_flag, args.status, kMmaTimeout)) break;
-          issue_s(n, st, keys.tiles == 1);
-        }
-        s_issued = false;
-        bool next_known = false, next_have = false, ok = true;
-        Keys next{};
-        const int tiles = keys.tiles, total = keys.total;
-        for (int j = 0; j < tiles; ++j, ++step) {
-          const int st_n = st + 1 == kStages ? 0 : st + 1;
-          const uint32_t ph_n = st + 1 == kStages ? ph ^ 1u : ph;
-          // The next S - of this item, or of the next one if that is known and its tiles have landed - goes as soon as the
-          // softmax warps hold the present one
-          ok = wait_role(s_free, step & 1u, abort_flag, args.status, kMmaTimeout);
-          if (!ok) break;
-          if (j + 1 < tiles) {
-            ok = wait_role(&k_full[st_n], ph_n, abort_flag, args.status, kMmaTimeout);
-            if (!ok) break;
-            issue_s(n, st_n, j + 2 == tiles);
-          } else {
-            if (__all_sync(0xffffffffu, mbar_test_wait(&item_full[n % kSlots], parity(n)))) {
-              read_item(n);
-              next_known = true;
-              next_have = it.rows > 0;
-              if (next_have) next = keys_of(args, it);
-            }
-            if (next_have && __all_sync(0xffffffffu, mbar_test_wait(&q_full[(n + 1) % kQStages], q_ready(n + 1)) &&
-                                                         mbar_test_wait(&k_full[st_n], ph_n))) {
-              issue_s(n + 1, st_n, next.tiles == 1);
-              s_issued = true;
-            }
-          }
-          ok = wait_role(p_full, step & 1u, abort_flag, args.status, kMmaTimeout) &&
-               wait_role(&v_full[st], ph, abort_flag, args.status, kMmaTimeout);
+        const Keys keys = keys_of(args, it);
+        const int first = (g + static_cast<int>(n)) & 1;  // the group's first tile
+        if (!wait_role(&q_full[n % kQStages], (n / kQStages) & 1u, abort_flag, args.status, kMmaTimeout)) break;
+        bool ok = true;
+        auto issue_s = [&](uint32_t c) {
+          if (!wait_role(&kf[c % kStages], (c / kStages) & 1u, abort_flag, args.status, kMmaTimeout)) return false;
+          tc_fence_after();
+          mma_scores(t_s, smem_desc(kDescK, s_q + (n % kQStages) * kQTile), smem_desc(kDescK, s_k + (c % kStages) * kKvTile), kIdescS,
+                     &s_full[g]);
+          if (elect_one()) umma_commit(&ke[c % kStages]);
+          return true;
+        };
+        if (first < keys.tiles) ok = issue_s(cnt);
+        for (int j = first; ok && j < keys.tiles; j += 2, ++cnt) {
+          ok = wait_role(&p_full[g], cnt & 1u, abort_flag, args.status, kMmaTimeout) &&
+               wait_role(&vf[cnt % kStages], (cnt / kStages) & 1u, abort_flag, args.status, kMmaTimeout);
           if (!ok) break;
           tc_fence_after();
-          const int valid = max(1, min(kRows, total - j * kRows));
-          mma_values(tmem_base + kTmemO, tmem_base + kTmemP, smem_desc(kDescV, s_v + st * kTile), kIdescO, j > 0 ? 1u : 0u,
+          const int valid = max(1, min(kKeys, keys.total - j * kKeys));
+          mma_values(t_o, t_s, smem_desc(kDescV, s_v + (cnt % kStages) * kKvTile), kIdescO, j > first ? 1u : 0u,
                      static_cast<uint32_t>((valid + 15) >> 4));
-          if (elect_one()) umma_commit(pv_done);
-          if (elect_one()) umma_commit(&v_empty[st]);
-          st = st_n;
-          ph = ph_n;
+          if (elect_one()) umma_commit(&ve[cnt % kStages]);
+          if (j + 2 < keys.tiles)
+            ok = issue_s(cnt + 1);
+          else if (elect_one())
+            umma_commit(&o_done[g]);
         }
         if (!ok) break;
-        if (elect_one()) umma_commit(o_done);
-        if (!next_known) {
-          if (!wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kMmaTimeout)) break;
-          read_item(n);
-          next_have = it.rows > 0;
-          if (next_have) next = keys_of(args, it);
-        }
-        have = next_have;
-        keys = next;
+        if (elect_one()) umma_commit(&q_empty[n % kQStages]);  // this group is done with Q
+        if (!wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kMmaTimeout)) break;
+        read_item(n);
+        have = it.rows > 0;
       }
-    } else if (BIAS && warp == 6) {
+    } else if (BIAS) {
       // ------------------------------------------------------------------- bias
       bool have = own_item(), ok = true;
-      uint32_t step = 0;
+      uint32_t count[2] = {0, 0};
       for (uint32_t n = 0; have && ok; ++n) {
         const Keys keys = keys_of(args, it);
         const float* bias = args.bias + static_cast<long long>(it.head) * args.bias_n;
         const int top = args.bias_n - 1;
-        for (int j = 0; j < keys.tiles; ++j, ++step) {
-          const int stage = static_cast<int>(step % kStages);
-          ok = wait_role(&bias_empty[stage], ((step / kStages) & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
+        for (int j = 0; j < keys.tiles; ++j) {
+          const int g = (j + static_cast<int>(n)) & 1;
+          const uint32_t cnt = g ? count[1]++ : count[0]++;
+          const int slot = g * kStages + static_cast<int>(cnt % kStages);
+          ok = wait_role(&bias_empty[slot], ((cnt / kStages) & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
           if (!ok) break;
-          BiasSlice* slice = reinterpret_cast<BiasSlice*>(smem + L::kBias) + stage;
-          const int u0 = j * kRows;
-          // index of the value at [0]: distance of column 0 and row 127
-          const int at2 = keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left;
-          const int at1 = u0 - it.p0 - 127 + args.bias_left;
-          const bool has_first = u0 < keys.ns;
-          const bool is_flat = !has_first && (at2 >= top || at2 + 254 <= 0);
-          if (lane == 0) flat[stage] = is_flat;
+          BiasSlice* slice = reinterpret_cast<BiasSlice*>(smem + L::kBias) + slot;
+          const int u0 = j * kKeys;
+          // index of the value of column 0 and row 127
+          const int at = keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left;
+          const bool is_flat = u0 >= keys.ns && (at >= top || at + kKeys + 126 <= 0);
+          if (lane == 0) flat[slot] = is_flat;
           if (is_flat) {
-            if (lane == 0) slice->second[0] = __ldg(bias + (at2 >= top ? top : 0)) * 1.4426950408889634f;
+            if (lane == 0) slice->copy[0][0] = __ldg(bias + (at >= top ? top : 0)) * 1.4426950408889634f;
           } else {
+            float v[6];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              slice->second[i * 32 + lane] = __ldg(bias + min(max(at2 + i * 32 + lane, 0), top)) * 1.4426950408889634f;
-            if (has_first) {
+            for (int i = 0; i < 6; ++i) v[i] = __ldg(bias + min(max(at + i * 32 + lane, 0), top)) * 1.4426950408889634f;
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                slice->first[i * 32 + lane] = __ldg(bias + min(max(at1 + i * 32 + lane, 0), top)) * 1.4426950408889634f;
-            }
+            for (int i = 0; i < 6; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (i * 32 + lane >= k) slice->copy[k][i * 32 + lane - k] = v[i];
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bias_full[stage]);
+          if (lane == 0) mbar_arrive(&bias_full[slot]);
         }
         if (!ok || !wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kLoadTimeout)) break;
         read_item(n);
@@ -571,67 +540,84 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
     }
   } else {
-    // ---------------------------------------------------------------- softmax (warps 0..3)
-    regs_inc<216>();
-    const int r = warp * 32 + lane;  // query row inside the tile == tensor-memory lane
-    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
-    const uint32_t t_s = t_lane + kTmemS, t_o = t_lane + kTmemO, t_p = t_lane + kTmemP;
+    // ---------------------------------------------------------------- softmax (warps 0..3 and 4..7)
+    regs_inc<96>();
+    const int g = warp >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // query row inside the tile == tensor-memory lane
+    const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t t_s = t_lane + 64u * g, t_o = t_lane + 128u + 64u * g;
     const float c = args.scale_log2e;
-    int stage = 0;
-    uint32_t phase = 0, step = 0;
+    uint32_t cnt = 0;      // the group's tiles so far
+    uint32_t o_items = 0;  // items in which it had any
+    bool lent = false;     // the other group may still be reading this one's O, reference and sum
+    uint32_t lent_parity = 0;
+    uint8_t* stage_out = smem + L::kOut + warp * (32 * 64);  // output rows, or what the other group needs to know
+    auto take_back = [&]() {
+      if (lent) mbar_wait_anyway(&merge_empty[g * 4 + quarter], lent_parity, abort_flag, args.status, kSoftmaxTimeout);
+      lent = false;
+    };
     bool have = smem_ok && own_item();
     for (uint32_t n = 0; have; ++n) {
       const Keys keys = keys_of(args, it);
+      const int first = (g + static_cast<int>(n)) & 1;
       const bool exists = r < it.rows;
-      const bool idle = warp * 32 >= it.rows;  // no row of this warp exists
+      const bool idle = quarter * 32 >= it.rows;  // no row of this warp exists
       // virtual keys that this row sees: [0, a_hi) and [b_lo, b_hi)
       const int p = it.p0 + r;
       const int hi = args.right < 0 ? it.k_len : min(it.k_len, p + args.right + 1);
       const int a_hi = args.left < 0 ? 0 : min(args.sinks, hi);
       const int b_lo = keys.ns + max((args.left < 0 ? 0 : p - args.left) - keys.ws, 0);
       const int b_hi = keys.ns + hi - keys.ws;
-      // A tile's weights are 2^(score - m_ref) with the reference of the tiles before, so that they need not wait for the tile's
-      // own maximum.  Where that turns out to be more than 2^kLag above a row's reference (fp16 holds the weights up to
-      // there) the warp's rows move theirs to their maxima, rescale O, and the tile's weights are formed again.  Rows that do
-      // not exist have no say, so results are a function of the inputs alone.
+      // The exponent reference of a row may lag its maximum by 2^kLag (fp16 holds the weights up to there); beyond, the warp's
+      // rows move theirs to their maxima and rescale O.  Rows that do not exist have no say, so results are a function of
+      // the inputs alone.
       constexpr float kLag = 12.0f;
       float m_ref = -INFINITY, l_run = 0.f;
-      for (int j = 0; j < keys.tiles; ++j, ++step) {
-        const int u0 = j * kRows;
-        mbar_wait_anyway_lane(s_full, step & 1u, abort_flag, args.status, kSoftmaxTimeout);
+      for (int j = first; j < keys.tiles; j += 2, ++cnt) {
+        const int u0 = j * kKeys;
+        const int slot = g * kStages + static_cast<int>(cnt % kStages);
+        mbar_wait_anyway_lane(&s_full[g], cnt & 1u, abort_flag, args.status, kSoftmaxTimeout);
         tc_fence_after();
-        auto wait_pv = [&]() {  // P and O belong to the previous tile's MMAs until those have retired
-          if (j == 0) return;   // (an item's first tile: the wait for the previous item's O covered it)
-          mbar_wait_anyway_lane(pv_done, (step - 1u) & 1u, abort_flag, args.status, kSoftmaxTimeout);
-          tc_fence_after();
-        };
         const float* slice = nullptr;
         bool is_flat = true;
         float scale = c, shift = 0.f;  // log2 units of what `s` holds below
         if (BIAS) {
-          const int bs = static_cast<int>(step % kStages);
-          mbar_wait_anyway_lane(&bias_full[bs], (step / kStages) & 1u, abort_flag, args.status, kSoftmaxTimeout);
-          slice = reinterpret_cast<const float*>(smem + L::kBias + bs * sizeof(BiasSlice)) + 127 - r;
-          is_flat = flat[bs] != 0;
-          if (is_flat) shift = slice[256 - 127 + r]; else scale = 1.0f;
+          mbar_wait_anyway_lane(&bias_full[slot], (cnt / kStages) & 1u, abort_flag, args.status, kSoftmaxTimeout);
+          const BiasSlice* all = reinterpret_cast<const BiasSlice*>(smem + L::kBias) + slot;
+          slice = &all->copy[(127 - r) & 3][(127 - r) & ~3];
+          is_flat = flat[slot] != 0;
+          if (is_flat) shift = all->copy[0][0]; else scale = 1.0f;
         }
-        if (idle) {
-          if (lane == 0) mbar_arrive(s_free);
-          wait_pv();  // (or this warp's next p_full would count for the tile that the others are still at)
-        } else {
-          const bool whole = __all_sync(0xffffffffu, !exists || (b_lo <= u0 && b_hi >= u0 + kRows));
-          uint32_t s[128];
+        if (!idle) {
+          const bool whole = __all_sync(0xffffffffu, !exists || (b_lo <= u0 && b_hi >= u0 + kKeys));
+          uint32_t s[64];
+          tmem_ld_32x32_at<0>(t_s, s);
+          tmem_ld_32x32_at<32>(t_s + 32, s);
+          tmem_ld_wait();
           float mx0 = -INFINITY, mx1 = -INFINITY;
-          unsigned some = 0xfu;  // chunks of 32 keys that any row of the warp sees
-          // scores of chunk CH: the bias added, masked keys out; the row's maximum
-          auto fix = [&](auto chunk) {
-            constexpr int B = decltype(chunk)::value * 32;
+          unsigned some = 3u;  // halves of the tile of which any row of the warp sees a key
+          // scores of half CH: the bias added, masked keys out; the row's maximum
+          auto fix = [&](auto half) {
+            constexpr int B = decltype(half)::value * 32;
             if (BIAS && !is_flat) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                const float* b = slice + (u0 + B + 16 * h < keys.ns ? 0 : 256);
+                if (u0 + B + 16 * h >= keys.ns) {
 #pragma unroll
-                for (int i = B + 16 * h; i < B + 16 * h + 16; ++i) s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b[i]));
+                  for (int i = B + 16 * h; i < B + 16 * h + 16; i += 4) {
+                    const float4 b = *reinterpret_cast<const float4*>(slice + i);
+                    s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b.x));
+                    s[i + 1] = __float_as_uint(fmaf(__uint_as_float(s[i + 1]), c, b.y));
+                    s[i + 2] = __float_as_uint(fmaf(__uint_as_float(s[i + 2]), c, b.z));
+                    s[i + 3] = __float_as_uint(fmaf(__uint_as_float(s[i + 3]), c, b.w));
+                  }
+                } else {  // the first run: its keys' distances are another stretch of the table, and there are few of them
+                  const float* table = args.bias + static_cast<long long>(it.head) * args.bias_n;
+#pragma unroll
+                  for (int i = B + 16 * h; i < B + 16 * h + 16; ++i)
+                    s[i] = __float_as_uint(fmaf(__ldg(table + min(max(u0 + i - p + args.bias_left, 0), args.bias_n - 1)), 1.4426950408889634f,
+                                                __uint_as_float(s[i]) * c));
+                }
               }
             }
             if (!whole) {
@@ -649,151 +635,146 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               mx1 = max3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
             }
           };
-          float minus = 0.f;
+          fix(Int<0>());
+          fix(Int<1>());
+          const float m_new = fmaxf(m_ref, fmaf(scale, fmaxf(mx0, mx1), shift));
+          if (j == first) {
+            m_ref = m_new;
+          } else if (__any_sync(0xffffffffu, exists && m_new - m_ref > kLag)) {
+            const float f = m_new == m_ref ? 1.0f : ex2(m_ref - m_new);
+#pragma unroll
+            for (int cb = 0; cb < kHeadDim; cb += 16) {
+              uint32_t v[16];
+              tmem_ld_32x16(t_o + cb, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+              tmem_st_32x16(t_o + cb, v);
+            }
+            l_run *= f;
+            m_ref = m_new;
+          }
+          const float minus = shift - (m_ref == -INFINITY ? 0.f : m_ref);  // (a row that has seen nothing yet keeps its masked scores at 2^-inf)
           unsigned long long l0 = 0ull, l1 = 0ull;  // pairs of zeros
-          // weights of chunk CH: fp16 pairs, fp32 sums
-          uint32_t pk[64];
-          auto weigh = [&](auto chunk) {
-            constexpr int B = decltype(chunk)::value * 32;
+          // weights of half CH: fp16 pairs over the scores, fp32 sums
+          auto weigh = [&](auto half) {
+            constexpr int B = decltype(half)::value * 32;
+            uint32_t pk[16];
             if (some & (1u << (B / 32))) {
               const unsigned long long sc2 = pack_f32x2(scale, scale), mi2 = pack_f32x2(minus, minus);
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 float t0, t1;
                 unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[B + 2 * i]), __uint_as_float(s[B + 2 * i + 1])), sc2, mi2), t0, t1);
-                if (i % 8 == 7) {  // one pair in eight goes round the special-function unit
+                if (i % 8 == 7) {  // round the special-function unit
                   ex2_pair_fma(t0, t1);
                 } else {
                   t0 = ex2(t0);
                   t1 = ex2(t1);
                 }
-                const float p0 = t0, p1 = t1;
-                if (i & 1) l1 = add_f32x2(l1, pack_f32x2(p0, p1)); else l0 = add_f32x2(l0, pack_f32x2(p0, p1));
-                pk[B / 2 + i] = pack_half2(p0, p1);
+                if (i & 1) l1 = add_f32x2(l1, pack_f32x2(t0, t1)); else l0 = add_f32x2(l0, pack_f32x2(t0, t1));
+                pk[i] = pack_half2(t0, t1);
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) pk[B / 2 + i] = 0u;
+              for (int i = 0; i < 16; ++i) pk[i] = 0u;
             }
+            tmem_st_32x16(t_s + B / 2, pk);
           };
-          auto store = [&](auto chunk) {
-            constexpr int B = decltype(chunk)::value * 16;
-            uint32_t v[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = pk[B + i];
-            tmem_st_32x16(t_p + B, v);
-          };
-          tmem_ld_32x32_at<0>(t_s, s);
-          tmem_ld_32x32_at<32>(t_s + 32, s);
-          tmem_ld_32x32_at<64>(t_s + 64, s);
-          tmem_ld_32x32_at<96>(t_s + 96, s);
-          tmem_ld_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(s_free);
-          fix(Int<0>());
-          fix(Int<1>());
-          fix(Int<2>());
-          fix(Int<3>());
-          const float m_new = fmaxf(m_ref, fmaf(scale, fmaxf(mx0, mx1), shift));
-          if (j == 0) {
-            m_ref = m_new;
-          } else if (__any_sync(0xffffffffu, exists && m_new - m_ref > kLag)) {
-            wait_pv();
-            const float f = m_new == m_ref ? 1.0f : ex2(m_ref - m_new);
-#pragma unroll
-            for (int cb = 0; cb < kHeadDim; cb += 32) {
-              uint32_t v[32];
-              tmem_ld_32x32(t_o + cb, v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-              tmem_st_32x32(t_o + cb, v);
-            }
-            l_run *= f;
-            m_ref = m_new;
-          }
-          minus = shift - (m_ref == -INFINITY ? 0.f : m_ref);  // (a row that has seen nothing yet keeps its masked scores at 2^-inf)
           weigh(Int<0>());
           weigh(Int<1>());
-          wait_pv();
-          store(Int<0>());
-          store(Int<1>());
-          weigh(Int<2>());
-          store(Int<2>());
-          weigh(Int<3>());
-          store(Int<3>());
           float la, lb;
           unpack_f32x2(add_f32x2(l0, l1), la, lb);
           l_run += la + lb;
         }
         if (BIAS) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bias_empty[step % kStages]);
+          if (lane == 0) mbar_arrive(&bias_empty[slot]);
         }
-        const int valid = min(kRows, keys.total - u0);
-        if (valid < kRows) {
+        const int valid = min(kKeys, keys.total - u0);
+        if (valid < kKeys) {
           // blank the V rows behind the last key (as far as they are multiplied): they may be anybody's
-          mbar_wait_anyway_lane(&v_full[stage], phase, abort_flag, args.status, kSoftmaxTimeout);
+          mbar_wait_anyway_lane(&v_full[slot], (cnt / kStages) & 1u, abort_flag, args.status, kSoftmaxTimeout);
           if (r >= valid && r < max(16, (valid + 15) & ~15)) {
-            uint4* vr = reinterpret_cast<uint4*>(smem + L::kV + stage * kTile + r * 128);
+            uint4* vr = reinterpret_cast<uint4*>(smem + L::kV + slot * kKvTile + r * 128);
 #pragma unroll
             for (int i = 0; i < 8; ++i) vr[i] = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_proxy_async_smem();
         }
+        if (j == first) take_back();  // the product of the item's first tile overwrites O
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (lane == 0) mbar_arrive(&p_full[g]);
       }
-      if (!mbar_wait_warp(o_done, n & 1u, abort_flag, args.status, kSoftmaxTimeout)) break;
-      tc_fence_after();
-      // O / row sum -> fp16 -> this warp's staging rows -> global memory: a slab of 32 rows that all exist by one bulk
-      // store, others by the threads, eight to a row
-      const float inv = 1.0f / l_run;
-      const bool some = l_run != 0.f;  // (a row that sees no key is 0; a NaN stays one)
-      if (lane == 0) tma_store_wait_read();
-      __syncwarp();
-      uint8_t* stage_out = smem + L::kOut + warp * (32 * 128);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t v[32];
-        tmem_ld_32x32(t_o + 32 * h, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          uint4 w;
-          auto pair = [&](int i) {
-            return some ? pack_half2(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv) : 0u;
-          };
-          w.x = pair(u * 8);
-          w.y = pair(u * 8 + 2);
-          w.z = pair(u * 8 + 4);
-          w.w = pair(u * 8 + 6);
-          *reinterpret_cast<uint4*>(stage_out + lane * 128 + (((4 * h + u) ^ (lane & 7)) << 4)) = w;
-        }
+      const bool any = first < keys.tiles;
+      if (any) {
+        if (!mbar_wait_warp(&o_done[g], o_items & 1u, abort_flag, args.status, kSoftmaxTimeout)) break;
+        ++o_items;
+        tc_fence_after();
       }
-      const bool whole_slab = warp * 32 + 32 <= it.rows;
-      if (whole_slab) fence_proxy_async_smem();
-      __syncwarp();
-      if (whole_slab) {
-        if (lane == 0) {
-          tma_store_2d(&tm_out, stage_out, it.head * kHeadDim, it.q_row + warp * 32);
-          tma_store_commit();
-        }
+      if (first == 0) {
+        // the group of the even tiles hands its part over
+        take_back();
+        reinterpret_cast<float2*>(stage_out)[lane] = make_float2(m_ref, l_run);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&merge_full[g * 4 + quarter]);
+        lent = true;
+        lent_parity = (n >> 1) & 1u;
       } else {
-        const int sub = lane >> 3, unit = lane & 7;
-        __half* out = args.out + static_cast<long long>(it.q_row + warp * 32) * args.out_stride + it.head * kHeadDim + unit * 8;
+        // the group of the odd ones puts the two together: O / row sum -> fp16 -> this warp's staging rows, half a row at a time
+        // -> global memory, four threads to a half row
+        const int other = (g ^ 1) * 4 + quarter;
+        take_back();
+        if (!mbar_wait_warp(&merge_full[other], (n >> 1) & 1u, abort_flag, args.status, kSoftmaxTimeout)) break;
+        tc_fence_after();
+        const float2 theirs = reinterpret_cast<const float2*>(smem + L::kOut + other * (32 * 64))[lane];
+        const float top = fmaxf(theirs.x, m_ref);
+        float f0 = theirs.x == -INFINITY ? 0.f : ex2(theirs.x - top);
+        float f1 = m_ref == -INFINITY ? 0.f : ex2(m_ref - top);
+        const float sum = fmaf(theirs.y, f0, l_run * f1);
+        const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // (a row that sees no key: zeros)
+        f0 *= inv;
+        f1 *= inv;
+        __half* out = args.out + static_cast<long long>(it.q_row + quarter * 32) * args.out_stride + it.head * kHeadDim + (lane & 3) * 8;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int row = 4 * k + sub;
-          const uint4 w = *reinterpret_cast<const uint4*>(stage_out + row * 128 + ((unit ^ (row & 7)) << 4));
-          if (warp * 32 + row < it.rows) *reinterpret_cast<uint4*>(out + row * args.out_stride) = w;
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a[32];
+          tmem_ld_32x32(t_lane + 128u + 64u * (g ^ 1) + 32 * h, a);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) a[i] = f0 != 0.f ? __float_as_uint(__uint_as_float(a[i]) * f0) : 0u;
+          if (any) {
+            uint32_t b[32];
+            tmem_ld_32x32(t_o + 32 * h, b);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) a[i] = f1 != 0.f ? __float_as_uint(fmaf(__uint_as_float(b[i]), f1, __uint_as_float(a[i]))) : a[i];
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint4 w;
+            w.x = pack_half2(__uint_as_float(a[u * 8]), __uint_as_float(a[u * 8 + 1]));
+            w.y = pack_half2(__uint_as_float(a[u * 8 + 2]), __uint_as_float(a[u * 8 + 3]));
+            w.z = pack_half2(__uint_as_float(a[u * 8 + 4]), __uint_as_float(a[u * 8 + 5]));
+            w.w = pack_half2(__uint_as_float(a[u * 8 + 6]), __uint_as_float(a[u * 8 + 7]));
+            *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = w;
+          }
+          if (h == 1) {  // all of the other group's part has been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&merge_empty[other]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = 8 * k + (lane >> 2);
+            const uint4 w = *reinterpret_cast<const uint4*>(stage_out + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+            if (quarter * 32 + row < it.rows) *reinterpret_cast<uint4*>(out + row * args.out_stride + 32 * h) = w;
+          }
+          __syncwarp();
         }
       }
       tc_fence_before();
@@ -802,7 +783,6 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       read_item(n);
       have = it.rows > 0;
     }
-    if (lane == 0) tma_store_wait_all();  // the staging rows must outlive the last bulk store
     tc_fence_before();
   }
 
@@ -810,14 +790,14 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   if (*abort_flag != 0) {  // copies in flight land before the block's memory goes to another
     for (int i = 0; i < 64; ++i) __nanosleep(2000);
   }
-  if (warp == 5) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 256);
   }
 }
 
 template <bool BIAS>
-cudaError_t launch_window(const CUtensorMap (&tm)[6], WindowArgs a, int sms, cudaStream_t stream) {
+cudaError_t launch_window(const CUtensorMap (&tm)[5], WindowArgs a, int sms, cudaStream_t stream) {
   auto kern = window_mha_kernel<BIAS>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<BIAS>::kBytes);
   if (e != cudaSuccess) return e;
@@ -830,7 +810,7 @@ cudaError_t launch_window(const CUtensorMap (&tm)[6], WindowArgs a, int sms, cud
   if (grid > 0x7fffffffLL - 0x10000) return cudaErrorInvalidValue;
   a.take_over = grid > 2LL * sms ? 1 : 0;
   return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Layout<BIAS>::kBytes, stream, tm[0], tm[1], tm[2], tm[3],
-                    tm[4], tm[5], a);
+                    tm[4], a);
 }
 
 // -------------------------------------------------------------------------------------------- few queries
@@ -1252,11 +1232,10 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
   const void *k = none ? a->q : a->k, *v = none ? a->q : a->v;
   const uint64_t k_rows = none ? a->q_rows : a->k_rows;
   const long long k_ld = none ? a->q_row_stride : a->k_row_stride, v_ld = none ? a->q_row_stride : a->v_row_stride;
-  CUtensorMap tm[6];
+  CUtensorMap tm[5];
   const bool ok = make_tmap_2d(&tm[0], a->q, a->q_rows, q_cols, a->q_row_stride, 64, 128) &&
-                  make_tmap_2d(&tm[1], k, k_rows, kv_cols, k_ld, 64, 128) && make_tmap_2d(&tm[2], v, k_rows, kv_cols, v_ld, 64, 128) &&
-                  make_tmap_2d(&tm[3], k, k_rows, kv_cols, k_ld, 64, kSeam) && make_tmap_2d(&tm[4], v, k_rows, kv_cols, v_ld, 64, kSeam) &&
-                  make_tmap_2d(&tm[5], a->out, a->q_rows, q_cols, a->out_row_stride, 64, 32);
+                  make_tmap_2d(&tm[1], k, k_rows, kv_cols, k_ld, 64, kKeys) && make_tmap_2d(&tm[2], v, k_rows, kv_cols, v_ld, 64, kKeys) &&
+                  make_tmap_2d(&tm[3], k, k_rows, kv_cols, k_ld, 64, kSeam) && make_tmap_2d(&tm[4], v, k_rows, kv_cols, v_ld, 64, kSeam);
   if (!ok) return BT_ERR_CUDA;
   e = w.bias != nullptr ? launch_window<true>(tm, w, dev.sms, stream) : launch_window<false>(tm, w, dev.sms, stream);
   if (e == cudaErrorInvalidValue) return BT_ERR_INVALID_ARG;
