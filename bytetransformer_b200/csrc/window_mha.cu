@@ -249,12 +249,12 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return below_hi & ~below_lo;
 }
 
-// The bias of a tile's second run of keys, for all its rows: value of (column c, row r) at c - r + 127, in log2 units.  Four
-// copies, each an element further on, so that a thread reads its row's values four at a time wherever they start; the pitch
-// keeps the copies that neighbouring rows read in different banks.
+// The bias of a tile for all its rows: value of (column c, row r) at c - r + 127, in log2 units; columns of the second run of
+// keys [0], of the first [1].  Four copies, each an element further on, so that a thread reads its row's values four at a
+// time wherever they start; the pitch keeps the copies that neighbouring rows read in different banks.
 constexpr int kBiasPitch = 200;
 struct BiasSlice {
-  float copy[4][kBiasPitch];
+  float copy[2][4][kBiasPitch];
 };
 
 template <bool BIAS>
@@ -266,7 +266,7 @@ struct Layout {
   static constexpr int kV = kK + 2 * kStages * kKvTile;
   static constexpr int kOut = kV + 2 * kStages * kKvTile;  // 32 rows x 64 bytes for each of the eight warps
   static constexpr int kBias = kOut + 8 * 32 * 64;
-  static constexpr int kBar = kBias + (BIAS ? 2 * kStages * static_cast<int>(sizeof(BiasSlice)) : 0);
+  static constexpr int kBar = kBias + (BIAS ? 2 * static_cast<int>(sizeof(BiasSlice)) : 0);
   static constexpr int kBytes = kBar + 1024;
 };
 
@@ -296,14 +296,14 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* item_full = bars + 42;            // [kSlots]
   uint64_t* item_empty = bars + 46;           // [kSlots]
   uint64_t* taken_full = bars + 50;
-  uint64_t* bias_full = bars + 51;            // [group][kStages] by the group's tiles
-  uint64_t* bias_empty = bars + 55;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 59);
+  uint64_t* bias_full = bars + 51;            // [group] by the group's tiles
+  uint64_t* bias_empty = bars + 53;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 55);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* taken = smem + L::kBar + 480;       // 16 bytes
   Item* items = reinterpret_cast<Item*>(smem + L::kBar + 496);
-  volatile int* flat = reinterpret_cast<volatile int*>(smem + L::kBar + 496 + kSlots * sizeof(Item));  // [group][kStages]
-  static_assert(496 + kSlots * sizeof(Item) + 2 * kStages * 4 <= 1024, "barriers and items");
+  volatile int* flat = reinterpret_cast<volatile int*>(smem + L::kBar + 496 + kSlots * sizeof(Item));  // [group]
+  static_assert(496 + kSlots * sizeof(Item) + 2 * 4 <= 1024, "barriers and items");
 
   const int warp = uniform_int(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
@@ -315,14 +315,14 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
       mbar_init(&o_done[s], 1);
+      mbar_init(&bias_full[s], 1);
+      mbar_init(&bias_empty[s], 4);
     }
     for (int s = 0; s < 2 * kStages; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
-      mbar_init(&bias_full[s], 1);
-      mbar_init(&bias_empty[s], 4);
     }
     for (int s = 0; s < 8; ++s) {
       mbar_init(&merge_full[s], 1);
@@ -480,7 +480,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         };
         if (first < keys.tiles) ok = issue_s(cnt);
         for (int j = first; ok && j < keys.tiles; j += 2, ++cnt) {
-          ok = wait_role(&p_full[g], cnt & 1u, abort_flag, args.status, kMmaTimeout) &&
+          ok = mbar_wait_warp(&p_full[g], cnt & 1u, abort_flag, args.status, kMmaTimeout) &&
                wait_role(&vf[cnt % kStages], (cnt / kStages) & 1u, abort_flag, args.status, kMmaTimeout);
           if (!ok) break;
           tc_fence_after();
@@ -510,29 +510,31 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int j = 0; j < keys.tiles; ++j) {
           const int g = (j + static_cast<int>(n)) & 1;
           const uint32_t cnt = g ? count[1]++ : count[0]++;
-          const int slot = g * kStages + static_cast<int>(cnt % kStages);
-          ok = wait_role(&bias_empty[slot], ((cnt / kStages) & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
+          ok = wait_role(&bias_empty[g], (cnt & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
           if (!ok) break;
-          BiasSlice* slice = reinterpret_cast<BiasSlice*>(smem + L::kBias) + slot;
+          BiasSlice* slice = reinterpret_cast<BiasSlice*>(smem + L::kBias) + g;
           const int u0 = j * kKeys;
           // index of the value of column 0 and row 127
-          const int at = keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left;
-          const bool is_flat = u0 >= keys.ns && (at >= top || at + kKeys + 126 <= 0);
-          if (lane == 0) flat[slot] = is_flat;
+          const int at[2] = {keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left, u0 - it.p0 - 127 + args.bias_left};
+          const bool is_flat = u0 >= keys.ns && (at[0] >= top || at[0] + kKeys + 126 <= 0);
+          if (lane == 0) flat[g] = is_flat;
           if (is_flat) {
-            if (lane == 0) slice->copy[0][0] = __ldg(bias + (at >= top ? top : 0)) * 1.4426950408889634f;
+            if (lane == 0) slice->copy[0][0][0] = __ldg(bias + (at[0] >= top ? top : 0)) * 1.4426950408889634f;
           } else {
-            float v[6];
+#pragma unroll 1
+            for (int run = 0; run < (u0 < keys.ns ? 2 : 1); ++run) {
+              float v[6];
 #pragma unroll
-            for (int i = 0; i < 6; ++i) v[i] = __ldg(bias + min(max(at + i * 32 + lane, 0), top)) * 1.4426950408889634f;
+              for (int i = 0; i < 6; ++i) v[i] = __ldg(bias + min(max(at[run] + i * 32 + lane, 0), top)) * 1.4426950408889634f;
 #pragma unroll
-            for (int i = 0; i < 6; ++i)
+              for (int i = 0; i < 6; ++i)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (i * 32 + lane >= k) slice->copy[k][i * 32 + lane - k] = v[i];
+                for (int k = 0; k < 4; ++k)
+                  if (i * 32 + lane >= k) slice->copy[run][k][i * 32 + lane - k] = v[i];
+            }
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bias_full[slot]);
+          if (lane == 0) mbar_arrive(&bias_full[g]);
         }
         if (!ok || !wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kLoadTimeout)) break;
         read_item(n);
@@ -548,13 +550,80 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t t_s = t_lane + 64u * g, t_o = t_lane + 128u + 64u * g;
     const float c = args.scale_log2e;
     uint32_t cnt = 0;      // the group's tiles so far
-    uint32_t o_items = 0;  // items in which it had any
-    bool lent = false;     // the other group may still be reading this one's O, reference and sum
-    uint32_t lent_parity = 0;
     uint8_t* stage_out = smem + L::kOut + warp * (32 * 64);  // output rows, or what the other group needs to know
+    uint32_t o_items[2] = {0, 0};            // items in which this group, the other one had tiles
+    uint32_t handed = 0, received = 0;
+    bool lent = false;                       // the other group may still be reading this one's O, reference and sum
+    bool ok = true;
     auto take_back = [&]() {
-      if (lent) mbar_wait_anyway(&merge_empty[g * 4 + quarter], lent_parity, abort_flag, args.status, kSoftmaxTimeout);
+      if (lent && !mbar_wait_warp(&merge_empty[g * 4 + quarter], (handed - 1u) & 1u, abort_flag, args.status, kSoftmaxTimeout)) ok = false;
       lent = false;
+    };
+    // The end of an item.  The group of the odd tiles says what its reference and sum are and goes on (its next product waits
+    // until its O has been read, see take_back).
+    auto hand_over = [&](float m, float l) {
+      reinterpret_cast<float2*>(stage_out)[lane] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&merge_full[g * 4 + quarter]);
+      lent = true;
+      ++handed;
+    };
+    auto merge = [&](float m, float l, bool both) {
+      // the group of the even ones puts the two together: O / row sum -> fp16 -> this warp's staging rows, half a row at a time
+      // -> global memory, four threads to a half row
+      const int other = (g ^ 1) * 4 + quarter;
+      float2 theirs = make_float2(-INFINITY, 0.f);
+      ok = mbar_wait_warp(&o_done[g], o_items[0] & 1u, abort_flag, args.status, kSoftmaxTimeout) && ok;
+      if (both) {
+        ok = mbar_wait_warp(&merge_full[other], received++ & 1u, abort_flag, args.status, kSoftmaxTimeout) && ok;
+        ok = mbar_wait_warp(&o_done[g ^ 1], o_items[1] & 1u, abort_flag, args.status, kSoftmaxTimeout) && ok;
+      }
+      tc_fence_after();
+      if (both) {
+        theirs = reinterpret_cast<const float2*>(smem + L::kOut + other * (32 * 64))[lane];
+      }
+      const float top = fmaxf(theirs.x, m);
+      float f0 = m == -INFINITY ? 0.f : ex2(m - top);
+      float f1 = theirs.x == -INFINITY ? 0.f : ex2(theirs.x - top);
+      const float sum = fmaf(theirs.y, f1, l * f0);
+      const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // (a row that sees no key: zeros)
+      f0 *= inv;
+      f1 *= inv;
+      __half* out = args.out + static_cast<long long>(it.q_row + quarter * 32) * args.out_stride + it.head * kHeadDim + (lane & 3) * 8;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t a[32];
+        tmem_ld_32x32(t_o + 32 * h, a);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) a[i] = f0 != 0.f ? __float_as_uint(__uint_as_float(a[i]) * f0) : 0u;
+        if (both) {
+          uint32_t b[32];
+          tmem_ld_32x32(t_lane + 128u + 64u * (g ^ 1) + 32 * h, b);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) a[i] = f1 != 0.f ? __float_as_uint(fmaf(__uint_as_float(b[i]), f1, __uint_as_float(a[i]))) : a[i];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          uint4 w;
+          w.x = pack_half2(__uint_as_float(a[u * 8]), __uint_as_float(a[u * 8 + 1]));
+          w.y = pack_half2(__uint_as_float(a[u * 8 + 2]), __uint_as_float(a[u * 8 + 3]));
+          w.z = pack_half2(__uint_as_float(a[u * 8 + 4]), __uint_as_float(a[u * 8 + 5]));
+          w.w = pack_half2(__uint_as_float(a[u * 8 + 6]), __uint_as_float(a[u * 8 + 7]));
+          *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = w;
+        }
+        if (h == 1) tc_fence_before();
+        __syncwarp();
+        if (h == 1 && both && lane == 0) mbar_arrive(&merge_empty[other]);  // all of the other group's part has been read
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = 8 * k + (lane >> 2);
+          const uint4 w = *reinterpret_cast<const uint4*>(stage_out + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+          if (quarter * 32 + row < it.rows) *reinterpret_cast<uint4*>(out + row * args.out_stride + 32 * h) = w;
+        }
+        __syncwarp();
+      }
     };
     bool have = smem_ok && own_item();
     for (uint32_t n = 0; have; ++n) {
@@ -582,11 +651,11 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         bool is_flat = true;
         float scale = c, shift = 0.f;  // log2 units of what `s` holds below
         if (BIAS) {
-          mbar_wait_anyway_lane(&bias_full[slot], (cnt / kStages) & 1u, abort_flag, args.status, kSoftmaxTimeout);
-          const BiasSlice* all = reinterpret_cast<const BiasSlice*>(smem + L::kBias) + slot;
-          slice = &all->copy[(127 - r) & 3][(127 - r) & ~3];
-          is_flat = flat[slot] != 0;
-          if (is_flat) shift = all->copy[0][0]; else scale = 1.0f;
+          mbar_wait_anyway_lane(&bias_full[g], cnt & 1u, abort_flag, args.status, kSoftmaxTimeout);
+          const BiasSlice* all = reinterpret_cast<const BiasSlice*>(smem + L::kBias) + g;
+          slice = &all->copy[0][(127 - r) & 3][(127 - r) & ~3];
+          is_flat = flat[g] != 0;
+          if (is_flat) shift = all->copy[0][0][0]; else scale = 1.0f;
         }
         if (!idle) {
           const bool whole = __all_sync(0xffffffffu, !exists || (b_lo <= u0 && b_hi >= u0 + kKeys));
@@ -602,21 +671,14 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (BIAS && !is_flat) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                if (u0 + B + 16 * h >= keys.ns) {
+                const float* from = slice + (u0 + B + 16 * h < keys.ns ? 4 * kBiasPitch : 0);
 #pragma unroll
-                  for (int i = B + 16 * h; i < B + 16 * h + 16; i += 4) {
-                    const float4 b = *reinterpret_cast<const float4*>(slice + i);
-                    s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b.x));
-                    s[i + 1] = __float_as_uint(fmaf(__uint_as_float(s[i + 1]), c, b.y));
-                    s[i + 2] = __float_as_uint(fmaf(__uint_as_float(s[i + 2]), c, b.z));
-                    s[i + 3] = __float_as_uint(fmaf(__uint_as_float(s[i + 3]), c, b.w));
-                  }
-                } else {  // the first run: its keys' distances are another stretch of the table, and there are few of them
-                  const float* table = args.bias + static_cast<long long>(it.head) * args.bias_n;
-#pragma unroll
-                  for (int i = B + 16 * h; i < B + 16 * h + 16; ++i)
-                    s[i] = __float_as_uint(fmaf(__ldg(table + min(max(u0 + i - p + args.bias_left, 0), args.bias_n - 1)), 1.4426950408889634f,
-                                                __uint_as_float(s[i]) * c));
+                for (int i = B + 16 * h; i < B + 16 * h + 16; i += 4) {
+                  const float4 b = *reinterpret_cast<const float4*>(from + i);
+                  s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b.x));
+                  s[i + 1] = __float_as_uint(fmaf(__uint_as_float(s[i + 1]), c, b.y));
+                  s[i + 2] = __float_as_uint(fmaf(__uint_as_float(s[i + 2]), c, b.z));
+                  s[i + 3] = __float_as_uint(fmaf(__uint_as_float(s[i + 3]), c, b.w));
                 }
               }
             }
@@ -642,7 +704,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             m_ref = m_new;
           } else if (__any_sync(0xffffffffu, exists && m_new - m_ref > kLag)) {
             const float f = m_new == m_ref ? 1.0f : ex2(m_ref - m_new);
-#pragma unroll
+#pragma unroll 1
             for (int cb = 0; cb < kHeadDim; cb += 16) {
               uint32_t v[16];
               tmem_ld_32x16(t_o + cb, v);
@@ -689,7 +751,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         if (BIAS) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bias_empty[slot]);
+          if (lane == 0) mbar_arrive(&bias_empty[g]);
         }
         const int valid = min(kKeys, keys.total - u0);
         if (valid < kKeys) {
@@ -702,81 +764,20 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           fence_proxy_async_smem();
         }
-        if (j == first) take_back();  // the product of the item's first tile overwrites O
         tmem_st_wait();
+        if (j == first) take_back();  // the product of an item's first tile overwrites O
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[g]);
       }
-      const bool any = first < keys.tiles;
-      if (any) {
-        if (!mbar_wait_warp(&o_done[g], o_items & 1u, abort_flag, args.status, kSoftmaxTimeout)) break;
-        ++o_items;
-        tc_fence_after();
-      }
-      if (first == 0) {
-        // the group of the even tiles hands its part over
-        take_back();
-        reinterpret_cast<float2*>(stage_out)[lane] = make_float2(m_ref, l_run);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&merge_full[g * 4 + quarter]);
-        lent = true;
-        lent_parity = (n >> 1) & 1u;
-      } else {
-        // the group of the odd ones puts the two together: O / row sum -> fp16 -> this warp's staging rows, half a row at a time
-        // -> global memory, four threads to a half row
-        const int other = (g ^ 1) * 4 + quarter;
-        take_back();
-        if (!mbar_wait_warp(&merge_full[other], (n >> 1) & 1u, abort_flag, args.status, kSoftmaxTimeout)) break;
-        tc_fence_after();
-        const float2 theirs = reinterpret_cast<const float2*>(smem + L::kOut + other * (32 * 64))[lane];
-        const float top = fmaxf(theirs.x, m_ref);
-        float f0 = theirs.x == -INFINITY ? 0.f : ex2(theirs.x - top);
-        float f1 = m_ref == -INFINITY ? 0.f : ex2(m_ref - top);
-        const float sum = fmaf(theirs.y, f0, l_run * f1);
-        const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // (a row that sees no key: zeros)
-        f0 *= inv;
-        f1 *= inv;
-        __half* out = args.out + static_cast<long long>(it.q_row + quarter * 32) * args.out_stride + it.head * kHeadDim + (lane & 3) * 8;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a[32];
-          tmem_ld_32x32(t_lane + 128u + 64u * (g ^ 1) + 32 * h, a);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) a[i] = f0 != 0.f ? __float_as_uint(__uint_as_float(a[i]) * f0) : 0u;
-          if (any) {
-            uint32_t b[32];
-            tmem_ld_32x32(t_o + 32 * h, b);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) a[i] = f1 != 0.f ? __float_as_uint(fmaf(__uint_as_float(b[i]), f1, __uint_as_float(a[i]))) : a[i];
-          }
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint4 w;
-            w.x = pack_half2(__uint_as_float(a[u * 8]), __uint_as_float(a[u * 8 + 1]));
-            w.y = pack_half2(__uint_as_float(a[u * 8 + 2]), __uint_as_float(a[u * 8 + 3]));
-            w.z = pack_half2(__uint_as_float(a[u * 8 + 4]), __uint_as_float(a[u * 8 + 5]));
-            w.w = pack_half2(__uint_as_float(a[u * 8 + 6]), __uint_as_float(a[u * 8 + 7]));
-            *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = w;
-          }
-          if (h == 1) {  // all of the other group's part has been read
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&merge_empty[other]);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = 8 * k + (lane >> 2);
-            const uint4 w = *reinterpret_cast<const uint4*>(stage_out + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
-            if (quarter * 32 + row < it.rows) *reinterpret_cast<uint4*>(out + row * args.out_stride + 32 * h) = w;
-          }
-          __syncwarp();
-        }
-      }
+      const bool both = keys.tiles > 1;
+      if (first == 0)
+        merge(m_ref, l_run, both);
+      else if (both)
+        hand_over(m_ref, l_run);
+      o_items[0] += first < keys.tiles ? 1u : 0u;
+      o_items[1] += 1 - first < keys.tiles ? 1u : 0u;
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (!mbar_wait_warp(&item_full[n % kSlots], parity(n), abort_flag, args.status, kSoftmaxTimeout)) break;
