@@ -470,15 +470,20 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int first = (g + static_cast<int>(n)) & 1;  // the group's first tile
         if (!wait_role(&q_full[n % kQStages], (n / kQStages) & 1u, abort_flag, args.status, kMmaTimeout)) break;
         bool ok = true;
-        auto issue_s = [&](uint32_t c) {
+        // (an item's last product with Q lets go of it)
+        auto issue_s = [&](uint32_t c, bool last) {
           if (!wait_role(&kf[c % kStages], (c / kStages) & 1u, abort_flag, args.status, kMmaTimeout)) return false;
           tc_fence_after();
           mma_scores(t_s, smem_desc(kDescK, s_q + (n % kQStages) * kQTile), smem_desc(kDescK, s_k + (c % kStages) * kKvTile), kIdescS,
                      &s_full[g]);
           if (elect_one()) umma_commit(&ke[c % kStages]);
+          if (last && elect_one()) umma_commit(&q_empty[n % kQStages]);
           return true;
         };
-        if (first < keys.tiles) ok = issue_s(cnt);
+        if (first < keys.tiles)
+          ok = issue_s(cnt, first + 2 >= keys.tiles);
+        else if (elect_one())
+          umma_commit(&q_empty[n % kQStages]);
         for (int j = first; ok && j < keys.tiles; j += 2, ++cnt) {
           ok = mbar_wait_warp(&p_full[g], cnt & 1u, abort_flag, args.status, kMmaTimeout) &&
                wait_role(&vf[cnt % kStages], (cnt / kStages) & 1u, abort_flag, args.status, kMmaTimeout);
@@ -489,12 +494,11 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                      static_cast<uint32_t>((valid + 15) >> 4));
           if (elect_one()) umma_commit(&ve[cnt % kStages]);
           if (j + 2 < keys.tiles)
-            ok = issue_s(cnt + 1);
+            ok = issue_s(cnt + 1, j + 4 >= keys.tiles);
           else if (elect_one())
             umma_commit(&o_done[g]);
         }
         if (!ok) break;
-        if (elect_one()) umma_commit(&q_empty[n % kQStages]);  // this group is done with Q
         if (!wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kMmaTimeout)) break;
         read_item(n);
         have = it.rows > 0;
@@ -592,17 +596,18 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       __half* out = args.out + static_cast<long long>(it.q_row + quarter * 32) * args.out_stride + it.head * kHeadDim + (lane & 3) * 8;
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
+        // (O is finite where a row has seen nothing: its weights were zeros)
         uint32_t a[32];
         tmem_ld_32x32(t_o + 32 * h, a);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) a[i] = f0 != 0.f ? __float_as_uint(__uint_as_float(a[i]) * f0) : 0u;
+        for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * f0);
         if (both) {
           uint32_t b[32];
           tmem_ld_32x32(t_lane + 128u + 64u * (g ^ 1) + 32 * h, b);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) a[i] = f1 != 0.f ? __float_as_uint(fmaf(__uint_as_float(b[i]), f1, __uint_as_float(a[i]))) : a[i];
+          for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), f1, __uint_as_float(a[i])));
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -699,6 +704,10 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           };
           fix(Int<0>());
           fix(Int<1>());
+          if (BIAS) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bias_empty[g]);
+          }
           const float m_new = fmaxf(m_ref, fmaf(scale, fmaxf(mx0, mx1), shift));
           if (j == first) {
             m_ref = m_new;
@@ -749,10 +758,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           unpack_f32x2(add_f32x2(l0, l1), la, lb);
           l_run += la + lb;
         }
-        if (BIAS) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bias_empty[g]);
-        }
+        if (BIAS && idle && lane == 0) mbar_arrive(&bias_empty[g]);
         const int valid = min(kKeys, keys.total - u0);
         if (valid < kKeys) {
           // blank the V rows behind the last key (as far as they are multiplied): they may be anybody's
