@@ -82,7 +82,8 @@ __device__ __forceinline__ Keys keys_of(const WindowArgs& a, const Item& it) {
   return k;
 }
 
-// Item n = (sequence, query tile, head), heads fastest; called by whole warps, 32 sequences at a time.  A sequence whose
+// Item n = (sequence, query tile, head), heads fastest, a sequence's last tiles (which see most keys where nothing behind them is
+// seen) first; called by whole warps, 32 sequences at a time.  A sequence whose
 // offsets do not describe rows of the buffers is left out and reported.
 __device__ __forceinline__ bool find_item(const WindowArgs& a, int n, int& cur_b, int& cur_first, Item& it) {
   const int lane = static_cast<int>(threadIdx.x & 31u);
@@ -119,9 +120,9 @@ __device__ __forceinline__ bool find_item(const WindowArgs& a, int n, int& cur_b
       cur_first += __shfl_sync(0xffffffffu, incl - items, src);
       cur_b += src;
       const int r = n - cur_first;
-      const int qt = r / a.heads;
-      if (qt < 0 || qt > (len - 1) / kRows) break;  // (offsets so wrong that the count of items passed 32 bits)
-      it.head = uniform_int(r - qt * a.heads);
+      const int from_end = r / a.heads, qt = (len - 1) / kRows - from_end;
+      if (from_end < 0 || qt < 0) break;  // (offsets so wrong that the count of items passed 32 bits)
+      it.head = uniform_int(r - from_end * a.heads);
       it.q_row = uniform_int(start + qt * kRows);
       it.rows = uniform_int(min(kRows, len - qt * kRows));
       it.p0 = uniform_int(qt * kRows + it.k_len - len);
@@ -157,23 +158,6 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-// 2^x of a pair on the FMA pipe: whole part by the rounding of x + 1.5 * 2^23, the rest, f in [-1/2, 1/2], by the polynomial of
-// degree 4 with the least relative error there (2.6e-6; Remez exchange).  Below 2^-126 it stays at that.
-__device__ __forceinline__ void ex2_pair_fma(float& x0, float& x1) {
-  const unsigned long long magic = pack_f32x2(12582912.f, 12582912.f), less = pack_f32x2(-12582912.f, -12582912.f);
-  const unsigned long long x = pack_f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const unsigned long long r = add_f32x2(x, magic);
-  const unsigned long long f = fma_f32x2(add_f32x2(r, less), pack_f32x2(-1.f, -1.f), x);
-  unsigned long long p = fma_f32x2(f, pack_f32x2(0.00957010221f, 0.00957010221f), pack_f32x2(0.0559178591f, 0.0559178591f));
-  p = fma_f32x2(p, f, pack_f32x2(0.240247443f, 0.240247443f));
-  p = fma_f32x2(p, f, pack_f32x2(0.693121791f, 0.693121791f));
-  p = fma_f32x2(p, f, pack_f32x2(0.999999285f, 0.999999285f));
-  float r0, r1, p0, p1;
-  unpack_f32x2(r, r0, r1);
-  unpack_f32x2(p, p0, p1);
-  x0 = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
-  x1 = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -372,7 +356,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // Tile j of item n belongs to group (j + n) & 1, so the group that had one tile more has one less next time.
 
   if (warp >= 8) {
-    regs_dec<48>();
+    regs_dec<32>();
     if (!smem_ok) {
       // straight to the teardown
     } else if (warp == 8) {
@@ -547,7 +531,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
   } else {
     // ---------------------------------------------------------------- softmax (warps 0..3 and 4..7)
-    regs_inc<96>();
+    regs_inc<104>();
     const int g = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;  // query row inside the tile == tensor-memory lane
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -737,12 +721,8 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               for (int i = 0; i < 16; ++i) {
                 float t0, t1;
                 unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[B + 2 * i]), __uint_as_float(s[B + 2 * i + 1])), sc2, mi2), t0, t1);
-                if (i % 8 == 7) {  // round the special-function unit
-                  ex2_pair_fma(t0, t1);
-                } else {
-                  t0 = ex2(t0);
-                  t1 = ex2(t1);
-                }
+                t0 = ex2(t0);
+                t1 = ex2(t1);
                 if (i & 1) l1 = add_f32x2(l1, pack_f32x2(t0, t1)); else l0 = add_f32x2(l0, pack_f32x2(t0, t1));
                 pk[i] = pack_half2(t0, t1);
               }
