@@ -786,8 +786,6 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 template <bool BIAS>
 cudaError_t launch_window(const CUtensorMap (&tm)[5], WindowArgs a, int sms, cudaStream_t stream) {
   auto kern = window_mha_kernel<BIAS>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<BIAS>::kBytes);
-  if (e != cudaSuccess) return e;
   // A block per item, by an upper bound: tiles of sequences of max_q queries, or of sequences that share q_rows rows
   long long tiles = static_cast<long long>(a.batch) * ((a.max_q + kRows - 1) / kRows);
   const long long by_rows = (a.q_rows + static_cast<long long>(a.batch) * (kRows - 1)) / kRows;
@@ -1119,7 +1117,8 @@ struct DeviceFacts {
   int sms = 0, major = 0;
   int* status = nullptr;
 };
-// What a call needs to know of the current device; looked up once (outside a capture, see bt_b200.h).
+// What a call needs to know of the current device, and what the device needs to know of the kernels; once (outside a
+// capture, see bt_b200.h).
 cudaError_t device_facts(DeviceFacts* f) {
   static std::mutex mu;
   static DeviceFacts known[64];
@@ -1135,6 +1134,10 @@ cudaError_t device_facts(DeviceFacts* f) {
     if (e != cudaSuccess) return e;
     n.status = device_status_word();
     if (n.status == nullptr) return cudaErrorUnknown;
+    e = cudaFuncSetAttribute(window_mha_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<false>::kBytes);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(window_mha_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<true>::kBytes);
+    if (e != cudaSuccess) return e;
     known[dev] = n;
   }
   *f = known[dev];
@@ -1221,9 +1224,14 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
   const long long k_ld = none ? a->q_row_stride : a->k_row_stride, v_ld = none ? a->q_row_stride : a->v_row_stride;
   CUtensorMap tm[5];
   const bool ok = make_tmap_2d(&tm[0], a->q, a->q_rows, q_cols, a->q_row_stride, 64, 128) &&
-                  make_tmap_2d(&tm[1], k, k_rows, kv_cols, k_ld, 64, kKeys) && make_tmap_2d(&tm[2], v, k_rows, kv_cols, v_ld, 64, kKeys) &&
-                  make_tmap_2d(&tm[3], k, k_rows, kv_cols, k_ld, 64, kSeam) && make_tmap_2d(&tm[4], v, k_rows, kv_cols, v_ld, 64, kSeam);
+                  make_tmap_2d(&tm[1], k, k_rows, kv_cols, k_ld, 64, kKeys) && make_tmap_2d(&tm[2], v, k_rows, kv_cols, v_ld, 64, kKeys);
   if (!ok) return BT_ERR_CUDA;
+  if (w.sinks > 0 && w.left >= 0) {  // a tile may hold the seam
+    if (!make_tmap_2d(&tm[3], k, k_rows, kv_cols, k_ld, 64, kSeam) || !make_tmap_2d(&tm[4], v, k_rows, kv_cols, v_ld, 64, kSeam)) return BT_ERR_CUDA;
+  } else {
+    tm[3] = tm[1];
+    tm[4] = tm[2];
+  }
   e = w.bias != nullptr ? launch_window<true>(tm, w, dev.sms, stream) : launch_window<false>(tm, w, dev.sms, stream);
   if (e == cudaErrorInvalidValue) return BT_ERR_INVALID_ARG;
   return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;

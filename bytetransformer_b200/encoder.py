@@ -24,6 +24,11 @@ WEIGHT_NAMES = (
 _LOOSE = {4, 5, 10, 11}  # LayerNorm gamma/beta: dtype not checked by the reference (CHECK_INPUT_LOOSE)
 
 
+_current_device = torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream_ptr(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -38,10 +43,10 @@ class _On:
 
     def __enter__(self):
         self.guard = None
-        if torch.cuda.current_device() != self.index:
+        if _current_device() != self.index:
             self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.guard is not None:
@@ -563,6 +568,7 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
 
 
 def _rmsnorm_args(x, residual, gamma, m_dev):
+    """(x is fp32, gamma is fp32) of a norm's arguments, which are refused here if they do not fit together."""
     x_fp32 = _half_or_float(x, "x")
     gamma_fp32 = _half_or_float(gamma, "gamma", x.device)
     if x.dim() != 2 or gamma.dim() != 1 or gamma.shape[0] != x.shape[1]:
@@ -624,17 +630,18 @@ def add_residual_rmsnorm_e4m3(x: torch.Tensor, residual: Optional[torch.Tensor],
     return out, scales, total
 
 
-def _rows(t: torch.Tensor, name: str, device, heads_of: int = 64) -> int:
+def _rows(t: torch.Tensor, name: str, device) -> int:
     """Heads of a matrix [rows, heads * 64] whose rows may be further apart than they are long."""
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if t.dtype != torch.float16:
         raise RuntimeError(f"Inconsistency of Tensor type: {name}")
-    if t.dim() != 2 or t.shape[1] == 0 or t.shape[1] % heads_of != 0 or t.stride(1) != 1:
+    cols = t.shape[1] if t.dim() == 2 else 0
+    if cols == 0 or cols % 64 != 0 or t.stride(1) != 1:
         raise RuntimeError(f"{name} must be [rows, heads*64] with contiguous rows")
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, the other tensors are on {device}")
-    return t.shape[1] // heads_of
+    return cols // 64
 
 
 def _ints(t: torch.Tensor, name: str, device) -> int:
@@ -655,7 +662,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     Rows that belong to no sequence are left as `out` has them (undefined without `out`)."""
     device = q.device
     heads, kv_heads = _rows(q, "q", device), _rows(k, "k", device)
-    if _rows(v, "v", device) != kv_heads or v.shape[0] != k.shape[0]:
+    rows, k_rows = q.shape[0], k.shape[0]
+    if _rows(v, "v", device) != kv_heads or v.shape[0] != k_rows:
         raise RuntimeError("k and v must have the same shape")
     batch = _ints(q_offsets, "q_offsets", device) - 1
     if _ints(k_offsets, "k_offsets", device) != batch + 1 or batch < 0:
@@ -668,13 +676,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
         if distance_bias.dim() != 2 or distance_bias.shape[0] != heads or distance_bias.device != device:
             raise RuntimeError("distance_bias must be [heads, n] on the device of the other tensors")
         n_bias = distance_bias.shape[1]
-    if out is not None and (_rows(out, "out", device) != heads or out.shape[0] != q.shape[0]):
+    if out is not None and (_rows(out, "out", device) != heads or out.shape[0] != rows):
         raise RuntimeError("out must have q's shape")
     lib = _abi.load()
     with _On(device) as stream:
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.float16, device=device)
-        rows, k_rows = q.shape[0], k.shape[0]
+            out = torch.empty(rows, heads * 64, dtype=torch.float16, device=device)
         if rows == 0 or batch == 0:
             return out
         ws, n = None, 0
