@@ -195,10 +195,12 @@ struct GradArgs {
   int groups;  // CTAs side by side over a row chunk's diagonals
   int chunks, chunk_rows;
   int parts;   // batch * chunks * groups
+  int walkers;
   Borders borders;
 };
 
-constexpr int kGradThreads = 256;
+constexpr int kGradWalkers = 192;  // threads that walk down the diagonals, at most
+constexpr int kGradOthers = 128;   // threads beside them for the rows' ragged ends; all sum the buckets
 constexpr int kGradRows = 128;  // rows of a chunk at most: the longest chain of single-precision additions
 
 // A CTA sums the diagonals of up to `kGradRows` rows of one plane (sequence, head), over a range of diagonals, then the
@@ -208,17 +210,18 @@ constexpr int kGradRows = 128;  // rows of a chunk at most: the longest chain of
 // into the thread's range, a number that only k_len mod V (M) decides and that repeats every V rows.  So every index of
 // a register is known at compile time, whatever the row length, and neighbouring threads load neighbouring vectors.
 // Rows that do not start on a 16-byte boundary have up to V - 1 elements ahead of their first whole vector and behind
-// their last; those are summed by diagonal, a thread each, ahead of the walk.
+// their last; those are summed by diagonal, a thread each, by threads of their own beside the walk.
 template <typename T, int M>
-__global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const __grid_constant__ GradArgs a) {
+__global__ void __launch_bounds__(kGradWalkers + kGradOthers, 2) relative_bias_grad_kernel(const __grid_constant__ GradArgs a) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  constexpr int kSpanMax = kGradThreads * V;
+  constexpr int kSpanMax = kGradWalkers * V;
   constexpr int kEdge = kGradRows + V;
-  __shared__ float low[kSpanMax + V], high[kSpanMax + V], block[kGradThreads + 1], edge[M != 0 ? 2 : 1][M != 0 ? kEdge : 1];
+  __shared__ float low[kSpanMax + V], high[kSpanMax + V], block[kGradWalkers + 1], edge[M != 0 ? 2 : 1][M != 0 ? kEdge : 1];
   __shared__ int first[kMaxBuckets];
   pdl_launch_dependents();
   const int t = threadIdx.x;
-  const int span = blockDim.x * V;
+  const int walkers = a.walkers;
+  const int span = walkers * V;
   for (int i = t; i < a.borders.count; i += blockDim.x) first[i] = a.borders.first[i];
   const int group = blockIdx.x % a.groups;
   const int chunk = blockIdx.x / a.groups;
@@ -240,26 +243,31 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
   if constexpr (M != 0) {
     // elements of row r (from q0) ahead of its first boundary
     auto lead_of = [&](int r) { return min((V - static_cast<int>((phase + static_cast<unsigned>(r) * M) % V)) % V, k_len); };
-    for (int x = t; x < 2 * kEdge; x += blockDim.x) {
-      const bool right = x >= kEdge;
+    for (int x = t - walkers; t >= walkers && x < rows + V - 1; x += kGradOthers) {
       // diagonal -(rows - 1) + x on the left, k_len - V + 1 - (rows - 1) + x on the right
-      const int d = (right ? k_len - V + 1 + x - kEdge : x) - (rows - 1);
-      T e[V - 1];
+      T e[2][V - 1];
 #pragma unroll
-      for (int i = 0; i < V - 1; ++i) {
-        const int col = right ? k_len - 1 - i : i;
-        const int r = col - d;
-        bool take = r >= 0 && r < rows && col >= 0 && col < k_len;
-        if (take) {
-          const int lead = lead_of(r);
-          take = right ? col >= lead + (k_len - lead) / V * V : col < lead;
+      for (int side = 0; side < 2; ++side) {
+        const int d = (side ? k_len - V + 1 + x : x) - (rows - 1);
+#pragma unroll
+        for (int i = 0; i < V - 1; ++i) {
+          const int col = side ? k_len - 1 - i : i;
+          const int r = col - d;
+          bool take = r >= 0 && r < rows && col >= 0 && col < k_len;
+          if (take) {
+            const int lead = lead_of(r);
+            take = side ? col >= lead + (k_len - lead) / V * V : col < lead;
+          }
+          e[side][i] = take ? base[static_cast<size_t>(r) * k_len + col] : static_cast<T>(0.f);
         }
-        e[i] = take ? base[static_cast<size_t>(r) * k_len + col] : static_cast<T>(0.f);
       }
-      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < V - 1; ++i) sum += static_cast<float>(e[i]);
-      edge[right][right ? x - kEdge : x] = sum;
+      for (int side = 0; side < 2; ++side) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < V - 1; ++i) sum += static_cast<float>(e[side][i]);
+        edge[side][x] = sum;
+      }
     }
   }
   float acc[2 * V - 1];
@@ -307,7 +315,7 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
   // one's values are added.
   const int n0 = c0 + 3 * V - 2 > 0 ? 0 : (-(c0 + 3 * V - 2)) / V + 1;
   const int n1 = min((rows + V - 1) / V, c0 < k_len ? (k_len - 1 - c0) / V + 1 : 0);
-  if (n0 < n1) {
+  if (t < walkers && n0 < n1) {
     uint4 v[V], w[V];
     load(v, n0);
 #pragma unroll 1
@@ -321,11 +329,13 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
     }
   }
   // Diagonal t * V + i of the range: the thread's own first V in `low`, what it holds of its right neighbour's in `high`
+  if (t < walkers) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) low[t * V + i] = acc[i];
+    for (int i = 0; i < V; ++i) low[t * V + i] = acc[i];
 #pragma unroll
-  for (int i = V; i < 2 * V - 1; ++i) high[t * V + i] = acc[i];
-  high[t * V + 2 * V - 1] = 0.f;
+    for (int i = V; i < 2 * V - 1; ++i) high[t * V + i] = acc[i];
+    high[t * V + 2 * V - 1] = 0.f;
+  }
   if (t == 0) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -335,7 +345,7 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
   }
   __syncthreads();
   // The diagonals' sums, in `low`, and those of V diagonals each, which the long runs below take.
-  for (int g = t; g <= static_cast<int>(blockDim.x); g += blockDim.x) {
+  for (int g = t; g <= walkers; g += blockDim.x) {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -344,8 +354,8 @@ __global__ void __launch_bounds__(kGradThreads) relative_bias_grad_kernel(const 
       if constexpr (M != 0) {
         if (x < span) {  // (the rest of the range is the next group's too)
           const int l = c_first + x + (rows - 1), r = l - (k_len - V + 1);
-          if (l >= 0 && l < kEdge) d += edge[0][l];
-          if (r >= 0 && r < kEdge) d += edge[1][r];
+          if (l >= 0 && l < rows + V - 1) d += edge[0][l];
+          if (r >= 0 && r < rows + V - 1) d += edge[1][r];
         }
       }
       low[x] = d;
@@ -415,7 +425,7 @@ bool bias_shape_ok(int num_buckets, int max_distance, int bidirectional, int hea
 
 struct GradSplit {
   int groups, chunks, chunk_rows;
-  int threads;  // of a CTA: no more than the diagonals ask for
+  int walkers;  // of a CTA: no more than the diagonals ask for
   long long parts;
 };
 GradSplit grad_split(int batch, int heads, int q_len, int k_len, int elem_bytes) {
@@ -427,14 +437,15 @@ GradSplit grad_split(int batch, int heads, int q_len, int k_len, int elem_bytes)
   while (s.chunk_rows > 16 && static_cast<long long>(batch) * heads * ((q_len + s.chunk_rows - 1) / s.chunk_rows) < 2 * 148) s.chunk_rows /= 2;
   s.chunks = (q_len + s.chunk_rows - 1) / s.chunk_rows;
   const long long vectors = (static_cast<long long>(k_len) + (q_len < s.chunk_rows ? q_len : s.chunk_rows) + 3 * v - 1) / v;
-  s.groups = static_cast<int>((vectors + kGradThreads - 1) / kGradThreads);
-  s.threads = static_cast<int>(((vectors + s.groups - 1) / s.groups + 31) / 32 * 32);
+  s.groups = static_cast<int>((vectors + kGradWalkers - 1) / kGradWalkers);
+  s.walkers = static_cast<int>(((vectors + s.groups - 1) / s.groups + 31) / 32 * 32);
   s.parts = static_cast<long long>(batch) * s.chunks * s.groups;
   return s;
 }
 
 template <typename T, int M>
-cudaError_t launch_grad(const GradArgs& a, int threads, cudaStream_t stream) {
+cudaError_t launch_grad(const GradArgs& a, cudaStream_t stream) {
+  const int threads = M != 0 ? a.walkers + kGradOthers : (a.walkers < kGradOthers ? kGradOthers : a.walkers);
   return launch_pdl(relative_bias_grad_kernel<T, M>, dim3(static_cast<unsigned>(a.groups) * a.chunks, a.heads, a.batch), dim3(threads),
                     0, stream, a);
 }
@@ -516,27 +527,28 @@ int bt_relative_position_bias_grad(const void* grad, int grad_fp32, int num_buck
   a.groups = split.groups;
   a.chunks = split.chunks;
   a.chunk_rows = split.chunk_rows;
+  a.walkers = split.walkers;
   a.parts = static_cast<int>(split.parts);
   bucket_borders(&a.borders, num_buckets, max_distance, bidirectional);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = cudaErrorInvalidValue;
   if (grad_fp32) {
     switch (k_len % 4) {
-      case 0: e = launch_grad<float, 0>(a, split.threads, s); break;
-      case 1: e = launch_grad<float, 1>(a, split.threads, s); break;
-      case 2: e = launch_grad<float, 2>(a, split.threads, s); break;
-      case 3: e = launch_grad<float, 3>(a, split.threads, s); break;
+      case 0: e = launch_grad<float, 0>(a, s); break;
+      case 1: e = launch_grad<float, 1>(a, s); break;
+      case 2: e = launch_grad<float, 2>(a, s); break;
+      case 3: e = launch_grad<float, 3>(a, s); break;
     }
   } else {
     switch (k_len % 8) {
-      case 0: e = launch_grad<__half, 0>(a, split.threads, s); break;
-      case 1: e = launch_grad<__half, 1>(a, split.threads, s); break;
-      case 2: e = launch_grad<__half, 2>(a, split.threads, s); break;
-      case 3: e = launch_grad<__half, 3>(a, split.threads, s); break;
-      case 4: e = launch_grad<__half, 4>(a, split.threads, s); break;
-      case 5: e = launch_grad<__half, 5>(a, split.threads, s); break;
-      case 6: e = launch_grad<__half, 6>(a, split.threads, s); break;
-      case 7: e = launch_grad<__half, 7>(a, split.threads, s); break;
+      case 0: e = launch_grad<__half, 0>(a, s); break;
+      case 1: e = launch_grad<__half, 1>(a, s); break;
+      case 2: e = launch_grad<__half, 2>(a, s); break;
+      case 3: e = launch_grad<__half, 3>(a, s); break;
+      case 4: e = launch_grad<__half, 4>(a, s); break;
+      case 5: e = launch_grad<__half, 5>(a, s); break;
+      case 6: e = launch_grad<__half, 6>(a, s); break;
+      case 7: e = launch_grad<__half, 7>(a, s); break;
     }
   }
   if (e == cudaSuccess)

@@ -75,7 +75,7 @@ constexpr int kRmsWarpRows = 4;  // rows (warps) of a CTA where a warp takes a r
 
 // WARPS warps to a row, NVEC vectors of 8 columns to a lane: hidden <= WARPS * 32 * 8 * NVEC.
 template <bool X_FP32, bool G_FP32, int OUT, int WARPS, int NVEC>
-__global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32) add_residual_rmsnorm_kernel(const RmsArgs a) {
+__global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32, WARPS >= 12 ? 2 : 1) add_residual_rmsnorm_kernel(const RmsArgs a) {
   __shared__ float scratch[2][WARPS];
   pdl_launch_dependents();
   constexpr int kLanes = WARPS * 32;
@@ -205,6 +205,7 @@ cudaError_t launch_by_width(const RmsArgs& a, cudaStream_t stream) {
   if (nvec <= 256) return launch_one<X_FP32, G_FP32, OUT, 4, 2>(a, stream);
   if (nvec <= 512) return launch_one<X_FP32, G_FP32, OUT, 8, 2>(a, stream);
   if (nvec <= 1024) return launch_one<X_FP32, G_FP32, OUT, 8, 4>(a, stream);
+  if (nvec <= 1536) return launch_one<X_FP32, G_FP32, OUT, 12, 4>(a, stream);
   return launch_one<X_FP32, G_FP32, OUT, 16, 4>(a, stream);
 }
 

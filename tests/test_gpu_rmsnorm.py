@@ -41,7 +41,7 @@ def inputs(rows, hidden, x_fp32, gamma_fp32, residual, device, seed=0):
     return tuple(t.to(device) if t is not None else None for t in (x, r, gamma))
 
 
-WIDTHS = [8, 16, 64, 120, 128, 136, 256, 264, 512, 520, 768, 776, 1024, 1032, 2048, 2056, 4096, 4104, 8192, 8200, 16384]
+WIDTHS = [8, 16, 64, 120, 128, 136, 256, 264, 512, 520, 768, 776, 1024, 1032, 2048, 2056, 4096, 4104, 8192, 8200, 12288, 12296, 16384]
 
 
 @pytest.mark.parametrize("hidden", WIDTHS)
