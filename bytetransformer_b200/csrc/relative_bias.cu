@@ -107,7 +107,7 @@ struct BiasArgs {
   const void* table;  // [buckets, heads]
   void* out;          // [heads, q_len, k_len]
   int heads, q_len, k_len, q_start;
-  int rows, cols;     // of a CTA's tile
+  int rows, cols;     // of a CTA's tile (the last one of a row: up to V columns more)
   Borders borders;
 };
 
@@ -128,9 +128,12 @@ __global__ void __launch_bounds__(kBiasThreads) relative_bias_kernel(const __gri
   const int q0 = blockIdx.y * a.rows;
   const int k0 = blockIdx.x * a.cols;
   const int rows = min(a.rows, a.q_len - q0);
-  const int cols = min(a.cols, a.k_len - k0);
-  const int diagonals = rows + cols - 1;
-  const int pitch = (a.rows + a.cols + V + V - 1) / V * V;  // elements of a copy, a multiple of 16 bytes
+  // A row's share of the tile starts and ends on 16-byte boundaries of its own (up to V - 1 columns on), except at the row's ends.
+  // (The last tile has more than V columns, so these boundaries lie inside it, or is the only one.)
+  const bool first_cols = blockIdx.x == 0, last_cols = blockIdx.x + 1 == gridDim.x;
+  const int cols = last_cols ? a.k_len - k0 : a.cols;
+  const int diagonals = rows + cols + (last_cols ? 0 : V - 1) - 1;
+  const int pitch = (a.rows + a.cols + 4 * V - 1) / V * V;  // elements of a copy, a multiple of 16 bytes
   T* copies = reinterpret_cast<T*>(smem);
   for (int i = threadIdx.x; i < a.borders.count; i += kBiasThreads) first[i] = a.borders.first[i];
   pdl_wait();
@@ -160,28 +163,27 @@ __global__ void __launch_bounds__(kBiasThreads) relative_bias_kernel(const __gri
   fence_proxy_async_smem();
   __syncthreads();
   T* out = reinterpret_cast<T*>(a.out) + (static_cast<size_t>(head) * a.q_len + q0) * a.k_len + k0;
-  // elements of row r ahead of its first 16-byte boundary
-  auto head_of = [&](int r) {
+  // elements of row r of the tile ahead of its first 16-byte boundary, and those from there on that whole vectors hold
+  auto lead_of = [&](int r) {
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out + static_cast<size_t>(r) * a.k_len) / sizeof(T));
     return min(static_cast<int>((V - at % V) % V), cols);
   };
+  auto body_of = [&](int lead) { return last_cols ? (cols - lead) / V * V : cols; };
   // (the lanes of a warp issue their copies one after the other: the rows go round the warps)
   for (int r = (threadIdx.x & 31) * (kBiasThreads / 32) + (threadIdx.x >> 5); r < rows; r += kBiasThreads) {
-    const int lead = head_of(r);
-    const int body = (cols - lead) / V * V;
+    const int lead = lead_of(r), body = body_of(lead);
     const int x = rows - 1 - r + lead;
     if (body > 0)
       bulk_store(out + static_cast<size_t>(r) * a.k_len + lead, copies + (x % V) * pitch + x / V * V, static_cast<uint32_t>(body * sizeof(T)));
   }
   tma_store_commit();
-  if (a.k_len % V != 0) {
-    // the ragged ends of the rows, 2 V - 2 elements at most: 2 V lanes for each row
+  if (a.k_len % V != 0 && (first_cols || last_cols)) {
+    // the rows' ragged ends, 2 V - 2 elements at most: 2 V lanes for each row
     for (int i = threadIdx.x; i < rows * 2 * V; i += kBiasThreads) {
       const int r = i / (2 * V), s = i % (2 * V);
-      const int lead = head_of(r);
-      const int body = (cols - lead) / V * V;
-      const int c = s < V ? s : lead + body + s - V;
-      if (s < V ? c < lead : c < cols) out[static_cast<size_t>(r) * a.k_len + c] = copies[rows - 1 - r + c];
+      const int lead = lead_of(r);
+      const int c = s < V ? s : lead + body_of(lead) + s - V;
+      if (s < V ? first_cols && c < lead : last_cols && c < cols) out[static_cast<size_t>(r) * a.k_len + c] = copies[rows - 1 - r + c];
     }
   }
   tma_store_wait_read();
@@ -200,7 +202,8 @@ struct GradArgs {
 };
 
 constexpr int kGradWalkers = 192;  // threads that walk down the diagonals, at most
-constexpr int kGradOthers = 128;   // threads beside them for the rows' ragged ends; all sum the buckets
+constexpr int kGradOthers = 64;    // threads beside them for the rows' ragged ends (32 to 128: 8 sequences, 12 heads, 509 x 509 17.0,
+                                   // 16.4, 25.3 us); all sum the buckets
 constexpr int kGradRows = 128;  // rows of a chunk at most: the longest chain of single-precision additions
 
 // A CTA sums the diagonals of up to `kGradRows` rows of one plane (sequence, head), over a range of diagonals, then the
@@ -445,7 +448,7 @@ GradSplit grad_split(int batch, int heads, int q_len, int k_len, int elem_bytes)
 
 template <typename T, int M>
 cudaError_t launch_grad(const GradArgs& a, cudaStream_t stream) {
-  const int threads = M != 0 ? a.walkers + kGradOthers : (a.walkers < kGradOthers ? kGradOthers : a.walkers);
+  const int threads = M != 0 ? a.walkers + kGradOthers : (a.walkers < 128 ? 128 : a.walkers);
   return launch_pdl(relative_bias_grad_kernel<T, M>, dim3(static_cast<unsigned>(a.groups) * a.chunks, a.heads, a.batch), dim3(threads),
                     0, stream, a);
 }
@@ -453,12 +456,12 @@ cudaError_t launch_grad(const GradArgs& a, cudaStream_t stream) {
 template <typename T, typename TableT>
 cudaError_t launch_bias(BiasArgs a, cudaStream_t stream) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  a.cols = a.k_len < 256 ? a.k_len : 256;
+  a.cols = a.k_len <= 256 + V ? a.k_len : 256;
   a.rows = a.q_len < 64 ? a.q_len : 64;
-  const size_t smem = static_cast<size_t>(V) * ((a.rows + a.cols + 2 * V - 1) / V * V) * sizeof(T);
+  const size_t smem = static_cast<size_t>(V) * ((a.rows + a.cols + 4 * V - 1) / V * V) * sizeof(T);
   const long long tiles_q = (a.q_len + a.rows - 1) / a.rows;
   if (tiles_q > 65535) return cudaErrorInvalidValue;
-  return launch_pdl(relative_bias_kernel<T, TableT>, dim3((a.k_len + a.cols - 1) / a.cols, static_cast<unsigned>(tiles_q), a.heads),
+  return launch_pdl(relative_bias_kernel<T, TableT>, dim3(a.k_len == a.cols ? 1 : (a.k_len - V + a.cols - 1) / a.cols, static_cast<unsigned>(tiles_q), a.heads),
                     dim3(kBiasThreads), smem, stream, a);
 }
 

@@ -34,7 +34,7 @@ def by_distance(q, k, start, buckets, dist, both):
 
 BUCKETS = [(32, 128, True), (32, 128, False), (4, 3, True), (2, 2, False), (256, 129, False), (256, 1 << 20, False),
            (48, 400, False), (64, 1000, True), (18, 20, True)]
-SHAPES = [(1, 1, 0), (1, 700, 699), (7, 5, 0), (64, 64, 0), (65, 1025, 3), (130, 197, 1000), (257, 1032, -300), (128, 8, 0),
+SHAPES = [(1, 1, 0), (1, 700, 699), (7, 5, 0), (64, 64, 0), (65, 1025, 3), (70, 263, 0), (70, 264, 0), (66, 265, 1), (3, 511, 0), (3, 513, 0), (5, 520, 0), (5, 521, 0), (130, 197, 1000), (257, 1032, -300), (128, 8, 0),
           (3, 4100, 2000), (200, 1027, 1 << 28), (5, 9, -(1 << 28))]
 
 
