@@ -12,7 +12,8 @@ __all__ = ["BtError", "LIB_PATH", "Encoder", "bert_transformer"]
 
 
 def __getattr__(name):
-    if name in ("Encoder", "bert_transformer", "build_offsets", "pack_rows", "restore_rows"):
+    if name in ("Encoder", "bert_transformer", "build_offsets", "pack_rows", "restore_rows", "relative_position_bias",
+                "relative_position_bias_grad", "add_residual_rmsnorm", "add_residual_rmsnorm_e4m3", "window_attention"):
         from . import encoder
         return getattr(encoder, name)
     raise AttributeError(name)

@@ -18,6 +18,7 @@
 //   O += P V takes them; the next S of a group is issued right behind that product.  One thread issues a group's MMAs and
 //   they execute in order, so no barrier stands between P V and the S that overwrites P.
 // window_few_kernel: calls of few queries (single tokens), see there.
+#include <float.h>
 #include <math.h>
 
 #include <mutex>
@@ -158,6 +159,12 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// A bias in log2 units.  The type's lowest value stays a number (a row that sees only such keys weighs them alike, as the
+// formula says), an infinity one (a key at such a distance is not seen).
+__device__ __forceinline__ float bias_log2(float b) {
+  const float x = b * 1.4426950408889634f;
+  return fabsf(b) < INFINITY ? fminf(fmaxf(x, -FLT_MAX), FLT_MAX) : x;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -504,16 +511,19 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const int u0 = j * kKeys;
           // index of the value of column 0 and row 127
           const int at[2] = {keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left, u0 - it.p0 - 127 + args.bias_left};
-          const bool is_flat = u0 >= keys.ns && (at[0] >= top || at[0] + kKeys + 126 <= 0);
+          // One value for the whole tile need not be added to each score (unless it is so large that the sum swallows the scores:
+          // then it has to, as in tiles of several values)
+          const float one = bias_log2(__ldg(bias + (at[0] >= top ? top : 0)));
+          const bool is_flat = u0 >= keys.ns && (at[0] >= top || at[0] + kKeys + 126 <= 0) && (fabsf(one) < 1e30f || one == -INFINITY);
           if (lane == 0) flat[g] = is_flat;
           if (is_flat) {
-            if (lane == 0) slice->copy[0][0][0] = __ldg(bias + (at[0] >= top ? top : 0)) * 1.4426950408889634f;
+            if (lane == 0) slice->copy[0][0][0] = one;
           } else {
 #pragma unroll 1
             for (int run = 0; run < (u0 < keys.ns ? 2 : 1); ++run) {
               float v[6];
 #pragma unroll
-              for (int i = 0; i < 6; ++i) v[i] = __ldg(bias + min(max(at[run] + i * 32 + lane, 0), top)) * 1.4426950408889634f;
+              for (int i = 0; i < 6; ++i) v[i] = bias_log2(__ldg(bias + min(max(at[run] + i * 32 + lane, 0), top)));
 #pragma unroll
               for (int i = 0; i < 6; ++i)
 #pragma unroll
@@ -948,7 +958,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __g
         const int h = i >> 1, u = u0 + 8 * n + 2 * c + (i & 1);
         const bool seen = u < a_hi[h] || (u >= b_lo[h] && u < b_hi[h]);
         float x = s[n][i] * w.scale_log2e;
-        if (BIAS) x = fmaf(__ldg(bias[h] + min(max(key_of(u) - pos[h] + w.bias_left, 0), w.bias_n - 1)), 1.4426950408889634f, x);
+        if (BIAS) x += bias_log2(__ldg(bias[h] + min(max(key_of(u) - pos[h] + w.bias_left, 0), w.bias_n - 1)));
         s[n][i] = seen ? x : -INFINITY;
         top[h] = fmaxf(top[h], s[n][i]);
       }

@@ -515,6 +515,12 @@ def _half_or_float(t: torch.Tensor, name: str, device=None) -> int:
     return int(t.dtype == torch.float32)
 
 
+def _check_distances(q_len, k_len, max_distance, q_start):
+    """The library's lengths and positions are 32 bits wide: what does not fit is refused before it is cut off."""
+    if q_len < 0 or k_len < 0 or max(q_len, k_len, abs(q_start)) > 1 << 29 or not 0 < max_distance <= 1 << 20:
+        raise RuntimeError("lengths and q_start must be at most 2^29, max_distance at most 2^20")
+
+
 def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_distance: int = 128,
                            bidirectional: bool = True, q_start: int = 0,
                            out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
@@ -527,6 +533,7 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_d
     if out_dtype not in (torch.float16, torch.float32):
         raise RuntimeError("out_dtype must be torch.float16 or torch.float32")
     buckets, heads = table.shape
+    _check_distances(q_len, k_len, max_distance, q_start)
     if q_len == 0 or k_len == 0:
         return torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
     lib = _abi.load()
@@ -549,6 +556,7 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
         raise RuntimeError("grad must be [heads, q_len, k_len] or [batch, heads, q_len, k_len]")
     batch = int(grad.shape[0]) if grad.dim() == 4 else 1
     heads, q_len, k_len = grad.shape[-3:]
+    _check_distances(q_len, k_len, max_distance, q_start)
     if grad.numel() == 0:
         return torch.zeros(num_buckets, heads, dtype=torch.float32, device=grad.device)
     lib = _abi.load()
@@ -676,8 +684,16 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
         if distance_bias.dim() != 2 or distance_bias.shape[0] != heads or distance_bias.device != device:
             raise RuntimeError("distance_bias must be [heads, n] on the device of the other tensors")
         n_bias = distance_bias.shape[1]
+        if not 0 <= bias_left < n_bias:
+            raise RuntimeError("bias_left must be a place in distance_bias")
     if out is not None and (_rows(out, "out", device) != heads or out.shape[0] != rows):
         raise RuntimeError("out must have q's shape")
+    if max(max_q_len, max_k_len) >= 1 << 30 or sinks < 0:
+        raise RuntimeError("max_q_len and max_k_len must be below 2^30, sinks not negative")
+    # bounds that no distance reaches, however large, are none (the library's are 32 bits wide)
+    left = -1 if left < 0 or left >= max_k_len else left
+    right = -1 if right < 0 or right >= 1 << 30 else right
+    sinks = min(sinks, max_k_len)
     lib = _abi.load()
     with _On(device) as stream:
         if out is None:
@@ -695,7 +711,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
             out.stride(0), q_offsets.data_ptr(), k_offsets.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
             batch, heads, kv_heads, rows, k_rows, max_q_len, max_k_len, left, right, sinks, scale,
-            distance_bias.data_ptr() if distance_bias is not None else None, n_bias, bias_left,
+            distance_bias.data_ptr() if distance_bias is not None else None, n_bias, bias_left if n_bias else 0,
             ws.data_ptr() if n else None, n)
         rc = lib.bt_window_attention(C.byref(a), stream)
     if rc != _abi.BT_OK:

@@ -349,7 +349,8 @@ int bt_add_residual_rmsnorm_e4m3(const void* x, int x_fp32, const void* residual
  *   of its Lk keys: the last query sees the last key.  Key j is visible to it if
  *       j <= p + right   and   (j >= p - left  or  j < sinks);        left < 0, right < 0: no such bound
  *       out = sum over visible j of softmax(scale * q.k_j + distance_bias[h, bias_left + (j - p)]) * v_j,
- *   and zeros where no key is visible (Lk = 0, p + right < 0).  Distances outside the table take its outermost values;
+ *   and zeros where no key is visible (Lk = 0, p + right < 0).  Distances outside the table take its outermost values; a
+ *   key at a distance with a bias of minus infinity is not visible;
  *   distance_bias (fp32 [head_num, bias_len], or NULL) is what bt_relative_position_bias makes of a learned table with
  *   q_len = 1, q_start = bias_left.
  *   Lk: k_offsets[b+1] - k_offsets[b] rows from k_offsets[b] of k and v, or k_lens[b] of them (k_lens not NULL): a cache

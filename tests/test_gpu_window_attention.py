@@ -44,7 +44,9 @@ def definition(q, k, v, q_off, k_off, k_lens, left, right, sinks, bias, bias_lef
                 s = s + bias[h].double()[(j - p + bias_left).clamp(0, bias.shape[1] - 1)]
             w = torch.softmax(s.masked_fill(~seen, -math.inf), dim=1).nan_to_num(0.0)
             o = w @ vv
-            big = float((qq.norm(dim=1).max() * kk.norm(dim=1).max() * scale)) + (float(bias.abs().max()) if bias is not None else 0.0)
+            # a bias of the type's lowest value or beyond swallows the score, here and there, to the last bit
+            small = bias[bias.abs() < 1e30] if bias is not None else torch.zeros(1)
+            big = float((qq.norm(dim=1).max() * kk.norm(dim=1).max() * scale)) + (float(small.abs().max()) if small.numel() else 0.0)
             slack = big * 70 * 2.0 ** -24 + 2.0 ** -21
             out[rows, c] = o
             tol[rows, c] = (w @ vv.abs()) * (2.0 ** -11 + 2 * slack) * 1.01 + \
@@ -185,6 +187,49 @@ def test_large_scores(cuda_device):
     q, k = (q.sign() * 2).half(), (k * 0 + ramp * q[:, :2 * D].sign()[:1]).half()
     check(q, k, v, off, off, 900, 900, None, 400, 50, 2)
     check(q, k, v, off, off, 900, 900, None, -1, -1, 0, torch.linspace(-60, 60, 600, device=cuda_device).repeat(2, 1), 300)
+
+
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min, -60000.0])
+@pytest.mark.parametrize("one", [False, True])
+def test_biases_that_mask(cuda_device, low, one):
+    """The type's lowest value, minus infinity: as masks by distance, and where a row sees nothing else."""
+    heads = 2
+    bias = torch.randn(heads, 201, device=cuda_device)
+    bias[0, :60] = low       # far to the left, for a head
+    bias[0, 101:103] = low
+    bias[1] = low            # every distance of the other
+    if one:
+        q, k, v, off = packed([300, 40, 1], heads, heads, cuda_device, seed=13)
+        q = q[:3]
+        q_off = torch.arange(4, dtype=torch.int32, device=cuda_device)
+        got = check(q, k, v, q_off, off, 1, 300, None, -1, 0, 0, bias, 100)
+    else:
+        q, k, v, off = packed([300, 40, 1], heads, heads, cuda_device, seed=13)
+        got = check(q, k, v, off, off, 300, 300, None, 250, 250, 2, bias, 100)
+    assert torch.isfinite(got).all()
+    if low == -math.inf:
+        assert (got[:, D:] == 0).all() and (got[:, :D] != 0).any()
+
+
+def test_infinite_and_nan_queries_stay_in_their_row(cuda_device):
+    q, k, v, off = packed([200, 70], 2, 2, cuda_device, seed=14)
+    clean = check(q, k, v, off, off, 200, 200, None, 60, 10, 2)
+    q[50, 3] = float("nan")
+    q[220, D + 5] = float("inf")
+    from bytetransformer_b200 import encoder as E
+    got = E.window_attention(q, k, v, off, off, 200, 200, left=60, right=10, sinks=2)
+    assert torch.isnan(got[50, :D]).all() and not torch.isfinite(got[220, D:]).any()
+    got[50, :D] = clean[50, :D]
+    got[220, D:] = clean[220, D:]
+    assert torch.isfinite(got).all() and ((got - clean).abs() <= 2.0 ** -9 * clean.abs() + 2.0 ** -14).all()
+
+
+def test_bounds_beyond_every_distance_are_none(cuda_device):
+    from bytetransformer_b200 import encoder as E
+    q, k, v, off = packed([200, 70], 2, 2, cuda_device, seed=15)
+    want = E.window_attention(q, k, v, off, off, 200, 200)
+    for big in (200, 1 << 30, (1 << 31) - 1, 1 << 31, 1 << 32, (1 << 32) + 3, 1 << 70):
+        assert torch.equal(want, E.window_attention(q, k, v, off, off, 200, 200, left=big, right=big, sinks=big))
 
 
 def test_rows_around_the_sequences_do_not_matter(cuda_device):
