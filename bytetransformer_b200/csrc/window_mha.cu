@@ -505,30 +505,39 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int j = 0; j < keys.tiles; ++j) {
           const int g = (j + static_cast<int>(n)) & 1;
           const uint32_t cnt = g ? count[1]++ : count[0]++;
-          ok = wait_role(&bias_empty[g], (cnt & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
-          if (!ok) break;
           BiasSlice* slice = reinterpret_cast<BiasSlice*>(smem + L::kBias) + g;
           const int u0 = j * kKeys;
           // index of the value of column 0 and row 127
           const int at[2] = {keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left, u0 - it.p0 - 127 + args.bias_left};
+          float v[6];
+          auto load = [&](int from) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) v[i] = __ldg(bias + min(max(from + i * 32 + lane, 0), top));
+          };
+          auto lay = [&](int run) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) {
+              const float x = bias_log2(v[i]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (i * 32 + lane >= k) slice->copy[run][k][i * 32 + lane - k] = x;
+            }
+          };
+          load(at[0]);  // (on the way while the group still reads the slice before)
+          ok = wait_role(&bias_empty[g], (cnt & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
+          if (!ok) break;
           // One value for the whole tile need not be added to each score (unless it is so large that the sum swallows the scores:
           // then it has to, as in tiles of several values)
-          const float one = bias_log2(__ldg(bias + (at[0] >= top ? top : 0)));
+          const float one = bias_log2(v[0]);
           const bool is_flat = u0 >= keys.ns && (at[0] >= top || at[0] + kKeys + 126 <= 0) && (fabsf(one) < 1e30f || one == -INFINITY);
           if (lane == 0) flat[g] = is_flat;
           if (is_flat) {
             if (lane == 0) slice->copy[0][0][0] = one;
           } else {
-#pragma unroll 1
-            for (int run = 0; run < (u0 < keys.ns ? 2 : 1); ++run) {
-              float v[6];
-#pragma unroll
-              for (int i = 0; i < 6; ++i) v[i] = bias_log2(__ldg(bias + min(max(at[run] + i * 32 + lane, 0), top)));
-#pragma unroll
-              for (int i = 0; i < 6; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (i * 32 + lane >= k) slice->copy[run][k][i * 32 + lane - k] = v[i];
+            lay(0);
+            if (u0 < keys.ns) {
+              load(at[1]);
+              lay(1);
             }
           }
           __syncwarp();
@@ -674,10 +683,14 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
                 for (int i = B + 16 * h; i < B + 16 * h + 16; i += 4) {
                   const float4 b = *reinterpret_cast<const float4*>(from + i);
-                  s[i] = __float_as_uint(fmaf(__uint_as_float(s[i]), c, b.x));
-                  s[i + 1] = __float_as_uint(fmaf(__uint_as_float(s[i + 1]), c, b.y));
-                  s[i + 2] = __float_as_uint(fmaf(__uint_as_float(s[i + 2]), c, b.z));
-                  s[i + 3] = __float_as_uint(fmaf(__uint_as_float(s[i + 3]), c, b.w));
+                  const unsigned long long c2 = pack_f32x2(c, c);
+                  float x0, x1;
+                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, pack_f32x2(b.x, b.y)), x0, x1);
+                  s[i] = __float_as_uint(x0);
+                  s[i + 1] = __float_as_uint(x1);
+                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), c2, pack_f32x2(b.z, b.w)), x0, x1);
+                  s[i + 2] = __float_as_uint(x0);
+                  s[i + 3] = __float_as_uint(x1);
                 }
               }
             }
