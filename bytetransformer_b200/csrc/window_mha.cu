@@ -6,9 +6,9 @@
 //   out_i = sum_j softmax_j(scale * q_i . k_j + bias[h, j - p]) v_j     over the keys it sees, 0 where it sees none.
 //
 // window_mha_kernel: 128 query rows of a head at a time.  The keys that any of them sees are a run of the first keys
-// and a run around the tile; the two are laid end to end ("virtual" keys: the first run, in steps of 16, then the second) and
+// and a run around the tile; the two are laid end to end ("virtual" keys: the first run, in steps of 32, then the second) and
 // walked in tiles of 64, so a handful of first tokens does not cost a tile of its own and the window starts wherever
-// the first row's does.  The tile that holds the seam is fetched in boxes of 16 keys.
+// the first row's does.  The tile that holds the seam is fetched in boxes of 32 keys.
 //   What bounds it is the chain of a softmax (scores from tensor memory, maximum, exponentials, weights back), not the tensor
 //   core: a warp by itself leaves the special-function unit idle more than half of the time.  So two groups of four warps
 //   share the 128 rows, one takes the even tiles, the other the odd ones, each with scores, weights, reference, sum and O of
@@ -38,7 +38,7 @@ constexpr int kQTile = kRows * kHeadDim * 2;   // 16 KiB
 constexpr int kKvTile = kKeys * kHeadDim * 2;  // 8 KiB
 constexpr int kThreads = 384;  // two groups of four softmax warps; loads, MMAs of either group, bias
 constexpr int kSlots = 4;  // items between the loader and the other roles
-constexpr int kSeam = 16;  // keys of a box of the tile with the seam
+constexpr int kSeam = 32;  // keys of a box of the tile with the seam
 
 struct WindowArgs {
   __half* out;
@@ -240,25 +240,27 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return below_hi & ~below_lo;
 }
 
-// The bias of a tile for all its rows: value of (column c, row r) at c - r + 127, in log2 units; columns of the second run of
-// keys [0], of the first [1].  Four copies, each an element further on, so that a thread reads its row's values four at a
-// time wherever they start; the pitch keeps the copies that neighbouring rows read in different banks.
-constexpr int kBiasPitch = 200;
+// The bias of half a tile for a warp's rows: value of (column c, lane l) at c - l + 31, in log2 units.  Four copies, each an
+// element further on, so that a lane reads its row's values four at a time wherever they start; the pitch keeps the copies
+// that neighbouring lanes read in different banks.
+constexpr int kBiasPitch = 72;
 struct BiasSlice {
-  float copy[2][4][kBiasPitch];
+  float copy[4][kBiasPitch];
 };
 
-template <bool BIAS>
 struct Layout {
-  static constexpr int kStages = 2;              // K and V tiles, for each group
-  static constexpr int kQStages = BIAS ? 1 : 2;  // (the bias takes the place of the second Q tile)
+  static constexpr int kStages = 2;  // Q tiles; K and V tiles for each group
   static constexpr int kQ = 0;
-  static constexpr int kK = kQ + kQStages * kQTile;
+  static constexpr int kK = kQ + kStages * kQTile;
   static constexpr int kV = kK + 2 * kStages * kKvTile;
-  static constexpr int kOut = kV + 2 * kStages * kKvTile;  // 32 rows x 64 bytes for each of the eight warps
-  static constexpr int kBias = kOut + 8 * 32 * 64;
-  static constexpr int kBar = kBias + (BIAS ? 2 * static_cast<int>(sizeof(BiasSlice)) : 0);
+  // For each of the eight warps: the bias of the half tile that it is at, then its reference and sums for the other group; or
+  // 32 output rows of 64 bytes
+  static constexpr int kOwn = kV + 2 * kStages * kKvTile;
+  static constexpr int kOwnBytes = 32 * 64;
+  static constexpr int kOwnSums = sizeof(BiasSlice);
+  static constexpr int kBar = kOwn + 8 * kOwnBytes;
   static constexpr int kBytes = kBar + 1024;
+  static_assert(kOwnSums % 8 == 0 && kOwnSums + 32 * 8 <= kOwnBytes, "a warp's own bytes");
 };
 
 template <bool BIAS>
@@ -266,8 +268,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k16,
                   const __grid_constant__ CUtensorMap tm_v16, const WindowArgs args) {
-  using L = Layout<BIAS>;
-  constexpr int kStages = L::kStages, kQStages = L::kQStages;
+  using L = Layout;
+  constexpr int kStages = L::kStages, kQStages = L::kStages;
   constexpr int kLoadTimeout = kStatusMhaLoadTimeout, kMmaTimeout = kStatusMhaMmaTimeout, kSoftmaxTimeout = kStatusMhaSoftmaxTimeout;
   extern __shared__ __align__(1024) uint8_t smem[];
 
@@ -287,14 +289,11 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* item_full = bars + 42;            // [kSlots]
   uint64_t* item_empty = bars + 46;           // [kSlots]
   uint64_t* taken_full = bars + 50;
-  uint64_t* bias_full = bars + 51;            // [group] by the group's tiles
-  uint64_t* bias_empty = bars + 53;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 55);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 51);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   uint8_t* taken = smem + L::kBar + 480;       // 16 bytes
   Item* items = reinterpret_cast<Item*>(smem + L::kBar + 496);
-  volatile int* flat = reinterpret_cast<volatile int*>(smem + L::kBar + 496 + kSlots * sizeof(Item));  // [group]
-  static_assert(496 + kSlots * sizeof(Item) + 2 * 4 <= 1024, "barriers and items");
+  static_assert(496 + kSlots * sizeof(Item) <= 1024, "barriers and items");
 
   const int warp = uniform_int(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
@@ -306,8 +305,6 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
       mbar_init(&o_done[s], 1);
-      mbar_init(&bias_full[s], 1);
-      mbar_init(&bias_empty[s], 4);
     }
     for (int s = 0; s < 2 * kStages; ++s) {
       mbar_init(&k_full[s], 1);
@@ -321,7 +318,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&item_full[s], 1);
-      mbar_init(&item_empty[s], BIAS ? 11 : 10);
+      mbar_init(&item_empty[s], 10);
     }
     mbar_init(taken_full, 1);
     *abort_flag = smem_ok ? 0 : 1;
@@ -494,59 +491,6 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         read_item(n);
         have = it.rows > 0;
       }
-    } else if (BIAS) {
-      // ------------------------------------------------------------------- bias
-      bool have = own_item(), ok = true;
-      uint32_t count[2] = {0, 0};
-      for (uint32_t n = 0; have && ok; ++n) {
-        const Keys keys = keys_of(args, it);
-        const float* bias = args.bias + static_cast<long long>(it.head) * args.bias_n;
-        const int top = args.bias_n - 1;
-        for (int j = 0; j < keys.tiles; ++j) {
-          const int g = (j + static_cast<int>(n)) & 1;
-          const uint32_t cnt = g ? count[1]++ : count[0]++;
-          BiasSlice* slice = reinterpret_cast<BiasSlice*>(smem + L::kBias) + g;
-          const int u0 = j * kKeys;
-          // index of the value of column 0 and row 127
-          const int at[2] = {keys.ws + u0 - keys.ns - it.p0 - 127 + args.bias_left, u0 - it.p0 - 127 + args.bias_left};
-          float v[6];
-          auto load = [&](int from) {
-#pragma unroll
-            for (int i = 0; i < 6; ++i) v[i] = __ldg(bias + min(max(from + i * 32 + lane, 0), top));
-          };
-          auto lay = [&](int run) {
-#pragma unroll
-            for (int i = 0; i < 6; ++i) {
-              const float x = bias_log2(v[i]);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (i * 32 + lane >= k) slice->copy[run][k][i * 32 + lane - k] = x;
-            }
-          };
-          load(at[0]);  // (on the way while the group still reads the slice before)
-          ok = wait_role(&bias_empty[g], (cnt & 1u) ^ 1u, abort_flag, args.status, kLoadTimeout);
-          if (!ok) break;
-          // One value for the whole tile need not be added to each score (unless it is so large that the sum swallows the scores:
-          // then it has to, as in tiles of several values)
-          const float one = bias_log2(v[0]);
-          const bool is_flat = u0 >= keys.ns && (at[0] >= top || at[0] + kKeys + 126 <= 0) && (fabsf(one) < 1e30f || one == -INFINITY);
-          if (lane == 0) flat[g] = is_flat;
-          if (is_flat) {
-            if (lane == 0) slice->copy[0][0][0] = one;
-          } else {
-            lay(0);
-            if (u0 < keys.ns) {
-              load(at[1]);
-              lay(1);
-            }
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bias_full[g]);
-        }
-        if (!ok || !wait_role(&item_full[n % kSlots], parity(n), abort_flag, args.status, kLoadTimeout)) break;
-        read_item(n);
-        have = it.rows > 0;
-      }
     }
   } else {
     // ---------------------------------------------------------------- softmax (warps 0..3 and 4..7)
@@ -557,7 +501,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const uint32_t t_s = t_lane + 64u * g, t_o = t_lane + 128u + 64u * g;
     const float c = args.scale_log2e;
     uint32_t cnt = 0;      // the group's tiles so far
-    uint8_t* stage_out = smem + L::kOut + warp * (32 * 64);  // output rows, or what the other group needs to know
+    uint8_t* own = smem + L::kOwn + warp * L::kOwnBytes;
     uint32_t o_items[2] = {0, 0};            // items in which this group, the other one had tiles
     uint32_t handed = 0, received = 0;
     bool lent = false;                       // the other group may still be reading this one's O, reference and sum
@@ -569,7 +513,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     // The end of an item.  The group of the odd tiles says what its reference and sum are and goes on (its next product waits
     // until its O has been read, see take_back).
     auto hand_over = [&](float m, float l) {
-      reinterpret_cast<float2*>(stage_out)[lane] = make_float2(m, l);
+      reinterpret_cast<float2*>(own + L::kOwnSums)[lane] = make_float2(m, l);
       __syncwarp();
       if (lane == 0) mbar_arrive(&merge_full[g * 4 + quarter]);
       lent = true;
@@ -587,7 +531,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       tc_fence_after();
       if (both) {
-        theirs = reinterpret_cast<const float2*>(smem + L::kOut + other * (32 * 64))[lane];
+        theirs = reinterpret_cast<const float2*>(smem + L::kOwn + other * L::kOwnBytes + L::kOwnSums)[lane];
       }
       const float top = fmaxf(theirs.x, m);
       float f0 = m == -INFINITY ? 0.f : ex2(m - top);
@@ -619,7 +563,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           w.y = pack_half2(__uint_as_float(a[u * 8 + 2]), __uint_as_float(a[u * 8 + 3]));
           w.z = pack_half2(__uint_as_float(a[u * 8 + 4]), __uint_as_float(a[u * 8 + 5]));
           w.w = pack_half2(__uint_as_float(a[u * 8 + 6]), __uint_as_float(a[u * 8 + 7]));
-          *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = w;
+          *reinterpret_cast<uint4*>(own + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = w;
         }
         if (h == 1) tc_fence_before();
         __syncwarp();
@@ -627,7 +571,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int row = 8 * k + (lane >> 2);
-          const uint4 w = *reinterpret_cast<const uint4*>(stage_out + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
+          const uint4 w = *reinterpret_cast<const uint4*>(own + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4));
           if (quarter * 32 + row < it.rows) *reinterpret_cast<uint4*>(out + row * args.out_stride + 32 * h) = w;
         }
         __syncwarp();
@@ -653,18 +597,22 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       for (int j = first; j < keys.tiles; j += 2, ++cnt) {
         const int u0 = j * kKeys;
         const int slot = g * kStages + static_cast<int>(cnt % kStages);
+        // The bias of a half: of (column 0, lane 31) at index bias_at; 63 values from there on, two to a lane, on the way while S is
+        // waited for.
+        int bias_at[2];
+        float bias_v[2][2];
+        if (BIAS) {
+          const float* table = args.bias + static_cast<long long>(it.head) * args.bias_n;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int u = u0 + 32 * h;
+            bias_at[h] = (u < keys.ns ? u : keys.ws + u - keys.ns) - (it.p0 + quarter * 32 + 31) + args.bias_left;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) bias_v[h][i] = __ldg(table + min(max(bias_at[h] + 32 * i + lane, 0), args.bias_n - 1));
+          }
+        }
         mbar_wait_anyway_lane(&s_full[g], cnt & 1u, abort_flag, args.status, kSoftmaxTimeout);
         tc_fence_after();
-        const float* slice = nullptr;
-        bool is_flat = true;
-        float scale = c, shift = 0.f;  // log2 units of what `s` holds below
-        if (BIAS) {
-          mbar_wait_anyway_lane(&bias_full[g], cnt & 1u, abort_flag, args.status, kSoftmaxTimeout);
-          const BiasSlice* all = reinterpret_cast<const BiasSlice*>(smem + L::kBias) + g;
-          slice = &all->copy[0][(127 - r) & 3][(127 - r) & ~3];
-          is_flat = flat[g] != 0;
-          if (is_flat) shift = all->copy[0][0][0]; else scale = 1.0f;
-        }
         if (!idle) {
           const bool whole = __all_sync(0xffffffffu, !exists || (b_lo <= u0 && b_hi >= u0 + kKeys));
           uint32_t s[64];
@@ -676,21 +624,34 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           // scores of half CH: the bias added, masked keys out; the row's maximum
           auto fix = [&](auto half) {
             constexpr int B = decltype(half)::value * 32;
-            if (BIAS && !is_flat) {
+            if (BIAS) {
+              constexpr int H = decltype(half)::value;
+              const unsigned long long c2 = pack_f32x2(c, c);
+              auto put = [&](int i, float b0, float b1) {
+                float x0, x1;
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, pack_f32x2(b0, b1)), x0, x1);
+                s[i] = __float_as_uint(x0);
+                s[i + 1] = __float_as_uint(x1);
+              };
+              const float v0 = bias_log2(bias_v[H][0]), v1 = bias_log2(bias_v[H][1]);
+              if (bias_at[H] >= args.bias_n - 1 || bias_at[H] + 62 <= 0) {  // one value for all
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float* from = slice + (u0 + B + 16 * h < keys.ns ? 4 * kBiasPitch : 0);
+                for (int i = B; i < B + 32; i += 2) put(i, v0, v0);
+              } else {
+                BiasSlice* slice = reinterpret_cast<BiasSlice*>(own);
+                __syncwarp();
 #pragma unroll
-                for (int i = B + 16 * h; i < B + 16 * h + 16; i += 4) {
+                for (int k = 0; k < 4; ++k) {
+                  if (lane >= k) slice->copy[k][lane - k] = v0;
+                  slice->copy[k][32 + lane - k] = v1;
+                }
+                __syncwarp();
+                const float* from = &slice->copy[(31 - lane) & 3][(31 - lane) & ~3];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
                   const float4 b = *reinterpret_cast<const float4*>(from + i);
-                  const unsigned long long c2 = pack_f32x2(c, c);
-                  float x0, x1;
-                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, pack_f32x2(b.x, b.y)), x0, x1);
-                  s[i] = __float_as_uint(x0);
-                  s[i + 1] = __float_as_uint(x1);
-                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), c2, pack_f32x2(b.z, b.w)), x0, x1);
-                  s[i + 2] = __float_as_uint(x0);
-                  s[i + 3] = __float_as_uint(x1);
+                  put(B + i, b.x, b.y);
+                  put(B + i + 2, b.z, b.w);
                 }
               }
             }
@@ -711,11 +672,8 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           };
           fix(Int<0>());
           fix(Int<1>());
-          if (BIAS) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bias_empty[g]);
-          }
-          const float m_new = fmaxf(m_ref, fmaf(scale, fmaxf(mx0, mx1), shift));
+          const float scale = BIAS ? 1.0f : c;  // log2 units of what `s` holds
+          const float m_new = fmaxf(m_ref, scale * fmaxf(mx0, mx1));
           if (j == first) {
             m_ref = m_new;
           } else if (__any_sync(0xffffffffu, exists && m_new - m_ref > kLag)) {
@@ -732,7 +690,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             l_run *= f;
             m_ref = m_new;
           }
-          const float minus = shift - (m_ref == -INFINITY ? 0.f : m_ref);  // (a row that has seen nothing yet keeps its masked scores at 2^-inf)
+          const float minus = m_ref == -INFINITY ? 0.f : -m_ref;  // (a row that has seen nothing yet keeps its masked scores at 2^-inf)
           unsigned long long l0 = 0ull, l1 = 0ull;  // pairs of zeros
           // weights of half CH: fp16 pairs over the scores, fp32 sums
           auto weigh = [&](auto half) {
@@ -761,7 +719,6 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           unpack_f32x2(add_f32x2(l0, l1), la, lb);
           l_run += la + lb;
         }
-        if (BIAS && idle && lane == 0) mbar_arrive(&bias_empty[g]);
         const int valid = min(kKeys, keys.total - u0);
         if (valid < kKeys) {
           // blank the V rows behind the last key (as far as they are multiplied): they may be anybody's
@@ -817,7 +774,7 @@ cudaError_t launch_window(const CUtensorMap (&tm)[5], WindowArgs a, int sms, cud
   const long long grid = tiles * a.heads;
   if (grid > 0x7fffffffLL - 0x10000) return cudaErrorInvalidValue;
   a.take_over = grid > 2LL * sms ? 1 : 0;
-  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Layout<BIAS>::kBytes, stream, tm[0], tm[1], tm[2], tm[3],
+  return launch_pdl(kern, dim3(static_cast<unsigned>(grid)), dim3(kThreads), Layout::kBytes, stream, tm[0], tm[1], tm[2], tm[3],
                     tm[4], a);
 }
 
@@ -1157,9 +1114,9 @@ cudaError_t device_facts(DeviceFacts* f) {
     if (e != cudaSuccess) return e;
     n.status = device_status_word();
     if (n.status == nullptr) return cudaErrorUnknown;
-    e = cudaFuncSetAttribute(window_mha_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<false>::kBytes);
+    e = cudaFuncSetAttribute(window_mha_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout::kBytes);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(window_mha_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<true>::kBytes);
+      e = cudaFuncSetAttribute(window_mha_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout::kBytes);
     if (e != cudaSuccess) return e;
     known[dev] = n;
   }
