@@ -619,7 +619,8 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           tmem_ld_32x32_at<0>(t_s, s);
           tmem_ld_32x32_at<32>(t_s + 32, s);
           tmem_ld_wait();
-          float mx0 = -INFINITY, mx1 = -INFINITY;
+          float top = -INFINITY;              // largest score of the row, in log2 units
+          float scale[2] = {c, c}, shift[2] = {0.f, 0.f};  // of what `s` holds of either half, to log2 units
           unsigned some = 3u;  // halves of the tile of which any row of the warp sees a key
           // scores of half CH: the bias added, masked keys out; the row's maximum
           auto fix = [&](auto half) {
@@ -634,10 +635,12 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 s[i + 1] = __float_as_uint(x1);
               };
               const float v0 = bias_log2(bias_v[H][0]), v1 = bias_log2(bias_v[H][1]);
-              if (bias_at[H] >= args.bias_n - 1 || bias_at[H] + 62 <= 0) {  // one value for all
-#pragma unroll
-                for (int i = B; i < B + 32; i += 2) put(i, v0, v0);
+              if ((bias_at[H] >= args.bias_n - 1 || bias_at[H] + 62 <= 0) && (fabsf(v0) < 1e30f || v0 == -INFINITY)) {
+                // One value for all need not be added to each score (unless it is so large that the sum swallows the scores: then it
+                // has to, as where there are several)
+                shift[H] = v0;
               } else {
+                scale[H] = 1.0f;
                 BiasSlice* slice = reinterpret_cast<BiasSlice*>(own);
                 __syncwarp();
 #pragma unroll
@@ -664,16 +667,17 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
               for (int i = 0; i < 32; ++i) s[B + i] = ((w >> i) & 1u) ? s[B + i] : 0xff800000u;
             }
+            float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
             for (int i = B; i < B + 32; i += 4) {
               mx0 = max3(mx0, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
               mx1 = max3(mx1, __uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
             }
+            top = fmaxf(top, BIAS ? fmaf(scale[B / 32], fmaxf(mx0, mx1), shift[B / 32]) : c * fmaxf(mx0, mx1));
           };
           fix(Int<0>());
           fix(Int<1>());
-          const float scale = BIAS ? 1.0f : c;  // log2 units of what `s` holds
-          const float m_new = fmaxf(m_ref, scale * fmaxf(mx0, mx1));
+          const float m_new = fmaxf(m_ref, top);
           if (j == first) {
             m_ref = m_new;
           } else if (__any_sync(0xffffffffu, exists && m_new - m_ref > kLag)) {
@@ -697,7 +701,8 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             constexpr int B = decltype(half)::value * 32;
             uint32_t pk[16];
             if (some & (1u << (B / 32))) {
-              const unsigned long long sc2 = pack_f32x2(scale, scale), mi2 = pack_f32x2(minus, minus);
+              const float mul = BIAS ? scale[B / 32] : c, add = BIAS ? shift[B / 32] + minus : minus;
+              const unsigned long long sc2 = pack_f32x2(mul, mul), mi2 = pack_f32x2(add, add);
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 float t0, t1;
