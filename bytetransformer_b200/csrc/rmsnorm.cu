@@ -7,6 +7,8 @@
 //
 // s also leaves as fp16 where the caller wants it (the next residual); the statistics are those of the fp32 sum, not of
 // its rounded copy.  HBM bound: every byte is read and written once, a row lives in registers between the two.
+// Measured on B200 (of the copy's 6.45 TB/s): 75776 x 768 fp16 69.9 us (1.03), 18645 x 1024 fp32 -> e4m3 with a scale per 128
+// columns 27.9 us (0.96), 4000 x 16384 fp32 -> fp16 98.3 us (1.03); 48 x 768 2.15 us, a launch.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -197,6 +199,8 @@ cudaError_t launch_one(const RmsArgs& a, cudaStream_t stream) {
 
 template <bool X_FP32, bool G_FP32, int OUT>
 cudaError_t launch_by_width(const RmsArgs& a, cudaStream_t stream) {
+  // A warp to a row as far as four vectors to a lane go; beyond, as many warps as leave two to four.  Rows of more than 8192 keep two
+  // CTAs to an SM by registers (one: 4000 x 16384 fp32 107.9 us instead of 98.3).
   const int nvec = a.hidden / 8;
   if (nvec <= 32) return launch_one<X_FP32, G_FP32, OUT, 1, 1>(a, stream);
   if (nvec <= 64) return launch_one<X_FP32, G_FP32, OUT, 1, 2>(a, stream);

@@ -11,7 +11,8 @@ algorithmic bytes (or flops) per launch, achieved GB/s (TFLOP/s) and the fractio
 Cases and their reference counterparts: offsets (remove_padding.h:36-101), pack / restore
 (remove_padding.h:104-121, layernorm.h:430-446), layernorm / layernorm_restore (layernorm.h:410-446),
 gelu (gemm_bias_act.cu:32-66), softmax (softmax.h:191-297), embedding (layernorm.h:219-240), pooler,
-mha_s64 / mha_s256 (attention_fused.cu:295-414, attention_fused_long.cu:171-312).
+mha_s64 / mha_s256 (attention_fused.cu:295-414, attention_fused_long.cu:171-312); without a counterpart there: relative_bias /
+relative_bias_grad, rmsnorm / rmsnorm_e4m3, window / window_token.
 """
 from __future__ import annotations
 
@@ -24,7 +25,7 @@ import numpy as np
 import torch
 
 ALL_CASES = ["offsets", "pack", "restore", "layernorm", "layernorm_restore", "gelu", "softmax", "embedding", "pooler",
-             "mha_s64", "mha_s256"]
+             "mha_s64", "mha_s256", "relative_bias", "relative_bias_grad", "rmsnorm", "rmsnorm_e4m3", "window", "window_token"]
 
 
 def _peaks():
@@ -186,6 +187,43 @@ def main():
             print("device status non-zero", file=sys.stderr)
             return 1
     return 0
+
+    if "relative_bias" in cases:
+        table = torch.randn(32, 16, generator=g).half().to(dev)
+        us = _time(lambda: E.relative_position_bias(table, 2048, 2048), args.iters, args.warmup)
+        report("relative_bias", "relative_bias_kernel", us, 2 * 16 * 2048 * 2048, note="16 heads, 2048 x 2048 fp16 (the wrapper allocates the output)")
+    if "relative_bias_grad" in cases:
+        grad = torch.randn(8, 16, 1024, 1024, dtype=torch.float16, device=dev)
+        us = _time(lambda: E.relative_position_bias_grad(grad, 32), args.iters, args.warmup)
+        report("relative_bias_grad", "relative_bias_grad_kernel + join", us, 2 * grad.numel(), note="8 sequences, 16 heads, 1024 x 1024 fp16")
+        del grad
+    if "rmsnorm" in cases or "rmsnorm_e4m3" in cases:
+        x, r = (torch.randn(M, H, dtype=torch.float16, device=dev) for _ in range(2))
+        gamma = torch.ones(H).half().to(dev)
+        if "rmsnorm" in cases:
+            us = _time(lambda: E.add_residual_rmsnorm(x, r, gamma), args.iters, args.warmup)
+            report("rmsnorm", "add_residual_rmsnorm_kernel", us, 8 * M * H, note=f"rows={M} H={H}, x and residual in, sum and fp16 norm out")
+        if "rmsnorm_e4m3" in cases:
+            us = _time(lambda: E.add_residual_rmsnorm_e4m3(x, r, gamma, group=128), args.iters, args.warmup)
+            report("rmsnorm_e4m3", "add_residual_rmsnorm_kernel", us, 7 * M * H + 4 * M * (H // 128),
+                   note=f"rows={M} H={H}, x and residual in, sum, e4m3 norm and a scale per 128 columns out")
+        del x, r
+    if "window" in cases:
+        Lw, left = 16384, 511
+        qkv = torch.randn(Lw, 3 * nh * 64, dtype=torch.float16, device=dev)
+        q, k, v = qkv.split([nh * 64] * 3, dim=1)
+        off = torch.tensor([0, Lw], dtype=torch.int32, device=dev)
+        us = _time(lambda: E.window_attention(q, k, v, off, off, Lw, Lw, left=left, right=0, sinks=4), args.iters, args.warmup)
+        pairs = sum(min(p, left) + 1 + min(4, max(0, p - left)) for p in range(Lw))
+        report("window", "window_mha_kernel", us, flops=4.0 * 64 * nh * pairs, note=f"one sequence of {Lw}, {left} keys back, 4 first ones, {nh} heads")
+        del qkv, q, k, v
+    if "window_token" in cases:
+        Bt, Lt = 64, 4096
+        cache = torch.randn(Bt * Lt, 2 * 4 * 64, dtype=torch.float16, device=dev)
+        q = torch.randn(Bt, 16 * 64, dtype=torch.float16, device=dev)
+        off = torch.arange(Bt + 1, dtype=torch.int32, device=dev)
+        us = _time(lambda: E.window_attention(q, cache[:, :256], cache[:, 256:], off, off * Lt, 1, Lt), args.iters, args.warmup)
+        report("window_token", "window_few_kernel + join", us, 2 * cache.numel(), note=f"one token for each of {Bt} sequences of {Lt} keys, 16 heads over 4")
 
 
 if __name__ == "__main__":
