@@ -180,14 +180,6 @@ def main():
                    args.iters, args.warmup)
         report(case, "attention (kernel chosen by shape)", us, nbytes=8 * Tm * H, flops=4.0 * H * sum(l * l for l in lens_m),
                note=f"16 sequences up to {L} tokens, T={Tm}: latency-bound (a few hundred items)")
-    if enc is not None:
-        st_word = enc.device_status()
-        enc.close()
-        if st_word != 0:
-            print("device status non-zero", file=sys.stderr)
-            return 1
-    return 0
-
     if "relative_bias" in cases:
         table = torch.randn(32, 16, generator=g).half().to(dev)
         us = _time(lambda: E.relative_position_bias(table, 2048, 2048), args.iters, args.warmup)
@@ -224,6 +216,13 @@ def main():
         off = torch.arange(Bt + 1, dtype=torch.int32, device=dev)
         us = _time(lambda: E.window_attention(q, cache[:, :256], cache[:, 256:], off, off * Lt, 1, Lt), args.iters, args.warmup)
         report("window_token", "window_few_kernel + join", us, 2 * cache.numel(), note=f"one token for each of {Bt} sequences of {Lt} keys, 16 heads over 4")
+    if enc is not None:
+        st_word = enc.device_status()
+        enc.close()
+        if st_word != 0:
+            print("device status non-zero", file=sys.stderr)
+            return 1
+    return 0
 
 
 if __name__ == "__main__":
