@@ -244,12 +244,11 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   return below_hi & ~below_lo;
 }
 
-// The bias of half a tile for a warp's rows: value of (column c, lane l) at c - l + 31, in log2 units.  Four copies, each an
-// element further on, so that a lane reads its row's values four at a time wherever they start; the pitch keeps the copies
+// The bias of a tile for a warp's rows: value of (column c of half h, lane l) at 64 h + c - l + 31, in log2 units.  Two copies, one an
+// element further on, so that a lane reads its row's values two at a time wherever they start; the pitch keeps the copies
 // that neighbouring lanes read in different banks.
-constexpr int kBiasPitch = 72;
 struct BiasSlice {
-  float copy[4][kBiasPitch];
+  float copy[2][144];
 };
 
 struct Layout {
@@ -257,7 +256,7 @@ struct Layout {
   static constexpr int kQ = 0;
   static constexpr int kK = kQ + kStages * kQTile;
   static constexpr int kV = kK + 2 * kStages * kKvTile;
-  // For each of the eight warps: the bias of the half tile that it is at, then its reference and sums for the other group; or
+  // For each of the eight warps: the bias of the tile that it is at, then its reference and sums for the other group; or
   // 32 output rows of 64 bytes
   static constexpr int kOwn = kV + 2 * kStages * kKvTile;
   static constexpr int kOwnBytes = 32 * 64;
@@ -601,19 +600,29 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       for (int j = first; j < keys.tiles; j += 2, ++cnt) {
         const int u0 = j * kKeys;
         const int slot = g * kStages + static_cast<int>(cnt % kStages);
-        // The bias of a half: of (column 0, lane 31) at index bias_at; 63 values from there on, two to a lane, on the way while S is
-        // waited for.
-        int bias_at[2];
-        float bias_v[2][2];
-        if (BIAS) {
+        // The bias, laid out while S is on its way: of a half, 63 values from that of (column 0, lane 31) on, at index `at`
+        float one[2] = {0.f, 0.f};        // a half's bias where it is one for all its keys and rows
+        bool several[2] = {false, false};
+        if (BIAS && !idle) {
           const float* table = args.bias + static_cast<long long>(it.head) * args.bias_n;
+          BiasSlice* slice = reinterpret_cast<BiasSlice*>(own);
+          __syncwarp();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int u = u0 + 32 * h;
-            bias_at[h] = (u < keys.ns ? u : keys.ws + u - keys.ns) - (it.p0 + quarter * 32 + 31) + args.bias_left;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) bias_v[h][i] = __ldg(table + min(max(bias_at[h] + 32 * i + lane, 0), args.bias_n - 1));
+            const int at = (u < keys.ns ? u : keys.ws + u - keys.ns) - (it.p0 + quarter * 32 + 31) + args.bias_left;
+            const float v0 = bias_log2(__ldg(table + min(max(at + lane, 0), args.bias_n - 1)));
+            const float v1 = bias_log2(__ldg(table + min(max(at + 32 + lane, 0), args.bias_n - 1)));
+            one[h] = v0;
+            // One value for all need not be added to each score (unless it is so large that the sum swallows the scores: then it has
+            // to, as where there are several)
+            several[h] = !((at >= args.bias_n - 1 || at + 62 <= 0) && (fabsf(v0) < 1e30f || v0 == -INFINITY));
+            slice->copy[0][64 * h + lane] = v0;
+            slice->copy[0][64 * h + 32 + lane] = v1;
+            if (lane > 0) slice->copy[1][64 * h + lane - 1] = v0;
+            slice->copy[1][64 * h + 31 + lane] = v1;
           }
+          __syncwarp();
         }
         mbar_wait_anyway_lane(&s_full[g], cnt & 1u, abort_flag, args.status, kSoftmaxTimeout);
         tc_fence_after();
@@ -631,35 +640,20 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             constexpr int B = decltype(half)::value * 32;
             if (BIAS) {
               constexpr int H = decltype(half)::value;
-              const unsigned long long c2 = pack_f32x2(c, c);
-              auto put = [&](int i, float b0, float b1) {
-                float x0, x1;
-                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, pack_f32x2(b0, b1)), x0, x1);
-                s[i] = __float_as_uint(x0);
-                s[i + 1] = __float_as_uint(x1);
-              };
-              const float v0 = bias_log2(bias_v[H][0]), v1 = bias_log2(bias_v[H][1]);
-              if ((bias_at[H] >= args.bias_n - 1 || bias_at[H] + 62 <= 0) && (fabsf(v0) < 1e30f || v0 == -INFINITY)) {
-                // One value for all need not be added to each score (unless it is so large that the sum swallows the scores: then it
-                // has to, as where there are several)
-                shift[H] = v0;
-              } else {
+              if (several[H]) {
                 scale[H] = 1.0f;
-                BiasSlice* slice = reinterpret_cast<BiasSlice*>(own);
-                __syncwarp();
+                const unsigned long long c2 = pack_f32x2(c, c);
+                const float* from = &reinterpret_cast<const BiasSlice*>(own)->copy[(31 - lane) & 1][64 * H + ((31 - lane) & ~1)];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  if (lane >= k) slice->copy[k][lane - k] = v0;
-                  slice->copy[k][32 + lane - k] = v1;
+                for (int i = 0; i < 32; i += 2) {
+                  const float2 b = *reinterpret_cast<const float2*>(from + i);
+                  float x0, x1;
+                  unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[B + i]), __uint_as_float(s[B + i + 1])), c2, pack_f32x2(b.x, b.y)), x0, x1);
+                  s[B + i] = __float_as_uint(x0);
+                  s[B + i + 1] = __float_as_uint(x1);
                 }
-                __syncwarp();
-                const float* from = &slice->copy[(31 - lane) & 3][(31 - lane) & ~3];
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                  const float4 b = *reinterpret_cast<const float4*>(from + i);
-                  put(B + i, b.x, b.y);
-                  put(B + i + 2, b.z, b.w);
-                }
+              } else {
+                shift[H] = one[H];
               }
             }
             if (!whole) {
