@@ -11,6 +11,7 @@ extended to a stack of layers.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import List, Optional, Sequence
 
 import torch
@@ -505,14 +506,17 @@ def masked_softmax_(logits, attr_mask, scale=1.0):
     return logits
 
 
+_FP32 = {torch.float16: 0, torch.float32: 1}
+
+
 def _half_or_float(t: torch.Tensor, name: str, device=None) -> int:
     """1 for fp32, 0 for fp16; anything else is refused.  `device`: where the call's other tensors are."""
     _check(t, name)
-    if t.dtype not in (torch.float16, torch.float32):
+    if t.dtype not in _FP32:
         raise RuntimeError(f"{name} must be fp16 or fp32")
     if device is not None and t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, the other tensors are on {device}")
-    return int(t.dtype == torch.float32)
+    return _FP32[t.dtype]
 
 
 def _check_distances(q_len, k_len, max_distance, q_start):
@@ -547,6 +551,15 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_d
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _bias_grad_workspace(fp32: int, num_buckets: int, batch: int, heads: int, q_len: int, k_len: int) -> int:
+    n = C.c_size_t()
+    rc = _abi.load().bt_relative_position_bias_grad_workspace(fp32, num_buckets, batch, heads, q_len, k_len, C.byref(n))
+    if rc != _abi.BT_OK:
+        raise _abi.BtError(rc, "bt_relative_position_bias_grad_workspace")
+    return n.value
+
+
 def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_distance: int = 128,
                                 bidirectional: bool = True, q_start: int = 0) -> torch.Tensor:
     """The gradient of relative_position_bias: [num_buckets, heads] fp32 from that of the bias, [heads, q, k], or of the
@@ -560,16 +573,13 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
     if grad.numel() == 0:
         return torch.zeros(num_buckets, heads, dtype=torch.float32, device=grad.device)
     lib = _abi.load()
+    n = _bias_grad_workspace(fp32, int(num_buckets), batch, heads, q_len, k_len)
     with _On(grad.device) as stream:
-        n = C.c_size_t()
-        rc = lib.bt_relative_position_bias_grad_workspace(fp32, int(num_buckets), batch, heads, q_len, k_len, C.byref(n))
-        if rc != _abi.BT_OK:
-            raise _abi.BtError(rc, "bt_relative_position_bias_grad_workspace")
         out = torch.empty(num_buckets, heads, dtype=torch.float32, device=grad.device)
-        ws = torch.empty(n.value, dtype=torch.int8, device=grad.device)
+        ws = torch.empty(n, dtype=torch.int8, device=grad.device)
         rc = lib.bt_relative_position_bias_grad(grad.data_ptr(), fp32, int(num_buckets), int(max_distance),
                                                 int(bool(bidirectional)), batch, heads, q_len, k_len, int(q_start),
-                                                out.data_ptr(), ws.data_ptr(), n.value, stream)
+                                                out.data_ptr(), ws.data_ptr(), n, stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_relative_position_bias_grad")
     return out
@@ -577,6 +587,12 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
 
 def _rmsnorm_args(x, residual, gamma, m_dev):
     """(x is fp32, gamma is fp32) of a norm's arguments, which are refused here if they do not fit together."""
+    device, shape = x.device, x.shape
+    if (m_dev is None and x.is_cuda and x.is_contiguous() and len(shape) == 2 and gamma.shape == shape[1:] and
+            gamma.device == device and gamma.is_contiguous() and x.dtype in _FP32 and gamma.dtype in _FP32 and
+            (residual is None or (residual.dtype == torch.float16 and residual.shape == shape and
+                                  residual.device == device and residual.is_contiguous()))):
+        return _FP32[x.dtype], _FP32[gamma.dtype]  # (the usual call; what follows finds out what is wrong, or takes m_dev)
     x_fp32 = _half_or_float(x, "x")
     gamma_fp32 = _half_or_float(gamma, "gamma", x.device)
     if x.dim() != 2 or gamma.dim() != 1 or gamma.shape[0] != x.shape[1]:
@@ -658,6 +674,14 @@ def _ints(t: torch.Tensor, name: str, device) -> int:
     return t.shape[0]
 
 
+@functools.lru_cache(maxsize=256)
+def _window_workspace(batch: int, heads: int, kv_heads: int, max_q_len: int, max_k_len: int, left: int, sinks: int) -> int:
+    """Bytes, or 0 where the arguments are such that the call itself will refuse them."""
+    n = C.c_size_t()
+    rc = _abi.load().bt_window_attention_workspace(batch, heads, kv_heads, max_q_len, max_k_len, left, sinks, C.byref(n))
+    return n.value if rc == _abi.BT_OK else 0
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor, k_offsets: torch.Tensor,
                      max_q_len: int, max_k_len: int, *, left: int = -1, right: int = -1, sinks: int = 0,
                      k_lens: Optional[torch.Tensor] = None, distance_bias: Optional[torch.Tensor] = None,
@@ -671,8 +695,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     device = q.device
     heads, kv_heads = _rows(q, "q", device), _rows(k, "k", device)
     rows, k_rows = q.shape[0], k.shape[0]
-    if _rows(v, "v", device) != kv_heads or v.shape[0] != k_rows:
+    if v.shape != k.shape:
         raise RuntimeError("k and v must have the same shape")
+    _rows(v, "v", device)
     batch = _ints(q_offsets, "q_offsets", device) - 1
     if _ints(k_offsets, "k_offsets", device) != batch + 1 or batch < 0:
         raise RuntimeError("q_offsets and k_offsets must have batch + 1 elements")
@@ -702,10 +727,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
             return out
         ws, n = None, 0
         if max_q_len * heads <= 16 * kv_heads:  # few queries: the keys may be cut into ranges
-            size = C.c_size_t()
-            if lib.bt_window_attention_workspace(batch, heads, kv_heads, max_q_len, max_k_len, left, sinks,
-                                                 C.byref(size)) == _abi.BT_OK and size.value:
-                n = size.value
+            n = _window_workspace(batch, heads, kv_heads, max_q_len, max_k_len, left, sinks)
+            if n:
                 ws = torch.empty(n, dtype=torch.int8, device=device)
         a = _abi.bt_window_attention_args(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
