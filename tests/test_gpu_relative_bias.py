@@ -135,6 +135,27 @@ def test_infinite_gradients_stay_in_their_bucket(cuda_device):
     assert (got[keep] == 0).all()
 
 
+def test_past_32_bits(cuda_device):
+    """More than 2^31 elements, rows that start at every alignment, the last ones looked at."""
+    from bytetransformer_b200 import encoder as E
+    heads, q, k = 3, 27_001, 27_003
+    table = torch.randn(32, heads, device=cuda_device, dtype=torch.float16)
+    bias = E.relative_position_bias(table, q, k)
+    for rows in (slice(0, 3), slice(q - 70, q)):
+        n = rows.stop - rows.start
+        part = E.relative_position_bias(table, n, k, q_start=rows.start)
+        assert torch.equal(bias[:, rows], part)
+    ids, at = by_distance(70, k, q - 70, 32, 128, True)
+    assert torch.equal(bias[2, q - 70:].cpu(), table[:, 2].cpu()[ids][at])
+    bias.fill_(1.0)  # as a gradient: the buckets' sizes
+    got = E.relative_position_bias_grad(bias, 32).cpu().double()
+    d = torch.arange(-(q - 1), k)
+    many = torch.minimum(torch.minimum(d + q, k - d), torch.tensor(min(q, k))).double()
+    member = torch.tensor([bucket(max(-200, min(200, int(x))), 32, 128, True) for x in d.tolist()])
+    want = torch.zeros(32, dtype=torch.float64).index_add_(0, member, many)[:, None].expand(32, heads)
+    assert ((got - want).abs() <= ROUNDINGS * 2.0 ** -24 * want).all()
+
+
 def test_another_stream_a_captured_graph_and_empty_calls(cuda_device):
     from bytetransformer_b200 import encoder as E
     table = torch.randn(32, 12, device=cuda_device, dtype=torch.float16)

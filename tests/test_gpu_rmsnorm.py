@@ -71,6 +71,21 @@ def test_many_rows(cuda_device):
     check_half(E.add_residual_rmsnorm(x, r, gamma)[0], y)
 
 
+def test_past_32_bits(cuda_device):
+    from bytetransformer_b200 import encoder as E
+    rows, hidden = 270_000, 8192  # 2.2e9 elements
+    x = torch.ones(rows, hidden, dtype=torch.float16, device=cuda_device)
+    x[-5:] = torch.randn(5, hidden, device=cuda_device).half()
+    gamma = torch.ones(hidden, dtype=torch.float16, device=cuda_device)
+    s, y = definition(x[-5:], x[-5:], gamma, 1e-6)
+    out, total = E.add_residual_rmsnorm(x, x, gamma)
+    check_half(out[-5:], y)
+    assert (out[:-5] == 1).all() and (total[:-5] == 2).all() and torch.equal(total[-5:], x[-5:] * 2)
+    del out, total
+    q, scales, _ = E.add_residual_rmsnorm_e4m3(x, None, gamma, group=128)
+    check_e4m3(q[-5:], scales[-5:], y, 128)
+
+
 def test_rows_of_zeros_and_tiny_rows(cuda_device):
     from bytetransformer_b200 import encoder as E
     x = torch.zeros(3, 256, dtype=torch.float16, device=cuda_device)

@@ -180,6 +180,20 @@ def test_single_tokens_of_many_sequences(cuda_device):
     check(q, kv[:, :D], kv[:, D:], q_off, k_off, 1, 300, None, 200, 0, 4)
 
 
+@pytest.mark.parametrize("q_len", [1, 200])
+def test_a_cache_past_32_bits(cuda_device, q_len):
+    """Rows whose place is more than 2^32 halves from the first."""
+    rows, heads, kv = 9_000_000, 4, 4
+    cache = torch.empty(rows, 2 * kv * D, dtype=torch.float16, device=cuda_device)
+    lens, starts = [300, 257, 900], [0, 4_500_000, 8_999_000]
+    for n, at in zip(lens, starts):
+        cache[at:at + n] = torch.randn(n, 2 * kv * D, device=cuda_device).half()
+    q = torch.randn(3 * q_len, heads * D, device=cuda_device).half()
+    q_off = torch.arange(4, dtype=torch.int32, device=cuda_device) * q_len
+    k_off = torch.tensor(starts + [rows], dtype=torch.int32, device=cuda_device)
+    check(q, cache[:, :kv * D], cache[:, kv * D:], q_off, k_off, q_len, rows, torch.tensor(lens).int().to(cuda_device), 150, 0, 4)
+
+
 def test_large_scores(cuda_device):
     """References that move in every tile, weights that all but one vanish."""
     q, k, v, off = packed([900, 130], 2, 2, cuda_device, seed=5)
