@@ -793,12 +793,14 @@ cudaError_t launch_window(const CUtensorMap (&tm)[5], WindowArgs a, int sms, cud
 constexpr int kFewRows = 16;
 constexpr int kFewWarps = 4;
 constexpr int kFewKeys = 32;  // of a step
+constexpr int kFewCluster = 8;  // ranges that a cluster holds
 
 struct FewArgs {
   WindowArgs w;
   const __half *q, *k, *v;
   long long q_stride, k_stride, v_stride;
   int splits;
+  int cluster;  // the ranges of an item are a cluster, which puts them together itself; else they are left in `partial_*`
   float* partial_o;  // [batch, kv_heads, splits, 16, 64]
   float2* partial_ml;  // [batch, kv_heads, splits, 16]: reference and sum
 };
@@ -809,6 +811,37 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint4 load16(const __half* p) { return *reinterpret_cast<const uint4*>(p); }
+// Every thread of every CTA of the cluster: what was written to shared memory before is visible to all after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 16 (8) bytes at the place of `p` in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ float4 load_of(const float* p, int rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t"
+      ".reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t"
+      "}\n"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(smem_u32(p)), "r"(rank)
+      : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 load_of(const float2* p, int rank) {
+  float2 v;
+  asm volatile(
+      "{\n\t"
+      ".reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %2, %3;\n\t"
+      "ld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t"
+      "}\n"
+      : "=f"(v.x), "=f"(v.y)
+      : "r"(smem_u32(p)), "r"(rank)
+      : "memory");
+  return v;
+}
 
 // The sequence of a CTA: rows of its queries, position of the first, its keys.  false: nothing to do.
 __device__ __forceinline__ bool few_item(const WindowArgs& a, int b, Item& it) {
@@ -830,8 +863,8 @@ __device__ __forceinline__ bool few_item(const WindowArgs& a, int b, Item& it) {
 
 template <bool BIAS>
 __global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __grid_constant__ FewArgs a) {
-  __shared__ float o_all[kFewWarps][kFewRows][kHeadDim + 4];
-  __shared__ float2 ml_all[kFewWarps][kFewRows];
+  __shared__ __align__(16) float o_all[kFewWarps][kFewRows][kHeadDim + 4];
+  __shared__ float2 ml_all[kFewWarps][kFewRows], ml_cta[kFewRows];
   pdl_launch_dependents();
   const WindowArgs& w = a.w;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -990,22 +1023,54 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __g
   __syncthreads();
   // eight columns of a row to a thread
   const int r = threadIdx.x >> 3, col = (threadIdx.x & 7) * 8;
-  if (r >= rows) return;
   float top = -INFINITY, sum = 0.f, acc[8];
 #pragma unroll
-  for (int i = 0; i < kFewWarps; ++i) top = fmaxf(top, ml_all[i][r].x);
-#pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+  if (r < rows) {
 #pragma unroll
-  for (int i = 0; i < kFewWarps; ++i) {
-    const float2 ml = ml_all[i][r];
-    if (ml.x == -INFINITY) continue;  // this warp has seen no key of the row
-    const float f = ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
+    for (int i = 0; i < kFewWarps; ++i) top = fmaxf(top, ml_all[i][r].x);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) acc[x] = fmaf(o_all[i][r][col + x], f, acc[x]);
+    for (int i = 0; i < kFewWarps; ++i) {
+      const float2 ml = ml_all[i][r];
+      if (ml.x == -INFINITY) continue;  // this warp has seen no key of the row
+      const float f = ex2(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc[x] = fmaf(o_all[i][r][col + x], f, acc[x]);
+    }
   }
-  if (a.splits == 1) {
+  bool write = r < rows;
+  if (a.cluster) {
+    // each CTA's result in its shared memory; the rows go round the CTAs, a row's reads all of them
+    float* mine = &o_all[0][r][col];  // (read by this thread alone)
+#pragma unroll
+    for (int x = 0; x < 8; ++x) mine[x] = acc[x];
+    if (col == 0) ml_cta[r] = make_float2(top, sum);
+    __syncwarp();
+    cluster_sync();
+    write = write && r % a.splits == split;
+    if (write) {
+      top = -INFINITY;
+      for (int i = 0; i < a.splits; ++i) top = fmaxf(top, load_of(&ml_cta[r], i).x);
+      sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+      for (int i = 0; i < a.splits; ++i) {
+        const float2 ml = load_of(&ml_cta[r], i);
+        const float4 o0 = load_of(mine, i), o1 = load_of(mine + 4, i);
+        if (ml.x == -INFINITY) continue;
+        const float f = ex2(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
+#pragma unroll
+        for (int x = 0; x < 8; ++x) acc[x] = fmaf(o[x], f, acc[x]);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // nobody's shared memory goes away while another reads it
+  }
+  if (!write) return;
+  if (a.splits == 1 || a.cluster) {
     const float inv = 1.0f / sum;
     uint4 out = make_uint4(0u, 0u, 0u, 0u);
     if (sum != 0.f)
@@ -1062,36 +1127,64 @@ __global__ void __launch_bounds__(256) window_few_join_kernel(const __grid_const
                             4 * x) = out;
 }
 
-// Whether a call takes the kernel for few queries, and into how many ranges it cuts a sequence's keys (0: the other kernel).
+// How a call of few queries is cut: ranges of a sequence's keys (0: the call is not one of few queries), and whether the ranges of
+// an item are a cluster of CTAs, which put their results together through each other's shared memory, or leave them to a second
+// kernel.
+struct FewSplit {
+  int ranges = 0;
+  bool cluster = false;
+};
 // 444 CTAs are resident (three to an SM).  A CTA's time goes with its keys and something like 200 more (its first loads wait for
 // one another, its results are put together), so of the numbers of ranges that leave a range 128 keys the one with the
 // shortest sum over the waves is taken.  us per call, 64 sequences of 4100 keys, 16 heads over 4, by ranges:
 // 1 66, 2 68, 3 56, 6 61; 8 of 4096, 12 heads, 4 ranges (one wave) 23.9, 5 31.6, 7 29.5; 2 of 30000, 12 heads, 18 38.0, 24 46.9.
-int few_splits(int batch, int kv_heads, int group, int max_q, int max_k, int left, int sinks) {
-  if (static_cast<long long>(max_q) * group > kFewRows || batch > 65535 || kv_heads > 65535) return 0;
-  constexpr long long kResident = 3 * 148, kOverhead = 200;
+// Clusters save the second kernel, but their CTAs come and go together: where all are resident at once 16 sequences of 1027
+// keys, one key/value head 7.2 us (second kernel: 7.8), 4 of 700, 2 heads 6.4 (7.5); where they are not, the 64 sequences of 4100
+// keys above 71 (55).
+FewSplit few_split(int batch, int kv_heads, int group, int max_q, int max_k, int left, int sinks) {
+  FewSplit f;
+  if (static_cast<long long>(max_q) * group > kFewRows || batch > 65535 || kv_heads > 65535) return f;
+  constexpr long long kResident = 3 * 148, kOverhead = 200, kTogether = 400;
   long long keys = max_k;
   if (left >= 0) keys = static_cast<long long>(left) + max_q + sinks + kSeam < keys ? static_cast<long long>(left) + max_q + sinks + kSeam : keys;
   const long long items = static_cast<long long>(batch) * kv_heads;
-  int best = 1;
-  long long best_cost = 0x7fffffffffffffffLL;
+  long long best = 0x7fffffffffffffffLL;
   for (int s = 1; s <= 148 && (s == 1 || s * 128LL <= keys); ++s) {
     const long long cost = (items * s + kResident - 1) / kResident * (keys / s + kOverhead);
-    if (cost < best_cost) {
-      best = s;
-      best_cost = cost;
+    if (cost < best) {
+      f.ranges = s;
+      best = cost;
     }
   }
-  return best;
+  f.cluster = f.ranges > 1 && f.ranges <= kFewCluster && items * f.ranges <= kTogether;
+  return f;
 }
-size_t few_workspace(long long items, int splits) {
-  return splits <= 1 ? 0 : static_cast<size_t>(items) * splits * kFewRows * (kHeadDim * 4 + 8);
+size_t few_workspace(long long items, FewSplit f) {
+  return f.ranges <= 1 || f.cluster ? 0 : static_cast<size_t>(items) * f.ranges * kFewRows * (kHeadDim * 4 + 8);
 }
 
 template <bool BIAS>
 cudaError_t launch_few(const FewArgs& a, int kv_heads, cudaStream_t stream) {
-  cudaError_t e = launch_pdl(window_few_kernel<BIAS>, dim3(a.splits, kv_heads, a.w.batch), dim3(kFewWarps * 32), 0, stream, a);
-  if (e == cudaSuccess && a.splits > 1) e = launch_pdl(window_few_join_kernel, dim3(a.w.max_q * a.w.group, kv_heads, a.w.batch), dim3(256), 0, stream, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.splits, kv_heads, a.w.batch);
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  if (pdl_take_attr()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.splits;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, window_few_kernel<BIAS>, a);
+  if (e == cudaSuccess && a.splits > 1 && !a.cluster) e = launch_pdl(window_few_join_kernel, dim3(a.w.max_q * a.w.group, kv_heads, a.w.batch), dim3(256), 0, stream, a);
   return e;
 }
 
@@ -1143,7 +1236,7 @@ extern "C" int bt_window_attention_workspace(int batch, int head_num, int kv_hea
       max_q_len > kMaxLength || max_k_len < 0 || max_k_len > kMaxLength || sinks < 0)
     return BT_ERR_INVALID_ARG;
   *bytes = few_workspace(static_cast<long long>(batch) * kv_head_num,
-                         few_splits(batch, kv_head_num, head_num / kv_head_num, max_q_len, max_k_len, left, sinks));
+                         few_split(batch, kv_head_num, head_num / kv_head_num, max_q_len, max_k_len, left, sinks));
   return BT_OK;
 }
 
@@ -1189,14 +1282,16 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
   w.status = dev.status;
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
   cudaError_t e;
-  const int splits = few_splits(a->batch, a->kv_head_num, w.group, a->max_q_len, a->max_k_len, a->left, a->sinks);
-  if (splits > 0) {
+  const FewSplit split = few_split(a->batch, a->kv_head_num, w.group, a->max_q_len, a->max_k_len, a->left, a->sinks);
+  if (split.ranges > 0) {
+    const int splits = split.ranges;
     const long long items = static_cast<long long>(a->batch) * a->kv_head_num;
-    const size_t need = few_workspace(items, splits);
+    const size_t need = few_workspace(items, split);
     if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return BT_ERR_WORKSPACE;
     if (!aligned(a->workspace, 16)) return BT_ERR_INVALID_ARG;
     FewArgs f{w, static_cast<const __half*>(a->q), static_cast<const __half*>(a->k), static_cast<const __half*>(a->v),
-              a->q_row_stride, a->k_row_stride, a->v_row_stride, splits, static_cast<float*>(a->workspace), nullptr};
+              a->q_row_stride, a->k_row_stride, a->v_row_stride, splits, split.cluster ? 1 : 0,
+              static_cast<float*>(a->workspace), nullptr};
     f.partial_ml = reinterpret_cast<float2*>(f.partial_o + items * splits * kFewRows * kHeadDim);
     e = w.bias != nullptr ? launch_few<true>(f, a->kv_head_num, stream) : launch_few<false>(f, a->kv_head_num, stream);
     return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;
