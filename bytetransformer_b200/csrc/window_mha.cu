@@ -785,20 +785,23 @@ cudaError_t launch_window(const CUtensorMap (&tm)[5], WindowArgs a, int sms, cud
 // The queries of a sequence times the heads that share a key/value head are at most 16 rows: what a step of generation
 // asks for.  The keys are read once and that is the time it takes, so a CTA belongs to a (sequence, key/value head, range of
 // its virtual keys) and all rows that need them; each of its four warps walks every fourth 32 keys with a softmax of its
-// own, on mma.sync (16 x 8 x 16: a tcgen05 tile would be one eighth full at best, and its operands would pass through shared
-// memory).  K and V go from global memory straight into the operands' registers: the order of the 64 dimensions in q.k and of
-// the output columns in p.v is free, and is chosen so that a thread's registers are 16 contiguous bytes of a row.
-// The next keys are requested as soon as a product has taken the last ones.  Bound by HBM and its latency: 32 sequences of 8192
-// keys, 32 heads over 8, 96 us (5.6 TB/s); 64 of 4100 keys, 16 heads over 4, 55 us (4.6 TB/s).
+// own, on mma.sync (16 x 8 x 16: a tcgen05 tile would be one eighth full at best).  A warp has a ring of its own of 32 keys and
+// values, fetched by TMA a few steps ahead; no warp waits for another before the range ends.
 constexpr int kFewRows = 16;
 constexpr int kFewWarps = 4;
 constexpr int kFewKeys = 32;  // of a step
 constexpr int kFewCluster = 8;  // ranges that a cluster holds
+constexpr int kFewStages = 3;   // of a warp's ring
+constexpr int kFewCtas = 2;     // to an SM
+constexpr int kFewTile = kFewKeys * kHeadDim * 2;  // 4 KiB of K, and of V
+constexpr int kFewRing = kFewStages * 2 * kFewTile;
+constexpr int kFewSmemBytes = kFewWarps * kFewRing;
+static_assert(kFewKeys == kSeam, "a step's keys are neighbours, also at the seam");
 
 struct FewArgs {
   WindowArgs w;
-  const __half *q, *k, *v;
-  long long q_stride, k_stride, v_stride;
+  const __half* q;
+  long long q_stride;
   int splits;
   int cluster;  // the ranges of an item are a cluster, which puts them together itself; else they are left in `partial_*`
   float* partial_o;  // [batch, kv_heads, splits, 16, 64]
@@ -810,7 +813,16 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 load16(const __half* p) { return *reinterpret_cast<const uint4*>(p); }
+// Four 8 x 8 matrices of 16-byte rows, lane l giving the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
 // Every thread of every CTA of the cluster: what was written to shared memory before is visible to all after.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -862,13 +874,30 @@ __device__ __forceinline__ bool few_item(const WindowArgs& a, int b, Item& it) {
 }
 
 template <bool BIAS>
-__global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __grid_constant__ FewArgs a) {
-  __shared__ __align__(16) float o_all[kFewWarps][kFewRows][kHeadDim + 4];
+__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas)
+window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FewArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t bars[kFewWarps][kFewStages];
   __shared__ float2 ml_all[kFewWarps][kFewRows], ml_cta[kFewRows];
+  __shared__ int abort_word;
+  // the warps' results, where their rings were
+  auto& o_all = *reinterpret_cast<float(*)[kFewWarps][kFewRows][kHeadDim + 4]>(smem);
+  static_assert(sizeof(o_all) <= kFewWarps * kFewRing, "the results fit");
   pdl_launch_dependents();
   const WindowArgs& w = a.w;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int warp = uniform_int(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, kv = blockIdx.y, b = blockIdx.z;
+  const bool smem_ok = (smem_u32(smem) & 1023u) == 0u;
+  volatile int* abort_flag = &abort_word;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kFewWarps * kFewStages; ++i) mbar_init(&bars[0][0] + i, 1);
+    abort_word = smem_ok ? 0 : 1;
+    fence_mbar_init();
+    if (!smem_ok && w.status != nullptr) atomicCAS(w.status, 0, kStatusMhaLoadTimeout + 0x10);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  __syncthreads();
   pdl_wait();
   Item it;
   if (!few_item(w, b, it)) return;
@@ -879,21 +908,33 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __g
   const int first = static_cast<int>(static_cast<long long>(steps) * split / a.splits);
   const int last = static_cast<int>(static_cast<long long>(steps) * (split + 1) / a.splits);
 
-  // Queries: row r is query r / group, head r % group.  Dimensions 32 i + 8 c + 4 s + {0, 1} and + {2, 3} stand at the places 2c,
-  // 2c + 1 and 2c + 8, 2c + 9 of the product's step 2 i + s.
-  uint32_t qa[2][2][4];  // [row half][i][register]
+  uint8_t* ring = smem + warp * kFewRing;
+  auto fetch = [&](int step, int stage) {
+    const int u0 = step * kFewKeys;
+    const int row = it.k_row + (u0 < keys.ns ? u0 : keys.ws + u0 - keys.ns);
+    if (elect_one()) {
+      uint8_t* dst = ring + stage * 2 * kFewTile;
+      mbar_arrive_expect_tx(&bars[warp][stage], 2 * kFewTile);
+      tma_load_2d(dst, &tm_k, &bars[warp][stage], kv * kHeadDim, row);
+      tma_load_2d(dst + kFewTile, &tm_v, &bars[warp][stage], kv * kHeadDim, row);
+    }
+    __syncwarp();
+  };
+  if (smem_ok) {
+#pragma unroll
+    for (int i = 0; i < kFewStages; ++i)
+      if (first + warp + i * kFewWarps < last) fetch(first + warp + i * kFewWarps, i);
+  }
+  // Queries: row r is query r / group, head r % group
+  uint32_t qa[4][4];  // [16 dimensions][register]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = g + 8 * h;
+    const __half* p = a.q + static_cast<long long>(it.q_row + r / w.group) * a.q_stride + (kv * w.group + r % w.group) * kHeadDim + 2 * c;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows)
-        v = load16(a.q + static_cast<long long>(it.q_row + r / w.group) * a.q_stride + (kv * w.group + r % w.group) * kHeadDim + i * 32 + c * 8);
-      qa[h][i][0] = v.x;
-      qa[h][i][1] = v.y;
-      qa[h][i][2] = v.z;
-      qa[h][i][3] = v.w;
+    for (int i = 0; i < 4; ++i) {
+      qa[i][h] = r < rows ? *reinterpret_cast<const uint32_t*>(p + 16 * i) : 0u;
+      qa[i][2 + h] = r < rows ? *reinterpret_cast<const uint32_t*>(p + 16 * i + 8) : 0u;
     }
   }
   // virtual keys that the thread's two rows see: [0, a_hi) and [b_lo, b_hi); their bias rows
@@ -909,54 +950,36 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __g
     b_hi[h] = keys.ns + hi - keys.ws;
     bias[h] = BIAS ? w.bias + static_cast<long long>(kv * w.group + r % w.group) * w.bias_n : nullptr;
   }
-  const __half* kb = a.k + static_cast<long long>(it.k_row) * a.k_stride + kv * kHeadDim;
-  const __half* vb = a.v + static_cast<long long>(it.k_row) * a.v_stride + kv * kHeadDim;
-  auto key_of = [&](int u) {  // (keys behind the last one: the last one's row, with a weight of 0)
-    u = min(u, keys.total - 1);
-    return u < keys.ns ? u : keys.ws + u - keys.ns;
-  };
-  uint4 kr[4][2], vr[2][4];  // K: keys 8 n + g, dimensions 32 i + 8 c ..; V: keys 16 s + {2c, 2c + 1, 2c + 8, 2c + 9}, dimensions 8 g ..
-  auto load_k = [&](int u0) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const __half* p = kb + static_cast<long long>(key_of(u0 + 8 * n + g)) * a.k_stride + c * 8;
-      kr[n][0] = load16(p);
-      kr[n][1] = load16(p + 32);
-    }
-  };
-  auto load_v = [&](int u0) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        vr[s][x] = load16(vb + static_cast<long long>(key_of(u0 + 16 * s + 2 * c + (x & 1) + (x >> 1) * 8)) * a.v_stride + g * 8);
-  };
+  auto key_of = [&](int u) { return u < keys.ns ? u : keys.ws + u - keys.ns; };
   float o[8][4];
 #pragma unroll
   for (int t = 0; t < 8; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[t][i] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  if (first + warp < last) {
-    load_k((first + warp) * kFewKeys);
-    load_v((first + warp) * kFewKeys);
-  }
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = smem_ok;
 #pragma unroll 1
-  for (int step = first + warp; step < last; step += kFewWarps) {
+  for (int step = first + warp; ok && step < last; step += kFewWarps) {
     const int u0 = step * kFewKeys;
-    const bool more = step + kFewWarps < last;
+    ok = mbar_wait_warp(&bars[warp][stage], phase, abort_flag, w.status, kStatusMhaLoadTimeout);
+    if (!ok) break;
+    uint8_t* tile = ring + stage * 2 * kFewTile;
+    const uint32_t k_tile = smem_u32(tile), v_tile = k_tile + kFewTile;
     float s[4][4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mma_16816(s[n], qa[0][i][0], qa[1][i][0], qa[0][i][1], qa[1][i][1], kr[n][i].x, kr[n][i].y);
-        mma_16816(s[n], qa[0][i][2], qa[1][i][2], qa[0][i][3], qa[1][i][3], kr[n][i].z, kr[n][i].w);
+      for (int i = 0; i < 2; ++i) {  // keys 8 n .. (row lane % 8), 16-byte units 4 i + lane / 8 of their 128 swizzled bytes
+        uint32_t k[4];
+        load_matrices(k, k_tile + (8 * n + (lane & 7)) * 128 + (((4 * i + (lane >> 3)) ^ (lane & 7)) << 4));
+        mma_16816(s[n], qa[2 * i][0], qa[2 * i][1], qa[2 * i][2], qa[2 * i][3], k[0], k[1]);
+        mma_16816(s[n], qa[2 * i + 1][0], qa[2 * i + 1][1], qa[2 * i + 1][2], qa[2 * i + 1][3], k[2], k[3]);
       }
     }
-    if (more) load_k(u0 + kFewWarps * kFewKeys);
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -994,18 +1017,36 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __g
         l[h] += p0 + p1;
         p[n][h] = pack_half2(p0, p1);
       }
+    if (u0 + kFewKeys > keys.total) {
+      // the values behind the last key may be anybody's: none
+      if (lane >= keys.total - u0) {
+        uint4* row = reinterpret_cast<uint4*>(tile + kFewTile + lane * 128);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      __syncwarp();
+    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
-      const uint32_t v0[4] = {vr[st][0].x, vr[st][0].y, vr[st][0].z, vr[st][0].w}, v1[4] = {vr[st][1].x, vr[st][1].y, vr[st][1].z, vr[st][1].w};
-      const uint32_t v2[4] = {vr[st][2].x, vr[st][2].y, vr[st][2].z, vr[st][2].w}, v3[4] = {vr[st][3].x, vr[st][3].y, vr[st][3].z, vr[st][3].w};
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {  // output column n of the product t is dimension 8 n + t: t picks a half of the registers
-        const uint32_t sel = (t & 1) ? 0x7632u : 0x5410u;
-        mma_16816(o[t], p[2 * st][0], p[2 * st][1], p[2 * st + 1][0], p[2 * st + 1][1], __byte_perm(v0[t >> 1], v1[t >> 1], sel),
-                  __byte_perm(v2[t >> 1], v3[t >> 1], sel));
+      for (int t = 0; t < 8; t += 2) {  // keys 16 st .. and 16 st + 8 .. of the dimensions 8 t .., then 8 t + 8 ..
+        const int key = 16 * st + (lane & 15);
+        uint32_t v[4];
+        load_matrices_transposed(v, v_tile + key * 128 + (((t + (lane >> 4)) ^ (key & 7)) << 4));
+        mma_16816(o[t], p[2 * st][0], p[2 * st][1], p[2 * st + 1][0], p[2 * st + 1][1], v[0], v[1]);
+        mma_16816(o[t + 1], p[2 * st][0], p[2 * st][1], p[2 * st + 1][0], p[2 * st + 1][1], v[2], v[3]);
       }
     }
-    if (more) load_v(u0 + kFewWarps * kFewKeys);
+    __syncwarp();  // the warp has read the tiles
+    if (step + kFewStages * kFewWarps < last) fetch(step + kFewStages * kFewWarps, stage);
+    if (++stage == kFewStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  __syncthreads();  // all rings are read
+  if (*abort_flag != 0) {  // copies in flight land before the block's memory goes to another
+    for (int i = 0; i < 64; ++i) __nanosleep(2000);
   }
   // The warps' results: O, reference and sum of each row
 #pragma unroll
@@ -1013,12 +1054,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 3) window_few_kernel(const __g
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     if (c == 0) ml_all[warp][g + 8 * h] = make_float2(m[h], l[h]);
-    float* dst = &o_all[warp][g + 8 * h][16 * c];
 #pragma unroll
-    for (int t = 0; t < 8; t += 4) {
-      *reinterpret_cast<float4*>(dst + t) = make_float4(o[t][2 * h], o[t + 1][2 * h], o[t + 2][2 * h], o[t + 3][2 * h]);
-      *reinterpret_cast<float4*>(dst + 8 + t) = make_float4(o[t][2 * h + 1], o[t + 1][2 * h + 1], o[t + 2][2 * h + 1], o[t + 3][2 * h + 1]);
-    }
+    for (int t = 0; t < 8; ++t)
+      *reinterpret_cast<float2*>(&o_all[warp][g + 8 * h][8 * t + 2 * c]) = make_float2(o[t][2 * h], o[t][2 * h + 1]);
   }
   __syncthreads();
   // eight columns of a row to a thread
@@ -1144,7 +1182,7 @@ struct FewSplit {
 FewSplit few_split(int batch, int kv_heads, int group, int max_q, int max_k, int left, int sinks) {
   FewSplit f;
   if (static_cast<long long>(max_q) * group > kFewRows || batch > 65535 || kv_heads > 65535) return f;
-  constexpr long long kResident = 3 * 148, kOverhead = 200, kTogether = 400;
+  constexpr long long kResident = kFewCtas * 148, kOverhead = 200, kTogether = kFewCtas * 133;
   long long keys = max_k;
   if (left >= 0) keys = static_cast<long long>(left) + max_q + sinks + kSeam < keys ? static_cast<long long>(left) + max_q + sinks + kSeam : keys;
   const long long items = static_cast<long long>(batch) * kv_heads;
@@ -1164,7 +1202,7 @@ size_t few_workspace(long long items, FewSplit f) {
 }
 
 template <bool BIAS>
-cudaError_t launch_few(const FewArgs& a, int kv_heads, cudaStream_t stream) {
+cudaError_t launch_few(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const FewArgs& a, int kv_heads, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.splits, kv_heads, a.w.batch);
   cfg.blockDim = dim3(kFewWarps * 32);
@@ -1183,7 +1221,8 @@ cudaError_t launch_few(const FewArgs& a, int kv_heads, cudaStream_t stream) {
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, window_few_kernel<BIAS>, a);
+  cfg.dynamicSmemBytes = kFewSmemBytes;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, window_few_kernel<BIAS>, tm_k, tm_v, a);
   if (e == cudaSuccess && a.splits > 1 && !a.cluster) e = launch_pdl(window_few_join_kernel, dim3(a.w.max_q * a.w.group, kv_heads, a.w.batch), dim3(256), 0, stream, a);
   return e;
 }
@@ -1214,6 +1253,8 @@ cudaError_t device_facts(DeviceFacts* f) {
     e = cudaFuncSetAttribute(window_mha_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout::kBytes);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(window_mha_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout::kBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(window_few_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(window_few_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmemBytes);
     if (e != cudaSuccess) return e;
     known[dev] = n;
   }
@@ -1282,6 +1323,11 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
   w.status = dev.status;
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
   cudaError_t e;
+  // Without any key rows the loads of the one masked tile that an item walks need some rows: those of q do.
+  const bool none = a->k_rows == 0;
+  const void *k = none ? a->q : a->k, *v = none ? a->q : a->v;
+  const uint64_t k_rows = none ? a->q_rows : a->k_rows;
+  const long long k_ld = none ? a->q_row_stride : a->k_row_stride, v_ld = none ? a->q_row_stride : a->v_row_stride;
   const FewSplit split = few_split(a->batch, a->kv_head_num, w.group, a->max_q_len, a->max_k_len, a->left, a->sinks);
   if (split.ranges > 0) {
     const int splits = split.ranges;
@@ -1289,18 +1335,15 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
     const size_t need = few_workspace(items, split);
     if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return BT_ERR_WORKSPACE;
     if (!aligned(a->workspace, 16)) return BT_ERR_INVALID_ARG;
-    FewArgs f{w, static_cast<const __half*>(a->q), static_cast<const __half*>(a->k), static_cast<const __half*>(a->v),
-              a->q_row_stride, a->k_row_stride, a->v_row_stride, splits, split.cluster ? 1 : 0,
+    CUtensorMap tm_k, tm_v;
+    if (!make_tmap_2d(&tm_k, k, k_rows, kv_cols, k_ld, 64, kFewKeys) || !make_tmap_2d(&tm_v, v, k_rows, kv_cols, v_ld, 64, kFewKeys))
+      return BT_ERR_CUDA;
+    FewArgs f{w, static_cast<const __half*>(a->q), a->q_row_stride, splits, split.cluster ? 1 : 0,
               static_cast<float*>(a->workspace), nullptr};
     f.partial_ml = reinterpret_cast<float2*>(f.partial_o + items * splits * kFewRows * kHeadDim);
-    e = w.bias != nullptr ? launch_few<true>(f, a->kv_head_num, stream) : launch_few<false>(f, a->kv_head_num, stream);
+    e = w.bias != nullptr ? launch_few<true>(tm_k, tm_v, f, a->kv_head_num, stream) : launch_few<false>(tm_k, tm_v, f, a->kv_head_num, stream);
     return e == cudaSuccess ? BT_OK : BT_ERR_CUDA;
   }
-  // Without any key rows the loads of the one masked tile that an item walks need some rows: those of q do.
-  const bool none = a->k_rows == 0;
-  const void *k = none ? a->q : a->k, *v = none ? a->q : a->v;
-  const uint64_t k_rows = none ? a->q_rows : a->k_rows;
-  const long long k_ld = none ? a->q_row_stride : a->k_row_stride, v_ld = none ? a->q_row_stride : a->v_row_stride;
   CUtensorMap tm[5];
   const bool ok = make_tmap_2d(&tm[0], a->q, a->q_rows, q_cols, a->q_row_stride, 64, 128) &&
                   make_tmap_2d(&tm[1], k, k_rows, kv_cols, k_ld, 64, kKeys) && make_tmap_2d(&tm[2], v, k_rows, kv_cols, v_ld, 64, kKeys);
