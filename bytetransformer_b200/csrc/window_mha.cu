@@ -786,13 +786,15 @@ cudaError_t launch_window(const CUtensorMap (&tm)[5], WindowArgs a, int sms, cud
 // asks for.  The keys are read once and that is the time it takes, so a CTA belongs to a (sequence, key/value head, range of
 // its virtual keys) and all rows that need them; each of its four warps walks every fourth 32 keys with a softmax of its
 // own, on mma.sync (16 x 8 x 16: a tcgen05 tile would be one eighth full at best).  A warp has a ring of its own of 32 keys and
-// values, fetched by TMA a few steps ahead; no warp waits for another before the range ends.
+// values, fetched by TMA a step ahead; no warp waits for another before the range ends.  Bound by HBM: 32 sequences of 8192 keys, 32 heads
+// over 8, 81.7 us (6.6 TB/s); 64 of 4100 keys, 16 heads over 4, 44.2 us (with loads straight into the operands' registers 98 and 55).
+// Rings of 2 stages and three CTAs to an SM, 3 and two, 4 and one, of the latter 44.2 / 46.2 / 68.2 us.
 constexpr int kFewRows = 16;
 constexpr int kFewWarps = 4;
 constexpr int kFewKeys = 32;  // of a step
 constexpr int kFewCluster = 8;  // ranges that a cluster holds
-constexpr int kFewStages = 3;   // of a warp's ring
-constexpr int kFewCtas = 2;     // to an SM
+constexpr int kFewStages = 2;   // of a warp's ring
+constexpr int kFewCtas = 3;     // to an SM
 constexpr int kFewTile = kFewKeys * kHeadDim * 2;  // 4 KiB of K, and of V
 constexpr int kFewRing = kFewStages * 2 * kFewTile;
 constexpr int kFewSmemBytes = kFewWarps * kFewRing;
@@ -1172,23 +1174,24 @@ struct FewSplit {
   int ranges = 0;
   bool cluster = false;
 };
-// 444 CTAs are resident (three to an SM).  A CTA's time goes with its keys and something like 200 more (its first loads wait for
-// one another, its results are put together), so of the numbers of ranges that leave a range 128 keys the one with the
-// shortest sum over the waves is taken.  us per call, 64 sequences of 4100 keys, 16 heads over 4, by ranges:
-// 1 66, 2 68, 3 56, 6 61; 8 of 4096, 12 heads, 4 ranges (one wave) 23.9, 5 31.6, 7 29.5; 2 of 30000, 12 heads, 18 38.0, 24 46.9.
+// A CTA's time goes with its keys and something like 200 more (its first loads wait for one another, its results are put
+// together), so of the numbers of ranges that leave a range 128 keys the one with the shortest sum over the waves is taken.
+// Three CTAs are resident to an SM, but two of them already keep the memory busy: waves are counted by two.  us per call with
+// waves of 296 / 370 / 444 / 592: 64 sequences of 4100 keys, 16 heads over 4, 44.2 / 51.3 / 50.3 / 56.8; 32 of 8192, 32 over 8, 81.7 / 91.1 /
+// 88.6 / 105; 40 of 3000, 8 heads, 45.4 / 41.4 / 45.2 / 47.4; 8 of 4096, 12 heads, 21.5 / 21.5 / 21.0 / 25.2.
 // Clusters save the second kernel, but their CTAs come and go together: where all are resident at once 16 sequences of 1027
 // keys, one key/value head 7.2 us (second kernel: 7.8), 4 of 700, 2 heads 6.4 (7.5); where they are not, the 64 sequences of 4100
-// keys above 71 (55).
+// keys above 71 (55; all with the registers' loads that the rings replaced).
 FewSplit few_split(int batch, int kv_heads, int group, int max_q, int max_k, int left, int sinks) {
   FewSplit f;
   if (static_cast<long long>(max_q) * group > kFewRows || batch > 65535 || kv_heads > 65535) return f;
-  constexpr long long kResident = kFewCtas * 148, kOverhead = 200, kTogether = kFewCtas * 133;
+  constexpr long long kWave = 2 * 148, kOverhead = 200, kTogether = 400;
   long long keys = max_k;
   if (left >= 0) keys = static_cast<long long>(left) + max_q + sinks + kSeam < keys ? static_cast<long long>(left) + max_q + sinks + kSeam : keys;
   const long long items = static_cast<long long>(batch) * kv_heads;
   long long best = 0x7fffffffffffffffLL;
   for (int s = 1; s <= 148 && (s == 1 || s * 128LL <= keys); ++s) {
-    const long long cost = (items * s + kResident - 1) / kResident * (keys / s + kOverhead);
+    const long long cost = (items * s + kWave - 1) / kWave * (keys / s + kOverhead);
     if (cost < best) {
       f.ranges = s;
       best = cost;
