@@ -521,7 +521,7 @@ def _half_or_float(t: torch.Tensor, name: str, device=None) -> int:
 
 def _check_distances(q_len, k_len, max_distance, q_start):
     """The library's lengths and positions are 32 bits wide: what does not fit is refused before it is cut off."""
-    if q_len < 0 or k_len < 0 or max(q_len, k_len, abs(q_start)) > 1 << 29 or not 0 < max_distance <= 1 << 20:
+    if not (0 <= q_len <= 1 << 29 and 0 <= k_len <= 1 << 29 and -(1 << 29) <= q_start <= 1 << 29 and 0 < max_distance <= 1 << 20):
         raise RuntimeError("lengths and q_start must be at most 2^29, max_distance at most 2^20")
 
 
@@ -697,9 +697,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     rows, k_rows = q.shape[0], k.shape[0]
     if v.shape != k.shape:
         raise RuntimeError("k and v must have the same shape")
-    _rows(v, "v", device)
+    if v.dtype != torch.float16 or v.device != device or v.stride(1) != 1:
+        _rows(v, "v", device)  # (says what is wrong)
     batch = _ints(q_offsets, "q_offsets", device) - 1
-    if _ints(k_offsets, "k_offsets", device) != batch + 1 or batch < 0:
+    if batch < 0 or k_offsets is not q_offsets and _ints(k_offsets, "k_offsets", device) != batch + 1:
         raise RuntimeError("q_offsets and k_offsets must have batch + 1 elements")
     if k_lens is not None and _ints(k_lens, "k_lens", device) != batch:
         raise RuntimeError("k_lens must have batch elements")

@@ -402,6 +402,10 @@ def test_python_refusals(cuda_device):
         call(q, k, v, off.long(), off, 20, 20)
     with pytest.raises(RuntimeError, match="batch"):
         call(q, k, v, off, off[:1], 20, 20)
+    with pytest.raises(RuntimeError, match="Tensor type: v"):
+        call(q, k, v.float(), off, off, 20, 20)
+    with pytest.raises(RuntimeError, match="v must be"):
+        call(q, k, torch.empty(2 * D, 20, device=cuda_device, dtype=torch.float16).t(), off, off, 20, 20)
     with pytest.raises(RuntimeError, match="k_lens"):
         call(q, k, v, off, off, 20, 20, k_lens=off)
     with pytest.raises(RuntimeError, match="distance_bias"):
