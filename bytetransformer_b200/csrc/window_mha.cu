@@ -14,7 +14,7 @@
 //   share the 128 rows, one takes the even tiles, the other the odd ones, each with scores, weights, reference, sum and O of
 //   its own; the two results are put together when the item ends (the groups take turns in that).  With two CTAs to an SM
 //   four warps take turns on each scheduler.
-//   Measured on B200: one sequence of 8192, 2047 keys back, 16 heads over 4: 99.5 us, 605 TFLOP/s of the visible pairs (one group
+//   Measured on B200: one sequence of 8192, 2047 keys back, 16 heads over 4: 100.4 us, 600 TFLOP/s of the visible pairs (one group
 //   with 128-key tiles: 116); 8 ragged sequences of up to 4096, 256 keys to either side, bias, 12 heads: 79 us.  A group's tile of 64
 //   keys takes 2546 clocks with four groups to an SM: 700 until S is there, 540 for scores and maximum, 1060 for the weights (the
 //   special-function unit works 448 of them), 240 to hand them over.
@@ -45,6 +45,8 @@ constexpr int kSlots = 4;  // items between the loader and the other roles
 constexpr int kSeam = 32;  // keys of a box of the tile with the seam
 
 struct WindowArgs {
+  const __half *q, *k, *v;
+  long long q_stride, k_stride, v_stride;
   __half* out;
   long long out_stride;
   const int *q_offsets, *k_offsets, *k_lens;
@@ -55,7 +57,7 @@ struct WindowArgs {
   const float* bias;  // [heads, bias_n]: distances -bias_left ..., the outermost values beyond
   int bias_n, bias_left;
   int* status;
-    int take_over;  // the grid has more blocks than are resident
+  int take_over;  // the grid has more blocks than are resident
   int by_rows;    // the grid has blocks for as many items as offsets that rise can hold, which others may exceed
 };
 
@@ -64,6 +66,7 @@ struct Item {
   int p0;              // position of the first
   int head;
   int k_row, k_len;    // the sequence's keys
+  int number;          // see find_item
 };
 
 // The virtual keys of an item.
@@ -237,6 +240,104 @@ struct Int {
   static constexpr int value = N;
 };
 
+// `t` grows to the largest magnitude of the halves of w, NaN above all.
+__device__ __forceinline__ void watch(__half2& t, uint32_t w) {
+  t = __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&w)), t);
+}
+__device__ __forceinline__ void watch_row(__half2& t, const __half* row) {
+#pragma unroll 1
+  for (int x = 0; x < kHeadDim; x += 8) {
+    const uint4 w = *reinterpret_cast<const uint4*>(row + x);
+    watch(t, w.x);
+    watch(t, w.y);
+    watch(t, w.z);
+    watch(t, w.w);
+  }
+}
+__device__ __forceinline__ bool not_finite(__half2 t) { return !(__low2float(t) < INFINITY) || !(__high2float(t) < INFINITY); }
+// Where values of keys that a row does not see are infinities or NaN, a product with their weights of zero leaves NaN in the row.
+// A row that came out so is looked at again, by a whole warp: if any key or value that it does not see, of those that its item
+// multiplied, holds such a number, the row is done anew over the keys that it sees alone.  Slow (32 keys at a time, without
+// matrix instructions), but nothing with finite inputs comes here.
+template <bool BIAS>
+__device__ __forceinline__ void redo_row(const WindowArgs& a, const Keys& keys, const Item& it, int i, int head) {
+  const int lane = static_cast<int>(threadIdx.x & 31u);
+  const int p = it.p0 + i, kv = head / a.group;
+  const int hi = a.right < 0 ? it.k_len : min(it.k_len, p + a.right + 1);
+  const int a_hi = a.left < 0 ? 0 : min(a.sinks, hi), lo = a.left < 0 ? 0 : p - a.left;
+  const float* table = BIAS ? a.bias + static_cast<long long>(head) * a.bias_n : nullptr;
+  auto key_of = [&](int u) { return u < keys.ns ? u : keys.ws + u - keys.ns; };
+  auto bias_of = [&](int u) {
+    return BIAS ? bias_log2(__ldg(table + min(max(key_of(u) - p + a.bias_left, 0), a.bias_n - 1))) : 0.f;
+  };
+  auto seen = [&](int u) {
+    const int key = key_of(u);
+    return u < keys.total && key < hi && (key >= lo || key < a_hi) && bias_of(u) != -INFINITY;
+  };
+  auto row_of = [&](const __half* base, long long stride, int u) {
+    return base + (static_cast<long long>(it.k_row) + key_of(u)) * stride + kv * kHeadDim;
+  };
+  bool redo = false;
+#pragma unroll 1
+  for (int u = lane; u - lane < keys.total && !redo; u += 32) {
+    __half2 t = __half2half2(__ushort_as_half(0));
+    if (u < keys.total && !seen(u)) {
+      watch_row(t, row_of(a.k, a.k_stride, u));
+      watch_row(t, row_of(a.v, a.v_stride, u));
+    }
+    redo = __any_sync(0xffffffffu, not_finite(t));
+  }
+  if (!redo) return;
+  const __half* q = a.q + static_cast<long long>(it.q_row + i) * a.q_stride + head * kHeadDim;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;  // dimensions 2 lane, 2 lane + 1
+#pragma unroll 1
+  for (int u0 = 0; u0 < keys.total; u0 += 32) {
+    const int u = u0 + lane;
+    const bool mine = seen(u);
+    unsigned left = __ballot_sync(0xffffffffu, mine);
+    if (left == 0u) continue;
+    float s = -INFINITY;
+    if (mine) {
+      const __half* k = row_of(a.k, a.k_stride, u);
+      float dot = 0.f;
+#pragma unroll 1
+      for (int x = 0; x < kHeadDim; x += 8) {
+        const uint4 qw = *reinterpret_cast<const uint4*>(q + x), kw = *reinterpret_cast<const uint4*>(k + x);
+        const uint32_t qs[4] = {qw.x, qw.y, qw.z, qw.w}, ks[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float2 qf = __half22float2(*reinterpret_cast<const __half2*>(&qs[y]));
+          const float2 kf = __half22float2(*reinterpret_cast<const __half2*>(&ks[y]));
+          dot = fmaf(qf.x, kf.x, fmaf(qf.y, kf.y, dot));
+        }
+      }
+      s = fmaf(dot, a.scale_log2e, bias_of(u));
+    }
+    float top = s;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float m_new = fmaxf(m, top);
+    const float f = m_new == m ? 1.0f : ex2(m - m_new);
+    m = m_new;
+    const float w = mine ? ex2(s - (m == -INFINITY ? 0.f : m)) : 0.f;
+    l = fmaf(l, f, w);
+    o0 *= f;
+    o1 *= f;
+    for (; left != 0u; left &= left - 1u) {
+      const int t = __ffs(left) - 1;
+      const float wt = __shfl_sync(0xffffffffu, w, t);
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(row_of(a.v, a.v_stride, u0 + t) + 2 * lane));
+      o0 = fmaf(wt, v.x, o0);
+      o1 = fmaf(wt, v.y, o1);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  __syncwarp();  // behind what the warp has written there
+  *reinterpret_cast<uint32_t*>(a.out + static_cast<long long>(it.q_row + i) * a.out_stride + head * kHeadDim + 2 * lane) =
+      pack_half2(o0 * inv, o1 * inv);
+}
 // Bits lo .. hi - 1 of a word.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
   const uint32_t below_hi = hi >= 32 ? 0xffffffffu : (hi > 0 ? (1u << hi) - 1u : 0u);
@@ -249,6 +350,15 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {
 // that neighbouring lanes read in different banks.
 struct BiasSlice {
   float copy[2][144];
+};
+
+// Items in which a softmax warp has found rows that are not finite, looked at again when the block has no more items (in the
+// loop they would cost it the registers).  A warp with kMany of them asks the loader to take over no more blocks, which
+// then start as others end: it meets four more at most, but for items that only offsets that fall bring (their rows
+// beyond the list's end stay as they are).
+struct Again {
+  static constexpr int kMany = 5, kSize = 10;
+  int current, count, item[kSize];
 };
 
 struct Layout {
@@ -294,9 +404,11 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   uint64_t* taken_full = bars + 50;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 51);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* enough = abort_flag + 1;  // no more blocks are to be taken over
   uint8_t* taken = smem + L::kBar + 480;       // 16 bytes
   Item* items = reinterpret_cast<Item*>(smem + L::kBar + 496);
-  static_assert(496 + kSlots * sizeof(Item) <= 1024, "barriers and items");
+  Again* again_all = reinterpret_cast<Again*>(smem + L::kBar + 496 + kSlots * sizeof(Item));
+  static_assert(496 + kSlots * sizeof(Item) + 8 * sizeof(Again) <= 1024, "barriers, items and what is looked at again");
 
   const int warp = uniform_int(static_cast<int>(threadIdx.x >> 5));
   const int lane = threadIdx.x & 31;
@@ -325,6 +437,11 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     mbar_init(taken_full, 1);
     *abort_flag = smem_ok ? 0 : 1;
+    *enough = 0;
+    for (int s = 0; s < 8; ++s) {
+      again_all[s].current = static_cast<int>(blockIdx.x);
+      again_all[s].count = 0;
+    }
     fence_mbar_init();
     if (!smem_ok && args.status != nullptr) atomicCAS(args.status, 0, kLoadTimeout + 0x10);
     tma_prefetch_desc(&tm_q);
@@ -358,7 +475,10 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     it.k_row = uniform_int(s->k_row);
     it.k_len = uniform_int(s->k_len);
     __syncwarp();
-    if (lane == 0) mbar_arrive(&item_empty[n % kSlots]);
+    if (lane == 0) {
+      if (warp < 8) again_all[warp].current = s->number;
+      mbar_arrive(&item_empty[n % kSlots]);
+    }
   };
   // Tile j of item n belongs to group (j + n) & 1, so the group that had one tile more has one less next time.
 
@@ -371,24 +491,25 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       int cur_b = 0, cur_first = 0;
       bool have = find_item(args, static_cast<int>(blockIdx.x), cur_b, cur_first, it);
       uint32_t asked = 0;
+      int cur_number = 0;
       int beyond = args.by_rows && blockIdx.x == 0 ? static_cast<int>(gridDim.x) : -1;
       // The next block that has not started, or, behind the last one, items that the grid's bound did not foresee: offsets
       // that fall can hold more than it does, so the first block's CTA looks there once (which reports such offsets too).
       auto take_next = [&]() {
         have = false;
         if (args.take_over && asked != 0xffffffffu) {
-          while (true) {
+          while (__any_sync(0xffffffffu, *enough == 0)) {
             if (elect_one()) launch_control_ask(taken, taken_full);
             if (!wait_role(taken_full, asked & 1u, abort_flag, args.status, kLoadTimeout)) return;
             ++asked;
             const int block = uniform_int(launch_control_answer(taken));
             if (block < 0) break;
-            have = find_item(args, block, cur_b, cur_first, it);
+            have = find_item(args, cur_number = block, cur_b, cur_first, it);
             if (have) return;
           }
           asked = 0xffffffffu;
         }
-        if (beyond >= 0) have = find_item(args, beyond++, cur_b, cur_first, it);
+        if (beyond >= 0) have = find_item(args, cur_number = beyond++, cur_b, cur_first, it);
         if (!have) beyond = -1;
       };
       uint32_t count[2] = {0, 0};  // tiles of the groups so far
@@ -438,6 +559,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (lane == 0) {
           Item w = it;
           if (!have) w.rows = 0;
+          w.number = cur_number;
           items[slot] = w;
           mbar_arrive(&item_full[slot]);
         }
@@ -522,7 +644,7 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       lent = true;
       ++handed;
     };
-    auto merge = [&](float m, float l, bool both) {
+    auto merge = [&](float m, float l, bool both, __half2& bad) {
       // the group of the even ones puts the two together: O / row sum -> fp16 -> this warp's staging rows, half a row at a time
       // -> global memory, four threads to a half row
       const int other = (g ^ 1) * 4 + quarter;
@@ -566,6 +688,10 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           w.y = pack_half2(__uint_as_float(a[u * 8 + 2]), __uint_as_float(a[u * 8 + 3]));
           w.z = pack_half2(__uint_as_float(a[u * 8 + 4]), __uint_as_float(a[u * 8 + 5]));
           w.w = pack_half2(__uint_as_float(a[u * 8 + 6]), __uint_as_float(a[u * 8 + 7]));
+          watch(bad, w.x);
+          watch(bad, w.y);
+          watch(bad, w.z);
+          watch(bad, w.w);
           *reinterpret_cast<uint4*>(own + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = w;
         }
         if (h == 1) tc_fence_before();
@@ -740,9 +866,15 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (lane == 0) mbar_arrive(&p_full[g]);
       }
       const bool both = keys.tiles > 1;
-      if (first == 0)
-        merge(m_ref, l_run, both);
-      else if (both)
+      if (first == 0) {
+        __half2 bad = __half2half2(__ushort_as_half(0));
+        merge(m_ref, l_run, both, bad);
+        if (__any_sync(0xffffffffu, exists && not_finite(bad)) && lane == 0) {
+          Again& mine = again_all[warp];
+          if (mine.count < Again::kSize) mine.item[mine.count++] = mine.current;
+          if (mine.count >= Again::kMany) *enough = 1;
+        }
+      } else if (both)
         hand_over(m_ref, l_run);
       o_items[0] += first < keys.tiles ? 1u : 0u;
       o_items[1] += 1 - first < keys.tiles ? 1u : 0u;
@@ -754,6 +886,17 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       have = it.rows > 0;
     }
     tc_fence_before();
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < again_all[warp].count; ++i) {
+      int b = 0, f = 0;
+      find_item(args, again_all[warp].item[i], b, f, it);
+      const Keys keys = keys_of(args, it);
+      __half2 bad = __half2half2(__ushort_as_half(0));
+      if (r < it.rows) watch_row(bad, args.out + static_cast<long long>(it.q_row + r) * args.out_stride + it.head * kHeadDim);
+      unsigned rows = __ballot_sync(0xffffffffu, not_finite(bad));
+      for (; rows != 0u; rows &= rows - 1u) redo_row<BIAS>(args, keys, it, quarter * 32 + __ffs(rows) - 1, it.head);
+    }
   }
 
   __syncthreads();
@@ -802,8 +945,6 @@ static_assert(kFewKeys == kSeam, "a step's keys are neighbours, also at the seam
 
 struct FewArgs {
   WindowArgs w;
-  const __half* q;
-  long long q_stride;
   int splits;
   int cluster;  // the ranges of an item are a cluster, which puts them together itself; else they are left in `partial_*`
   float* partial_o;  // [batch, kv_heads, splits, 16, 64]
@@ -905,6 +1046,8 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   if (!few_item(w, b, it)) return;
   const Keys keys = keys_of(w, it);
   const int rows = it.rows * w.group;
+  // virtual keys between the first tokens and the window that none of the rows sees: of one step
+  const int hole_lo = min(w.sinks, keys.total), hole_hi = w.left < 0 ? 0 : keys.ns > 0 ? keys.ns : max(0, it.p0 - w.left) - keys.ws;
   // this CTA's virtual keys, in whole steps
   const int steps = (keys.total + kFewKeys - 1) / kFewKeys;
   const int first = static_cast<int>(static_cast<long long>(steps) * split / a.splits);
@@ -932,7 +1075,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = g + 8 * h;
-    const __half* p = a.q + static_cast<long long>(it.q_row + r / w.group) * a.q_stride + (kv * w.group + r % w.group) * kHeadDim + 2 * c;
+    const __half* p = w.q + static_cast<long long>(it.q_row + r / w.group) * w.q_stride + (kv * w.group + r % w.group) * kHeadDim + 2 * c;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       qa[i][h] = r < rows ? *reinterpret_cast<const uint32_t*>(p + 16 * i) : 0u;
@@ -1019,9 +1162,10 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         l[h] += p0 + p1;
         p[n][h] = pack_half2(p0, p1);
       }
-    if (u0 + kFewKeys > keys.total) {
-      // the values behind the last key may be anybody's: none
-      if (lane >= keys.total - u0) {
+    if (u0 + kFewKeys > keys.total || (u0 < hole_hi && hole_lo < hole_hi)) {
+      // the values that no row sees: none (those behind the last key may be anybody's)
+      const int u = u0 + lane;
+      if (u >= keys.total || (u >= hole_lo && u < hole_hi)) {
         uint4* row = reinterpret_cast<uint4*>(tile + kFewTile + lane * 128);
 #pragma unroll
         for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -1109,16 +1253,23 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     __syncwarp();
     cluster_sync();  // nobody's shared memory goes away while another reads it
   }
-  if (!write) return;
   if (a.splits == 1 || a.cluster) {
-    const float inv = 1.0f / sum;
-    uint4 out = make_uint4(0u, 0u, 0u, 0u);
-    if (sum != 0.f)
-      out = make_uint4(pack_half2(acc[0] * inv, acc[1] * inv), pack_half2(acc[2] * inv, acc[3] * inv), pack_half2(acc[4] * inv, acc[5] * inv),
-                       pack_half2(acc[6] * inv, acc[7] * inv));
-    *reinterpret_cast<uint4*>(w.out + static_cast<long long>(it.q_row + r / w.group) * w.out_stride + (kv * w.group + r % w.group) * kHeadDim +
-                              col) = out;
-  } else {
+    __half2 bad = __half2half2(__ushort_as_half(0));
+    if (write) {
+      const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+      const uint4 out = make_uint4(pack_half2(acc[0] * inv, acc[1] * inv), pack_half2(acc[2] * inv, acc[3] * inv),
+                                   pack_half2(acc[4] * inv, acc[5] * inv), pack_half2(acc[6] * inv, acc[7] * inv));
+      *reinterpret_cast<uint4*>(w.out + static_cast<long long>(it.q_row + r / w.group) * w.out_stride +
+                                (kv * w.group + r % w.group) * kHeadDim + col) = out;
+      watch(bad, out.x);
+      watch(bad, out.y);
+      watch(bad, out.z);
+      watch(bad, out.w);
+    }
+    const unsigned again = __ballot_sync(0xffffffffu, not_finite(bad));
+    for (int i = 0; again != 0u && i < 4; ++i)
+      if ((again >> (8 * i)) & 0xffu) redo_row<BIAS>(w, keys, it, (4 * warp + i) / w.group, kv * w.group + (4 * warp + i) % w.group);
+  } else if (write) {
     const long long at = ((static_cast<long long>(b) * gridDim.y + kv) * a.splits + split) * kFewRows + r;
     if (col == 0) a.partial_ml[at] = make_float2(top, sum);
     float4* dst = reinterpret_cast<float4*>(a.partial_o + at * kHeadDim + col);
@@ -1128,6 +1279,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 }
 
 // The ranges of a row put together: sixteen threads by four columns, each of sixteen groups takes every sixteenth range.
+template <bool BIAS>
 __global__ void __launch_bounds__(256) window_few_join_kernel(const __grid_constant__ FewArgs a) {
   __shared__ float4 o_all[16][16];
   __shared__ float2 ml_all[16];
@@ -1158,13 +1310,18 @@ __global__ void __launch_bounds__(256) window_few_join_kernel(const __grid_const
   o_all[part][x] = acc;
   if (x == 0) ml_all[part] = make_float2(top, sum);
   __syncthreads();
-  if (part != 0) return;
-  for (int i = 1; i < min(16, a.splits); ++i) take(ml_all[i], o_all[i][x]);
-  const float inv = 1.0f / sum;
-  uint2 out = make_uint2(0u, 0u);
-  if (sum != 0.f) out = make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
-  *reinterpret_cast<uint2*>(w.out + static_cast<long long>(it.q_row + r / w.group) * w.out_stride + (kv * w.group + r % w.group) * kHeadDim +
-                            4 * x) = out;
+  if (threadIdx.x >= 32) return;
+  __half2 bad = __half2half2(__ushort_as_half(0));
+  if (part == 0) {
+    for (int i = 1; i < min(16, a.splits); ++i) take(ml_all[i], o_all[i][x]);
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    const uint2 out = make_uint2(pack_half2(acc.x * inv, acc.y * inv), pack_half2(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(w.out + static_cast<long long>(it.q_row + r / w.group) * w.out_stride +
+                              (kv * w.group + r % w.group) * kHeadDim + 4 * x) = out;
+    watch(bad, out.x);
+    watch(bad, out.y);
+  }
+  if (__any_sync(0xffffffffu, not_finite(bad))) redo_row<BIAS>(w, keys_of(w, it), it, r / w.group, kv * w.group + r % w.group);
 }
 
 // How a call of few queries is cut: ranges of a sequence's keys (0: the call is not one of few queries), and whether the ranges of
@@ -1226,7 +1383,7 @@ cudaError_t launch_few(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const F
   cfg.numAttrs = n;
   cfg.dynamicSmemBytes = kFewSmemBytes;
   cudaError_t e = cudaLaunchKernelEx(&cfg, window_few_kernel<BIAS>, tm_k, tm_v, a);
-  if (e == cudaSuccess && a.splits > 1 && !a.cluster) e = launch_pdl(window_few_join_kernel, dim3(a.w.max_q * a.w.group, kv_heads, a.w.batch), dim3(256), 0, stream, a);
+  if (e == cudaSuccess && a.splits > 1 && !a.cluster) e = launch_pdl(window_few_join_kernel<BIAS>, dim3(a.w.max_q * a.w.group, kv_heads, a.w.batch), dim3(256), 0, stream, a);
   return e;
 }
 
@@ -1303,6 +1460,12 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
   if (device_facts(&dev) != cudaSuccess) return BT_ERR_CUDA;
   if (dev.major != 10) return BT_ERR_UNSUPPORTED;
   WindowArgs w;
+  w.q = static_cast<const __half*>(a->q);
+  w.k = static_cast<const __half*>(a->k);
+  w.v = static_cast<const __half*>(a->v);
+  w.q_stride = a->q_row_stride;
+  w.k_stride = a->k_row_stride;
+  w.v_stride = a->v_row_stride;
   w.out = static_cast<__half*>(a->out);
   w.out_stride = a->out_row_stride;
   w.q_offsets = a->q_offsets;
@@ -1341,7 +1504,7 @@ extern "C" int bt_window_attention(const bt_window_attention_args* a, void* stre
     CUtensorMap tm_k, tm_v;
     if (!make_tmap_2d(&tm_k, k, k_rows, kv_cols, k_ld, 64, kFewKeys) || !make_tmap_2d(&tm_v, v, k_rows, kv_cols, v_ld, 64, kFewKeys))
       return BT_ERR_CUDA;
-    FewArgs f{w, static_cast<const __half*>(a->q), a->q_row_stride, splits, split.cluster ? 1 : 0,
+    FewArgs f{w, splits, split.cluster ? 1 : 0,
               static_cast<float*>(a->workspace), nullptr};
     f.partial_ml = reinterpret_cast<float2*>(f.partial_o + items * splits * kFewRows * kHeadDim);
     e = w.bias != nullptr ? launch_few<true>(tm_k, tm_v, f, a->kv_head_num, stream) : launch_few<false>(tm_k, tm_v, f, a->kv_head_num, stream);

@@ -357,8 +357,8 @@ int bt_add_residual_rmsnorm_e4m3(const void* x, int x_fp32, const void* residual
  *   with room to grow.  Query head h reads key/value head h / (head_num / kv_head_num).  Row strides in halves, multiples of 8;
  *   data pointers 16-byte aligned; q_offsets, k_offsets int32[batch+1], k_lens int32[batch], on the device.  max_q_len,
  *   max_k_len: upper bounds of Lq and Lk.  Rows of q and out from q_offsets[batch] on are neither read into a result nor written.
- *   The values in a sequence's own rows of k and v must be finite where any of 128 neighbouring queries sees them; what
- *   other rows hold does not matter.  out may not overlap q, k or v.
+ *   Keys and values that a query does not see, a sequence's own or others', do not matter to it, also where they are infinities
+ *   or NaN (rows beside which they are get done a second time, without matrix instructions).  out may not overlap q, k or v.
  *   Offsets or lengths that do not describe rows of the buffers make the sequence a no-op and set the device's status
  *   word, as in bt_attention (bt_device_status of any handle of the device).
  *   The current device is the one used; the first call on it looks its properties up and must be outside a stream capture. */

@@ -418,3 +418,87 @@ def test_python_refusals(cuda_device):
         call(q, k, v, off, off, 20, 20, scale=0.0)
     with pytest.raises(BtError):  # rows that start anywhere
         call(torch.zeros(20, 4 * D + 4, device=cuda_device, dtype=torch.float16)[:, :4 * D], k, v, off, off, 20, 20)
+
+
+def poisoned(q, k, v, off, k_off, max_q, max_k, rows, where, k_lens=None, **how):
+    """Puts `where` into rows of k and v.  Rows of q that see none of them come out as without it (against the definition in
+    64 bits); those that see one do not stay finite in the dimensions of v that hold it."""
+    from bytetransformer_b200 import encoder as E
+    args = {"left": -1, "right": -1, "sinks": 0, "bias": None, "bias_left": 0, **how}
+    k, v = k.clone(), v.clone()
+    k[rows], v[rows] = 0.0, 0.0
+    group = q.shape[1] // k.shape[1]
+    want, tol = definition(q, k, v, off, k_off, k_lens, *(args[n] for n in ("left", "right", "sinks", "bias", "bias_left")))
+    mark = torch.zeros_like(v)
+    mark[rows] = 1.0  # 1 of v: the weight of what is poisoned
+    ask = {"left": args["left"], "right": args["right"], "sinks": args["sinks"], "k_lens": k_lens, "distance_bias": args["bias"],
+           "bias_left": args["bias_left"]}
+    weight = definition(q, k, mark, off, k_off, k_lens, *(args[n] for n in ("left", "right", "sinks", "bias", "bias_left")))[0]
+    sees = (weight != 0).view(len(q), -1, D).any(2)  # [row, head]
+    v[rows, 1::3] = where
+    for poison_keys in (False, True):
+        if poison_keys:
+            k[rows, 5::7] = where
+        got = E.window_attention(q, k, v, off, k_off, max_q, max_k, **ask).double()
+        ok = ((got - want).abs() <= tol) | torch.isnan(want)
+        ok = ok.view(len(q), -1, D)
+        assert ok[~sees].all(), ((~ok).any(2) & ~sees).nonzero()[:8].tolist()
+        hit = torch.zeros(v.shape[1], dtype=torch.bool, device=q.device)
+        hit[1::3] = True
+        hit = hit.view(-1, D).repeat_interleave(group, 0)  # [head, dimension]
+        if not poison_keys:  # (a score that infinities in k make -inf leaves its key without weight)
+            assert not torch.isfinite(got.view(len(q), -1, D)[sees[:, :, None] & hit[None]]).any()
+    return sees
+
+
+@pytest.mark.parametrize("where", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("left,right,sinks", [(-1, 0, 0), (70, 0, 0), (70, 0, 4), (3, 5, 40), (0, 0, 1)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_what_a_row_does_not_see_does_not_matter(cuda_device, where, left, right, sinks, with_bias):
+    lens = [300, 1, 700, 130]
+    q, k, v, off = packed(lens, 4, 2, cuda_device, seed=21)
+    bias = torch.randn(4, 33, device=cuda_device) if with_bias else None
+    how = {"left": left, "right": right, "sinks": sinks, "bias": bias, "bias_left": 16}
+    for rows in ([299], [100, 301, 650], [4, 39, 305, 340, 1130], [64, 365, 1001 + 64]):
+        sees = poisoned(q, k, v, off, off, 700, 700, rows, where, **how)
+        assert sees.any() and not sees.all()
+
+
+@pytest.mark.parametrize("where", [math.inf, math.nan])
+@pytest.mark.parametrize("batch,room", [(3, 500), (12, 4000), (300, 200)])
+@pytest.mark.parametrize("q_len,left,right,sinks", [(1, 60, 0, 4), (3, -1, 0, 0), (4, 20, 0, 33), (2, 60, 1, 5)])
+def test_what_a_token_does_not_see_does_not_matter(cuda_device, batch, room, q_len, left, right, sinks, where):
+    """Caches with what has left the window, tokens that follow one another; one range of keys, clusters, the second kernel."""
+    heads, kv = 8, 2
+    g = torch.Generator().manual_seed(22)
+    q = torch.randn(batch * q_len, heads * D, generator=g).half().to(cuda_device)
+    kv_rows = torch.randn(batch * room, 2 * kv * D, generator=g).half().to(cuda_device)
+    lens = torch.randint(room // 2, room + 1, (batch,), generator=g)
+    off = torch.arange(batch + 1, dtype=torch.int32, device=cuda_device) * q_len
+    k_off = torch.arange(batch + 1, dtype=torch.int32, device=cuda_device) * room
+    firsts = torch.arange(batch) * room
+    lens_dev = lens.int().to(cuda_device)
+    for spots in ([lens - 1], [firsts * 0 + 6, lens - 75], [firsts * 0 + 31, lens - 62, lens - 2]):
+        rows = torch.cat([firsts + s for s in spots])[::2].tolist()
+        poisoned(q, kv_rows[:, :kv * D], kv_rows[:, kv * D:], off, k_off, q_len, room, rows, where, k_lens=lens_dev, left=left, right=right,
+                 sinks=sinks)
+
+
+def test_what_a_bias_hides_does_not_matter(cuda_device):
+    q, k, v, off = packed([300, 90], 2, 1, cuda_device, seed=23)
+    bias = torch.randn(2, 201, device=cuda_device)
+    bias[0, :70] = bias[1, 120:150] = -math.inf
+    for where in (math.inf, math.nan):
+        poisoned(q, k, v, off, off, 300, 300, [40, 200, 350], where, bias=bias, bias_left=100)
+        ones = torch.arange(3, dtype=torch.int32, device=cuda_device)
+        poisoned(q[:2], k, v, ones, off, 1, 300, [180, 350], where, bias=bias, bias_left=100)
+
+
+def test_many_rows_that_do_not_see_something(cuda_device):
+    """Every item of blocks that take over one another holds what some of its rows must not see."""
+    lens = [(i * 53) % 400 + 1 for i in range(70)]
+    q, k, v, off = packed(lens, 8, 4, cuda_device, seed=24)
+    firsts = torch.tensor([0] + lens).cumsum(0)[:-1]
+    rows = torch.cat([firsts + torch.tensor(lens) - 1, (firsts + 127)[torch.tensor(lens) > 128]]).tolist()
+    poisoned(q, k, v, off, off, 400, 400, rows, math.nan, left=-1, right=0, sinks=0)
+    poisoned(q, k, v, off, off, 400, 400, rows, math.inf, left=90, right=0, sinks=3)
