@@ -43,6 +43,7 @@ constexpr int kKvTile = kKeys * kHeadDim * 2;  // 8 KiB
 constexpr int kThreads = 384;  // two groups of four softmax warps; loads, MMAs of either group, bias
 constexpr int kSlots = 4;  // items between the loader and the other roles
 constexpr int kSeam = 32;  // keys of a box of the tile with the seam
+constexpr float kOneBias = 1048576.0f;  // a bias that is one for many keys is kept out of their scores below this (log2 units)
 
 struct WindowArgs {
   const __half *q, *k, *v;
@@ -740,9 +741,11 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             const float v0 = bias_log2(__ldg(table + min(max(at + lane, 0), args.bias_n - 1)));
             const float v1 = bias_log2(__ldg(table + min(max(at + 32 + lane, 0), args.bias_n - 1)));
             one[h] = v0;
-            // One value for all need not be added to each score (unless it is so large that the sum swallows the scores: then it has
-            // to, as where there are several)
-            several[h] = !((at >= args.bias_n - 1 || at + 62 <= 0) && (fabsf(v0) < 1e30f || v0 == -INFINITY));
+            // One value for all need not be added to each score: it goes into the exponent's offset, less the reference.  That needs a
+            // reference that is no coarser than the weights' range allows (below 2^20 it is rounded to 2^-4 at worst); beyond,
+            // it would lose the scores (at 1e9 its steps are 128) and leave their weights without bound.  There the value is
+            // added to each score, as where there are several, and the sum swallows the score for all alike.
+            several[h] = !((at >= args.bias_n - 1 || at + 62 <= 0) && (fabsf(v0) < kOneBias || v0 == -INFINITY));
             slice->copy[0][64 * h + lane] = v0;
             slice->copy[0][64 * h + 32 + lane] = v1;
             if (lane > 0) slice->copy[1][64 * h + lane - 1] = v0;

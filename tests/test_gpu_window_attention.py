@@ -502,3 +502,67 @@ def test_many_rows_that_do_not_see_something(cuda_device):
     rows = torch.cat([firsts + torch.tensor(lens) - 1, (firsts + 127)[torch.tensor(lens) > 128]]).tolist()
     poisoned(q, k, v, off, off, 400, 400, rows, math.nan, left=-1, right=0, sinks=0)
     poisoned(q, k, v, off, off, 400, 400, rows, math.inf, left=90, right=0, sinks=3)
+
+
+def swallowed(q, k, v, off, rows_of, left, right, bias, bias_left):
+    """`definition` where a bias of 1e9 and more leaves nothing of a score in single precision (a step is 128 there in the kernels' log2
+    units, so a score of less than 44 changes nothing): such keys weigh by their bias alone.  A smaller bias costs a score half a
+    step of the sum, twice because the sum of weights has it too."""
+    heads, group = q.shape[1] // D, q.shape[1] // k.shape[1]
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    ends = off.tolist()
+    for b, (first, last) in enumerate(rows_of):
+        n, m = ends[b + 1] - ends[b], last - first
+        p = torch.arange(m, device=q.device)[:, None] + n - m
+        j = torch.arange(n, device=q.device)[None, :]
+        seen = torch.ones(m, n, dtype=torch.bool, device=q.device)
+        if right >= 0:
+            seen &= j <= p + right
+        if left >= 0:
+            seen &= j >= p - left
+        for h in range(heads):
+            c, d = slice(h * D, h * D + D), slice(h // group * D, h // group * D + D)
+            qq, kk, vv = (t.double() for t in (q[first:last, c], k[ends[b]:ends[b + 1], d], v[ends[b]:ends[b + 1], d]))
+            s = qq @ kk.t() * 0.125
+            assert float(s.abs().max()) < 44
+            add = bias[h].double()[(j - p + bias_left).clamp(0, bias.shape[1] - 1)]
+            low = add.abs() >= 1e9
+            w = torch.softmax((torch.where(low, 0.0, s) + add).masked_fill(~seen, -math.inf), dim=1)
+            finite = torch.where(low, 0.0, add)
+            slack = float(qq.norm(dim=1).max() * kk.norm(dim=1).max() * 0.125) * 70 * 2.0 ** -24 + 2.0 ** -21
+            slack = slack + float(finite.abs().max()) * 2.0 ** -23
+            out[first:last, c] = w @ vv
+            tol[first:last, c] = (w @ vv.abs()) * (2.0 ** -11 + 2 * slack) * 1.01 + \
+                seen.sum(1, keepdim=True) * 2.0 ** -25 * float(vv.abs().max()) + (w @ vv).abs() * 2.0 ** -11 + 2.0 ** -25
+    return out, tol
+
+
+@pytest.mark.parametrize("low", [-1e4, -1e5, -1e9, -1e12, -1e29, 1e9, 1e12])
+@pytest.mark.parametrize("side", ["left", "right", "both"])
+@pytest.mark.parametrize("left,right", [(-1, -1), (-1, 0), (400, 300)])
+@pytest.mark.parametrize("last", [0, 1])
+def test_biases_that_swallow_the_scores(cuda_device, low, side, left, right, last):
+    """Masks by distance like -1e9: whole tiles of nothing else ahead of, behind and between tiles with other biases, and rows that
+    see nothing else, with scores far beyond fp16's range of exponents.  last: one query for each sequence."""
+    from bytetransformer_b200 import encoder as E
+    lens = [700, 260, 64]
+    q, k, v, off = packed(lens, 2, 1, cuda_device, seed=31)
+    q, k = (q * 2.2).half(), (k * 2.2).half()
+    bias = torch.randn(2, 201, device=cuda_device)
+    if side in ("left", "both"):
+        bias[:, :70] = low
+    if side in ("right", "both"):
+        bias[:, 140:] = low
+    bias[1] = low
+    ends = off.tolist()
+    if last:
+        rows = [(i, i + 1) for i in range(3)]
+        q = torch.stack([q[e - 1] for e in ends[1:]])
+        q_off = torch.arange(4, dtype=torch.int32, device=cuda_device)
+    else:
+        rows, q_off = list(zip(ends, ends[1:])), off
+    want, tol = swallowed(q, k, v, off, rows, left, right, bias, 100)
+    got = E.window_attention(q, k, v, q_off, off, 1 if last else 700, 700, left=left, right=right, distance_bias=bias, bias_left=100)
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist(), int((~torch.isfinite(got)).sum()))
