@@ -1001,6 +1001,9 @@ __device__ __forceinline__ float2 load_of(const float2* p, int rank) {
   return v;
 }
 
+// A range (reference, sum) of whose keys the row sees none.  Scores that are NaN leave the reference alone, and a sum that is not 0.
+__device__ __forceinline__ bool saw_nothing(float2 ml) { return ml.x == -INFINITY && ml.y == 0.f; }
+
 // The sequence of a CTA: rows of its queries, position of the first, its keys.  false: nothing to do.
 __device__ __forceinline__ bool few_item(const WindowArgs& a, int b, Item& it) {
   const int start = a.q_offsets[b], len = a.q_offsets[b + 1] - start;
@@ -1219,7 +1222,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
     for (int i = 0; i < kFewWarps; ++i) {
       const float2 ml = ml_all[i][r];
-      if (ml.x == -INFINITY) continue;  // this warp has seen no key of the row
+      if (saw_nothing(ml)) continue;
       const float f = ex2(ml.x - top);
       sum = fmaf(ml.y, f, sum);
 #pragma unroll
@@ -1245,7 +1248,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       for (int i = 0; i < a.splits; ++i) {
         const float2 ml = load_of(&ml_cta[r], i);
         const float4 o0 = load_of(mine, i), o1 = load_of(mine + 4, i);
-        if (ml.x == -INFINITY) continue;
+        if (saw_nothing(ml)) continue;
         const float f = ex2(ml.x - top);
         sum = fmaf(ml.y, f, sum);
         const float o[8] = {o0.x, o0.y, o0.z, o0.w, o1.x, o1.y, o1.z, o1.w};
@@ -1296,7 +1299,7 @@ __global__ void __launch_bounds__(256) window_few_join_kernel(const __grid_const
   float top = -INFINITY, sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto take = [&](float2 ml, float4 o) {
-    if (ml.x == -INFINITY) return;  // no key of the range is seen
+    if (saw_nothing(ml)) return;
     const float next = fmaxf(top, ml.x), f0 = ex2(top - next), f1 = ex2(ml.x - next);
     top = next;
     sum = fmaf(ml.y, f1, sum * f0);

@@ -566,3 +566,35 @@ def test_biases_that_swallow_the_scores(cuda_device, low, side, left, right, las
     got = E.window_attention(q, k, v, q_off, off, 1 if last else 700, 700, left=left, right=right, distance_bias=bias, bias_left=100)
     bad = ~((got.double() - want).abs() <= tol)
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[0].tolist(), int((~torch.isfinite(got)).sum()))
+
+
+@pytest.mark.parametrize("batch,room", [(3, 100), (2, 1500), (40, 3000), (300, 200)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_nan_in_a_token_or_in_a_key_that_it_sees_reaches_the_result(cuda_device, batch, room, with_bias):
+    """One range of keys, clusters, the second kernel: a range, or a warp's share of one, all of whose scores are NaN is not one in which
+    nothing is seen.  Other rows keep every bit."""
+    from bytetransformer_b200 import encoder as E
+    heads, kv = 8, 8
+    g = torch.Generator().manual_seed(41)
+    q = torch.randn(batch, heads * D, generator=g).half().to(cuda_device)
+    cache = torch.randn(batch * room, 2 * kv * D, generator=g).half().to(cuda_device)
+    off = torch.arange(batch + 1, dtype=torch.int32, device=cuda_device)
+    bias = torch.randn(heads, 65, generator=g).to(cuda_device) if with_bias else None
+
+    def call(q, cache, left):
+        return E.window_attention(q, cache[:, :kv * D], cache[:, kv * D:], off, off * room, 1, room, left=left, right=0, distance_bias=bias,
+                                  bias_left=64).view(batch, heads, D)
+    for left in (-1, room // 2, 0):
+        clean = call(q, cache, left)
+        assert torch.isfinite(clean).all()
+        sick = q.clone().view(batch, heads, D)
+        sick[1, 2, 7] = sick[batch - 1, 0, 63] = float("nan")
+        got = call(sick.view(batch, -1), cache, left)
+        rows = torch.zeros(batch, heads, dtype=torch.bool, device=cuda_device)
+        rows[1, 2] = rows[batch - 1, 0] = True
+        assert torch.isnan(got[rows]).all() and torch.equal(got[~rows], clean[~rows])
+        sick = cache.clone()
+        sick[2 * room - 1, 2 * D + 9] = float("nan")  # the key of the token itself, for a head
+        got = call(q, sick, left)
+        rows[batch - 1, 0] = False
+        assert torch.isnan(got[rows]).all() and torch.equal(got[~rows], clean[~rows])
