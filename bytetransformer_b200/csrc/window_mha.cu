@@ -1176,6 +1176,7 @@ window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
       }
+      fence_proxy_async_smem();  // ahead of the copy that fills this stage again
       __syncwarp();
     }
 #pragma unroll
