@@ -668,6 +668,11 @@ def _rows(t: torch.Tensor, name: str, device) -> int:
     return cols // 64
 
 
+def _pitch(t: torch.Tensor) -> int:
+    """Elements from a row to the next.  The stride of a single row says nothing, whatever it is."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def _ints(t: torch.Tensor, name: str, device) -> int:
     if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.device != device:
         raise RuntimeError(f"{name} must be a contiguous int32 vector on the device of the other tensors")
@@ -732,8 +737,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
             if n:
                 ws = torch.empty(n, dtype=torch.int8, device=device)
         a = _abi.bt_window_attention_args(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), k.stride(0), v.stride(0),
-            out.stride(0), q_offsets.data_ptr(), k_offsets.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _pitch(q), _pitch(k), _pitch(v), _pitch(out),
+            q_offsets.data_ptr(), k_offsets.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
             batch, heads, kv_heads, rows, k_rows, max_q_len, max_k_len, left, right, sinks, scale,
             distance_bias.data_ptr() if distance_bias is not None else None, n_bias, bias_left if n_bias else 0,
             ws.data_ptr() if n else None, n)

@@ -598,3 +598,27 @@ def test_nan_in_a_token_or_in_a_key_that_it_sees_reaches_the_result(cuda_device,
         got = call(q, sick, left)
         rows[batch - 1, 0] = False
         assert torch.isnan(got[rows]).all() and torch.equal(got[~rows], clean[~rows])
+
+
+def test_a_single_row_of_any_stride(cuda_device):
+    """torch leaves the stride of a dimension of one element to chance: one token, one key, a result of one row."""
+    from bytetransformer_b200 import encoder as E
+
+    def row(t, stride):
+        return t.reshape(1, -1).as_strided((1, t.numel()), (stride, 1))
+    g = torch.Generator().manual_seed(51)
+    q = torch.randn(1, 4 * D, generator=g).half().to(cuda_device)
+    k, v = (torch.randn(30, 2 * D, generator=g).half().to(cuda_device) for _ in range(2))
+    one = torch.tensor([0, 1], dtype=torch.int32, device=cuda_device)
+    ends = torch.tensor([0, 30], dtype=torch.int32, device=cuda_device)
+    want = E.window_attention(q, k, v, one, ends, 1, 30)
+    want_one = E.window_attention(q, k[:1], v[:1], one, one, 1, 1)
+    for stride in (0, 1, 7, 10 ** 6, 1 << 40):
+        out = torch.empty_like(q)
+        E.window_attention(row(q, stride), k, v, one, ends, 1, 30, out=row(out, stride))
+        assert torch.equal(out, want)
+        assert torch.equal(E.window_attention(q, row(k[0], stride), row(v[0], stride), one, one, 1, 1), want_one)
+    many = torch.randn(200, 4 * D, generator=g).half().to(cuda_device)  # the block kernel over one key
+    offs = torch.tensor([0, 200], dtype=torch.int32, device=cuda_device)
+    assert torch.equal(E.window_attention(many, row(k[0], 1), row(v[0], 1), offs, one, 200, 1),
+                       E.window_attention(many, k[:1], v[:1], offs, one, 200, 1))
