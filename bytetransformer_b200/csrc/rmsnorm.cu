@@ -56,20 +56,28 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8]) {
   return make_uint2(w[0], w[1]);
 }
 
-// Sum or maximum over the WARPS warps of a row (one warp: lanes only).  `slot` alternates between calls.
+// The larger of two, NaN if either is: a group with NaN gets a scale that says so.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Sum or maximum over the WARPS warps of a row (one warp: lanes only).  No barrier stands behind the last reads of `scratch`: each
+// call in a kernel has a row of it to itself.
 template <int WARPS, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* scratch) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, u) : v + u;
+    v = MAX ? max_or_nan(v, u) : v + u;
   }
   if (WARPS == 1) return v;
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
   v = scratch[0];
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) v = MAX ? fmaxf(v, scratch[w]) : v + scratch[w];
+  for (int w = 1; w < WARPS; ++w) v = MAX ? max_or_nan(v, scratch[w]) : v + scratch[w];
   return v;
 }
 
@@ -148,14 +156,14 @@ __global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32, W
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         s[i][j] = s[i][j] * rstd * g[j];
-        if (OUT == kRmsRowScale) top = fmaxf(top, fabsf(s[i][j]));
+        if (OUT == kRmsRowScale) top = max_or_nan(top, fabsf(s[i][j]));
       }
       if (OUT == kRmsHalf) reinterpret_cast<uint4*>(a.out)[at + v] = pack8(s[i]);
     }
   }
   if (OUT == kRmsRowScale) {
     top = row_reduce<WARPS, true>(top, scratch[1]);
-    const float scale = fmaxf(top, 0x1p-100f) / 448.0f;
+    const float scale = max_or_nan(top, 0x1p-100f) / 448.0f;
     const float inv = 1.0f / scale;
     if (t == 0) a.scales[row] = scale;
 #pragma unroll
@@ -175,10 +183,10 @@ __global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32, W
       const int v = i * kLanes + t;
       float m = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(s[i][j]));
+      for (int j = 0; j < 8; ++j) m = max_or_nan(m, fabsf(s[i][j]));
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float scale = fmaxf(m, 0x1p-100f) / 448.0f;
+      for (int o = 8; o > 0; o >>= 1) m = max_or_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float scale = max_or_nan(m, 0x1p-100f) / 448.0f;
       const float inv = 1.0f / scale;
       if (v < nvec) {
         if ((t & 15) == 0) a.scales[static_cast<size_t>(row) * groups + (v >> 4)] = scale;

@@ -194,3 +194,31 @@ def test_python_refusals(cuda_device):
         E.add_residual_rmsnorm(torch.zeros(4, 12, dtype=torch.float16, device=cuda_device), None,
                                torch.ones(12, dtype=torch.float16, device=cuda_device))
     assert E.add_residual_rmsnorm(x[:0], r[:0], gamma)[0].shape == (0, 64)
+
+
+@pytest.mark.parametrize("hidden", [64, 520, 768, 2056, 4096, 12296])
+@pytest.mark.parametrize("group", [0, 128])
+def test_a_scale_says_where_its_group_holds_nan(cuda_device, hidden, group):
+    """scale = max |y| over the group, which is NaN where a y is: by NaN in the row, by an infinity (it makes NaN of itself, the rest is
+    finite), by NaN in gamma for its columns alone."""
+    from bytetransformer_b200 import encoder as E
+    x, r, gamma = inputs(7, hidden, False, False, True, cuda_device)
+    clean = E.add_residual_rmsnorm_e4m3(x, r, gamma, group=group)
+    at = hidden - 3
+    x[1, 2], x[4, at] = float("nan"), float("inf")
+    q, scales, _ = E.add_residual_rmsnorm_e4m3(x, r, gamma, group=group)
+    sick = torch.zeros_like(scales, dtype=torch.bool)
+    sick[1] = True
+    sick[4, at // 128 if group else 0] = True
+    assert torch.equal(torch.isnan(scales), sick)
+    wide = sick.repeat_interleave(group or hidden, dim=1)[:, :hidden]
+    assert torch.equal(torch.isnan(q.float()), wide)
+    keep = [0, 2, 3, 5, 6]
+    assert torch.equal(q[keep].view(torch.uint8), clean[0][keep].view(torch.uint8)) and torch.equal(scales[keep], clean[1][keep])
+    gamma[at] = float("nan")
+    x, r, _ = inputs(7, hidden, False, False, True, cuda_device)
+    q, scales, _ = E.add_residual_rmsnorm_e4m3(x, r, gamma, group=group)
+    columns = torch.zeros(scales.shape[1], dtype=torch.bool, device=cuda_device)
+    columns[at // 128 if group else 0] = True
+    assert torch.equal(torch.isnan(scales), columns[None].expand_as(scales))
+    assert torch.equal(scales[:, ~columns], clean[1][:, ~columns])
