@@ -222,3 +222,17 @@ def test_a_scale_says_where_its_group_holds_nan(cuda_device, hidden, group):
     columns[at // 128 if group else 0] = True
     assert torch.equal(torch.isnan(scales), columns[None].expand_as(scales))
     assert torch.equal(scales[:, ~columns], clean[1][:, ~columns])
+
+
+@pytest.mark.parametrize("hidden", [136, 768, 4096])
+def test_every_group_uses_the_largest_number(cuda_device, hidden):
+    """The largest value of each 128 columns, not of the row alone, is +-448."""
+    from bytetransformer_b200 import encoder as E
+    x, r, gamma = inputs(40, hidden, True, False, True, cuda_device)
+    x[3, :128] = 0.0
+    r[3, :128] = 0.0
+    q, scales, _ = E.add_residual_rmsnorm_e4m3(x, r, gamma, group=128)
+    top = torch.stack([p.double().abs().amax(1) for p in q.float().split(128, dim=1)], dim=1)
+    want = torch.full_like(top, 448.0)
+    want[3, 0] = 0.0
+    assert torch.equal(top, want) and top.shape == scales.shape
