@@ -233,6 +233,10 @@ int rms(const void* x, int x_fp32, const void* residual, const void* gamma, int 
         float* scales, int kind, const int* m_dev, int m_rows, int hidden, float eps, void* stream) {
   if (!x || !gamma || !out || m_rows <= 0 || hidden <= 0 || hidden % 8 != 0 || hidden > 16384 || !(eps >= 0.f)) return BT_ERR_INVALID_ARG;
   if (!aligned16(x) || !aligned16(residual) || !aligned16(gamma) || !aligned16(sum_out) || !aligned16(out)) return BT_ERR_INVALID_ARG;
+  // In place only element for element: rows go on at once, and where elements differ in size one row's results lie on another's
+  // input.
+  if (out == sum_out || (out == x && (x_fp32 || kind != kRmsHalf)) || (out == residual && kind != kRmsHalf) || (sum_out == x && x_fp32))
+    return BT_ERR_INVALID_ARG;
   RmsArgs a{x, static_cast<const __half*>(residual), gamma, static_cast<__half*>(sum_out), out, scales, m_dev, m_rows, hidden, eps};
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;

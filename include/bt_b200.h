@@ -336,7 +336,8 @@ int bt_relative_position_bias_grad(const void* grad, int grad_fp32, int num_buck
  *     scale = max(max|y|, 2^-100) / 448,  out = y / scale (y: the fp16 form's result before rounding)
  *   for each row (group = 0, scales float[m_rows]) or each 128 columns of a row, the last of which may be fewer (group =
  *   128, scales float[m_rows, ceil(hidden / 128)]).  hidden % 8 == 0, <= 16384; pointers 16-byte aligned (m_dev, scales: 4).
- *   sum_out may be x (fp16) or residual, and out may be x (fp16), element for element; m_dev may be NULL. */
+ *   In place, element for element: sum_out may be an fp16 x or the residual, and so may out in the fp16 form where sum_out is not the
+ *   same.  No other overlap: out in 8 bits over x or residual, results over an fp32 x and out over sum_out are refused.  m_dev may be NULL. */
 int bt_add_residual_rmsnorm(const void* x, int x_fp32, const void* residual, const void* gamma, int gamma_fp32, void* sum_out,
                             void* out, const int* m_dev, int m_rows, int hidden, float eps, void* stream);
 int bt_add_residual_rmsnorm_e4m3(const void* x, int x_fp32, const void* residual, const void* gamma, int gamma_fp32,

@@ -236,3 +236,22 @@ def test_every_group_uses_the_largest_number(cuda_device, hidden):
     want = torch.full_like(top, 448.0)
     want[3, 0] = 0.0
     assert torch.equal(top, want) and top.shape == scales.shape
+
+
+@pytest.mark.parametrize("hidden", [768, 4096])
+def test_in_place_the_other_ways(cuda_device, hidden):
+    """The result over the residual and the sum over x; with 8 bits the sum over the residual."""
+    from bytetransformer_b200 import _abi
+    from bytetransformer_b200 import encoder as E
+    lib, stream = _abi.load(), torch.cuda.current_stream().cuda_stream
+    x, r, gamma = inputs(50, hidden, False, False, True, cuda_device)
+    out, total = E.add_residual_rmsnorm(x, r, gamma)
+    q, scales, _ = E.add_residual_rmsnorm_e4m3(x, r, gamma)
+    x1, r1 = x.clone(), r.clone()
+    assert lib.bt_add_residual_rmsnorm(x1.data_ptr(), 0, r1.data_ptr(), gamma.data_ptr(), 0, x1.data_ptr(), r1.data_ptr(), None, 50,
+                                       hidden, 1e-6, stream) == 0
+    assert torch.equal(r1, out) and torch.equal(x1, total)
+    q1, scales1, r1 = torch.empty_like(q), torch.empty_like(scales), r.clone()
+    assert lib.bt_add_residual_rmsnorm_e4m3(x.data_ptr(), 0, r1.data_ptr(), gamma.data_ptr(), 0, r1.data_ptr(), q1.data_ptr(),
+                                            scales1.data_ptr(), 0, None, 50, hidden, 1e-6, stream) == 0
+    assert torch.equal(q1.view(torch.uint8), q.view(torch.uint8)) and torch.equal(scales1, scales) and torch.equal(r1, total)

@@ -106,3 +106,21 @@ def test_window_workspace(lib):
     for bad in [(0, 8, 2, 1, 9, -1, 0), (1, 8, 3, 1, 9, -1, 0), (1, 8, 2, 0, 9, -1, 0), (1, 8, 2, 1, -1, -1, 0), (1, 8, 2, 1, 9, -1, -1)]:
         assert ask(*bad, C.byref(n)) == _abi.BT_ERR_INVALID_ARG
     assert ask(1, 8, 2, 1, 9, -1, 0, None) == _abi.BT_ERR_INVALID_ARG
+
+
+X, RES, SUM, OUT = P, 2 * P, 3 * P, 4 * P
+
+
+@pytest.mark.parametrize("x_fp32,group,total,out", [
+    (0, None, SUM, SUM), (1, None, SUM, SUM), (0, None, X, X), (0, None, RES, RES),      # two results in one place
+    (1, None, SUM, X), (1, None, X, OUT), (1, None, None, X), (1, 0, X, OUT),           # halves over single precision
+    (0, 0, SUM, X), (0, 128, SUM, X), (1, 128, None, X), (0, 0, SUM, RES), (0, 128, None, RES)])  # 8 bits over something else
+def test_norm_over_its_own_inputs(lib, x_fp32, group, total, out):
+    """Elements of another size lie on other rows' inputs, which may not have been read yet.  (What is allowed reaches a launch: it
+    is tested on the device.)"""
+    args = [X, x_fp32, RES, 5 * P, 0, total, out]
+    if group is None:
+        rc = lib.bt_add_residual_rmsnorm(*args, None, 4, 768, 1e-6, None)
+    else:
+        rc = lib.bt_add_residual_rmsnorm_e4m3(*args, 6 * P, group, None, 4, 768, 1e-6, None)
+    assert rc == _abi.BT_ERR_INVALID_ARG
