@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32, W
   pdl_wait();
   int rows = a.rows;
   if (a.m_dev != nullptr) rows = min(rows, *a.m_dev);
-  const int row = blockIdx.x * kRows + threadIdx.x / kLanes;
-  if (row >= rows) return;  // (of a row's warps all or none)
+  const unsigned row = blockIdx.x * kRows + threadIdx.x / kLanes;  // (the last block's rows may pass 2^31)
+  if (rows <= 0 || row >= static_cast<unsigned>(rows)) return;       // (of a row's warps all or none)
   const size_t at = static_cast<size_t>(row) * nvec;
   uint4 xv[NVEC][X_FP32 ? 2 : 1], rv[NVEC];
 #pragma unroll
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32, W
 template <bool X_FP32, bool G_FP32, int OUT, int WARPS, int NVEC>
 cudaError_t launch_one(const RmsArgs& a, cudaStream_t stream) {
   constexpr int kRows = WARPS == 1 ? kRmsWarpRows : 1;
-  return launch_pdl(add_residual_rmsnorm_kernel<X_FP32, G_FP32, OUT, WARPS, NVEC>, dim3((a.rows + kRows - 1) / kRows),
+  return launch_pdl(add_residual_rmsnorm_kernel<X_FP32, G_FP32, OUT, WARPS, NVEC>, dim3((static_cast<unsigned>(a.rows) + kRows - 1) / kRows),
                     dim3(WARPS == 1 ? kRmsWarpRows * 32 : WARPS * 32), 0, stream, a);
 }
 

@@ -519,8 +519,14 @@ def _half_or_float(t: torch.Tensor, name: str, device=None) -> int:
     return _FP32[t.dtype]
 
 
+def _check_sizes(*sizes):
+    """The library's sizes are 32 bits wide: what does not fit is refused before it is cut off."""
+    if max(sizes) >= 1 << 31 or min(sizes) < 0:
+        raise RuntimeError("sizes must be below 2^31 and not negative")
+
+
 def _check_distances(q_len, k_len, max_distance, q_start):
-    """The library's lengths and positions are 32 bits wide: what does not fit is refused before it is cut off."""
+    """The same for lengths and positions, whose sums have to fit too."""
     if not (0 <= q_len <= 1 << 29 and 0 <= k_len <= 1 << 29 and -(1 << 29) <= q_start <= 1 << 29 and 0 < max_distance <= 1 << 20):
         raise RuntimeError("lengths and q_start must be at most 2^29, max_distance at most 2^20")
 
@@ -537,6 +543,7 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_d
     if out_dtype not in (torch.float16, torch.float32):
         raise RuntimeError("out_dtype must be torch.float16 or torch.float32")
     buckets, heads = table.shape
+    _check_sizes(buckets, heads)
     _check_distances(q_len, k_len, max_distance, q_start)
     if q_len == 0 or k_len == 0:
         return torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
@@ -569,6 +576,7 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
         raise RuntimeError("grad must be [heads, q_len, k_len] or [batch, heads, q_len, k_len]")
     batch = int(grad.shape[0]) if grad.dim() == 4 else 1
     heads, q_len, k_len = grad.shape[-3:]
+    _check_sizes(num_buckets, batch, heads)
     _check_distances(q_len, k_len, max_distance, q_start)
     if grad.numel() == 0:
         return torch.zeros(num_buckets, heads, dtype=torch.float32, device=grad.device)
@@ -614,6 +622,7 @@ def add_residual_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], gamm
     fp16.  Rows from *m_dev on are left unwritten."""
     x_fp32, gamma_fp32 = _rmsnorm_args(x, residual, gamma, m_dev)
     rows, hidden = x.shape
+    _check_sizes(rows, hidden)
     lib = _abi.load()
     with _On(x.device) as stream:
         out = torch.empty(rows, hidden, dtype=torch.float16, device=x.device)
@@ -637,6 +646,7 @@ def add_residual_rmsnorm_e4m3(x: torch.Tensor, residual: Optional[torch.Tensor],
     if group not in (0, 128):
         raise RuntimeError("group must be 0 (a scale per row) or 128 (a scale per 128 columns)")
     rows, hidden = x.shape
+    _check_sizes(rows, hidden)
     lib = _abi.load()
     with _On(x.device) as stream:
         out = torch.empty(rows, hidden, dtype=torch.float8_e4m3fn, device=x.device)
@@ -719,8 +729,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
             raise RuntimeError("bias_left must be a place in distance_bias")
     if out is not None and (_rows(out, "out", device) != heads or out.shape[0] != rows):
         raise RuntimeError("out must have q's shape")
-    if max(max_q_len, max_k_len) >= 1 << 30 or sinks < 0:
-        raise RuntimeError("max_q_len and max_k_len must be below 2^30, sinks not negative")
+    if max(max_q_len, max_k_len) >= 1 << 30 or min(max_q_len, max_k_len, sinks) < 0:
+        raise RuntimeError("max_q_len and max_k_len must be below 2^30, they and sinks not negative")
+    _check_sizes(batch, rows, k_rows, heads, n_bias)
     # bounds that no distance reaches, however large, are none (the library's are 32 bits wide)
     left = -1 if left < 0 or left >= max_k_len else left
     right = -1 if right < 0 or right >= 1 << 30 else right

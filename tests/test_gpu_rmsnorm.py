@@ -255,3 +255,16 @@ def test_in_place_the_other_ways(cuda_device, hidden):
     assert lib.bt_add_residual_rmsnorm_e4m3(x.data_ptr(), 0, r1.data_ptr(), gamma.data_ptr(), 0, r1.data_ptr(), q1.data_ptr(),
                                             scales1.data_ptr(), 0, None, 50, hidden, 1e-6, stream) == 0
     assert torch.equal(q1.view(torch.uint8), q.view(torch.uint8)) and torch.equal(scales1, scales) and torch.equal(r1, total)
+
+
+def test_as_many_rows_as_32_bits_count(cuda_device):
+    """2^31 - 1 rows of 8: the last block has room for a row that 32 bits do not count."""
+    from bytetransformer_b200 import encoder as E
+    rows = (1 << 31) - 1
+    x = torch.empty(rows, 8, dtype=torch.float16, device=cuda_device)
+    x[:5], x[-5:] = torch.randn(5, 8, device=cuda_device).half(), torch.randn(5, 8, device=cuda_device).half()
+    x[5:-5].fill_(2.0)
+    gamma = torch.linspace(0.5, 2.0, 8, device=cuda_device).half()
+    out, _ = E.add_residual_rmsnorm(x, None, gamma)
+    for part in (slice(0, 9), slice(rows // 2, rows // 2 + 9), slice(rows - 9, rows)):
+        check_half(out[part], definition(x[part], None, gamma, 1e-6)[1])

@@ -124,3 +124,41 @@ def test_norm_over_its_own_inputs(lib, x_fp32, group, total, out):
     else:
         rc = lib.bt_add_residual_rmsnorm_e4m3(*args, 6 * P, group, None, 4, 768, 1e-6, None)
     assert rc == _abi.BT_ERR_INVALID_ARG
+
+
+class OnCuda(torch.Tensor):
+    """A tensor without memory that says it is on the device: nothing here gets as far as reading it."""
+    is_cuda = True
+
+
+def big(*shape, dtype=torch.float16):
+    return torch.empty(*shape, dtype=dtype, device="meta").as_subclass(OnCuda)
+
+
+CUT = (1 << 32) + 8  # 8 in 32 bits
+
+
+def test_sizes_past_32_bits_are_refused_not_cut(lib):
+    from bytetransformer_b200 import encoder as E
+    off, two = big(3, dtype=torch.int32), big(2, dtype=torch.int32)
+    q = big(64, 128)
+    for call in [
+            lambda: E.add_residual_rmsnorm(big(CUT, 8), None, big(8)),
+            lambda: E.add_residual_rmsnorm(big(8, CUT), None, big(CUT)),
+            lambda: E.add_residual_rmsnorm_e4m3(big(CUT, 8), None, big(8), group=128),
+            lambda: E.add_residual_rmsnorm(big(CUT, 8), None, big(8), m_dev=big(1, dtype=torch.int32)),
+            lambda: E.relative_position_bias(big(CUT, 4), 4, 4),
+            lambda: E.relative_position_bias(big(32, CUT), 4, 4),
+            lambda: E.relative_position_bias_grad(big(CUT, 4, 4), 32),
+            lambda: E.relative_position_bias_grad(big(CUT, 1, 4, 4), 32),
+            lambda: E.relative_position_bias_grad(big(2, 4, 4), CUT),
+            lambda: E.relative_position_bias_grad(big(2, 4, 4), -32),
+            lambda: E.window_attention(q, q, q, big(CUT, dtype=torch.int32), big(CUT, dtype=torch.int32), 8, 8),
+            lambda: E.window_attention(big(CUT, 64), q[:, :64], q[:, :64], off, off, 8, 8),
+            lambda: E.window_attention(q, big(CUT, 64), big(CUT, 64), off, off, 8, 8),
+            lambda: E.window_attention(big(1, CUT * 64), q, q, two, two, 1, 8),
+            lambda: E.window_attention(q, q, q, off, off, 8, 8, distance_bias=big(2, CUT, dtype=torch.float32), bias_left=4),
+            lambda: E.window_attention(q, q, q, off, off, 8 - (1 << 32), 8),
+            lambda: E.window_attention(q, q, q, off, off, 8, 8 - (1 << 32))]:
+        with pytest.raises(RuntimeError, match="2\\^3"):
+            call()
