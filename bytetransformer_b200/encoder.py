@@ -740,7 +740,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     with _On(device) as stream:
         if out is None:
             out = torch.empty(rows, heads * 64, dtype=torch.float16, device=device)
-        if rows == 0 or batch == 0:
+        if rows == 0 or batch == 0 or max_q_len == 0:
             return out
         ws, n = None, 0
         if max_q_len * heads <= 16 * kv_heads:  # few queries: the keys may be cut into ranges

@@ -622,3 +622,14 @@ def test_a_single_row_of_any_stride(cuda_device):
     offs = torch.tensor([0, 200], dtype=torch.int32, device=cuda_device)
     assert torch.equal(E.window_attention(many, row(k[0], 1), row(v[0], 1), offs, one, 200, 1),
                        E.window_attention(many, k[:1], v[:1], offs, one, 200, 1))
+
+
+def test_a_batch_without_queries(cuda_device):
+    """The longest of no queries at all is 0: nothing is written."""
+    from bytetransformer_b200 import encoder as E
+    q, k, v, off = packed([30, 20], 4, 2, cuda_device, seed=52)
+    none = torch.zeros(3, dtype=torch.int32, device=cuda_device)
+    out = torch.full_like(q, 7.0)
+    assert E.window_attention(q, k, v, none, off, 0, 30, out=out) is out and (out == 7).all()
+    assert (E.window_attention(q, k, v, none, off, 1, 30, out=out) == 7).all()
+    assert E.window_attention(q, k, v, none, off, 0, 30).shape == q.shape
