@@ -531,31 +531,66 @@ def _check_distances(q_len, k_len, max_distance, q_start):
         raise RuntimeError("lengths and q_start must be at most 2^29, max_distance at most 2^20")
 
 
-def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_distance: int = 128,
-                           bidirectional: bool = True, q_start: int = 0,
-                           out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
-    """[heads, q_len, k_len] = table[bucket(k - (q + q_start)), head]: the learned bias by buckets of distance, as
-    Encoder.forward_general takes it (fp16) or, with q_len = 1 and out_dtype float32, by distance as window_attention
-    does.  table [num_buckets, heads] fp16 or fp32; the buckets are those of bt_relative_position_bias."""
-    fp32 = _half_or_float(table, "table")
-    if table.dim() != 2:
-        raise RuntimeError("table must be [num_buckets, heads]")
-    if out_dtype not in (torch.float16, torch.float32):
-        raise RuntimeError("out_dtype must be torch.float16 or torch.float32")
+def _relative_bias(table, q_len, k_len, max_distance, bidirectional, q_start, out_dtype):
+    """The launch of relative_position_bias, whose arguments have been looked at."""
     buckets, heads = table.shape
-    _check_sizes(buckets, heads)
-    _check_distances(q_len, k_len, max_distance, q_start)
     if q_len == 0 or k_len == 0:
         return torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
     lib = _abi.load()
     with _On(table.device) as stream:
         out = torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
-        rc = lib.bt_relative_position_bias(table.data_ptr(), fp32, buckets, int(max_distance), int(bool(bidirectional)),
-                                           heads, q_len, k_len, int(q_start), out.data_ptr(),
+        rc = lib.bt_relative_position_bias(table.data_ptr(), _FP32[table.dtype], buckets, int(max_distance),
+                                           int(bool(bidirectional)), heads, q_len, k_len, int(q_start), out.data_ptr(),
                                            int(out_dtype == torch.float32), stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_relative_position_bias")
     return out
+
+
+class _RelativeBias(torch.autograd.Function):
+    """relative_position_bias of a table that asks for its gradient."""
+
+    @staticmethod
+    def forward(ctx, table, *how):
+        ctx.table, ctx.how = (table.shape[0], table.dtype), how
+        return _relative_bias(table, *how)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        if torch.cuda.is_current_stream_capturing():
+            # autograd itself does not survive a capture that meets leaves of a graph recorded outside it
+            raise RuntimeError("the backward pass of relative_position_bias cannot be captured: capture "
+                               "relative_position_bias_grad")
+        buckets, dtype = ctx.table
+        _, _, max_distance, bidirectional, q_start, _ = ctx.how
+        grad = grad.contiguous()
+        if grad.data_ptr() % 16 != 0:  # (part of something larger)
+            grad = grad.clone()
+        got = relative_position_bias_grad(grad, buckets, max_distance=max_distance, bidirectional=bidirectional,
+                                          q_start=q_start)
+        return (got.to(dtype),) + (None,) * len(ctx.how)
+
+
+def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_distance: int = 128,
+                           bidirectional: bool = True, q_start: int = 0,
+                           out_dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """[heads, q_len, k_len] = table[bucket(k - (q + q_start)), head]: the learned bias by buckets of distance, as
+    Encoder.forward_general takes it (fp16) or, with q_len = 1 and out_dtype float32, by distance as window_attention
+    does.  table [num_buckets, heads] fp16 or fp32; the buckets are those of bt_relative_position_bias.
+    A table that requires its gradient gets it through autograd, by relative_position_bias_grad, in the table's type;
+    that backward pass is refused in a stream capture (relative_position_bias_grad itself is not).  The encoder and
+    window_attention are forward passes only: what they make of the bias has no history."""
+    _half_or_float(table, "table")
+    if table.dim() != 2:
+        raise RuntimeError("table must be [num_buckets, heads]")
+    if out_dtype not in (torch.float16, torch.float32):
+        raise RuntimeError("out_dtype must be torch.float16 or torch.float32")
+    _check_sizes(*table.shape)
+    _check_distances(q_len, k_len, max_distance, q_start)
+    if table.requires_grad and torch.is_grad_enabled():
+        return _RelativeBias.apply(table, q_len, k_len, max_distance, bidirectional, q_start, out_dtype)
+    return _relative_bias(table, q_len, k_len, max_distance, bidirectional, q_start, out_dtype)
 
 
 @functools.lru_cache(maxsize=256)

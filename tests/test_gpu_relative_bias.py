@@ -209,3 +209,83 @@ def test_the_general_path_takes_it_as_attention_bias(cuda_device):
     by_hand = table[ids].t()[:, at].contiguous().to(cuda_device)
     assert torch.equal(enc.forward_general(x, mask, E.relative_position_bias(table.to(cuda_device), S, S)),
                        enc.forward_general(x, mask, by_hand))
+
+
+@pytest.mark.parametrize("table_type", [torch.float16, torch.float32])
+@pytest.mark.parametrize("out_type", [torch.float16, torch.float32])
+def test_a_table_gets_its_gradient(cuda_device, table_type, out_type):
+    """Through the bias into the table, from gradients of every layout, against the sum by buckets in 64 bits."""
+    from bytetransformer_b200 import encoder as E
+    heads, q, k, buckets, dist, start = 3, 45, 67, 16, 20, 5
+    g = torch.Generator().manual_seed(61)
+    ids, at = by_distance(q, k, start, buckets, dist, True)
+    member = ids[at].reshape(-1)
+    data = torch.randn(buckets, heads, generator=g).to(table_type).to(cuda_device)
+    w = torch.randn(heads, q, k, generator=g).to(out_type).to(cuda_device)
+    ones = torch.ones((), dtype=out_type, device=cuda_device)
+    odd = torch.empty(w.numel() + 1, dtype=out_type, device=cuda_device)[1:].view(heads, q, k).copy_(w)
+    for grad in (w, ones.expand(heads, q, k), w.transpose(1, 2).contiguous().transpose(1, 2), odd):
+        table = data.clone().requires_grad_()
+        bias = E.relative_position_bias(table, q, k, max_distance=dist, q_start=start, out_dtype=out_type)
+        assert bias.requires_grad and torch.equal(bias.detach(), E.relative_position_bias(data, q, k, max_distance=dist, q_start=start,
+                                                                                         out_dtype=out_type))
+        bias.backward(grad)
+        assert table.grad.dtype == table_type
+        flat = grad.cpu().double().reshape(heads, -1)
+        want = torch.zeros(heads, buckets, dtype=torch.float64).index_add_(1, member, flat).t()
+        size = torch.zeros(heads, buckets, dtype=torch.float64).index_add_(1, member, flat.abs()).t()
+        step = want.abs() * 2.0 ** -11 + 2.0 ** -25 if table_type == torch.float16 else 0.0
+        assert ((table.grad.cpu().double() - want).abs() <= ROUNDINGS * 2.0 ** -24 * size * 1.001 + step).all()
+    with torch.no_grad():
+        assert not E.relative_position_bias(table, q, k).requires_grad
+    assert not E.relative_position_bias(table.detach(), q, k).requires_grad
+    with pytest.raises(RuntimeError):  # no second derivative
+        table = data.clone().requires_grad_()
+        first, = torch.autograd.grad(E.relative_position_bias(table, q, k).float().sum(), table, create_graph=True)
+        first.float().sum().backward()
+
+
+def test_the_gradient_of_a_shared_table_adds_up_and_by_differences(cuda_device):
+    """A table used twice, as two layers use it, within a larger expression: linear in the table, so a difference is its gradient."""
+    from bytetransformer_b200 import encoder as E
+    table = torch.randn(16, 2, device=cuda_device, requires_grad=True)
+    w = torch.randn(2, 9, 14, device=cuda_device)
+
+    def total(t):
+        a = E.relative_position_bias(t, 9, 14, max_distance=20, out_dtype=torch.float32)
+        b = E.relative_position_bias(t, 1, 14, max_distance=20, q_start=13, bidirectional=False, out_dtype=torch.float32)
+        return (a * w).double().sum() + (b * 3.0).double().sum()
+    total(table).backward()
+    step = torch.zeros_like(table)
+    for at in range(table.numel()):
+        step.view(-1)[at] = 1.0
+        with torch.no_grad():
+            moved = total(step)
+        assert abs(float(moved) - float(table.grad.view(-1)[at])) <= (ROUNDINGS + 2) * 2.0 ** -24 * float(w.abs().sum() + 3 * 28)
+        step.view(-1)[at] = 0.0
+    assert E.relative_position_bias(table, 0, 5).sum().requires_grad
+    E.relative_position_bias(table, 0, 5).sum().backward()
+
+
+def test_a_captured_backward_pass_is_refused(cuda_device):
+    """With a graph of the same table alive outside the capture, autograd would end the process; the forward pass and
+    relative_position_bias_grad are captured as ever."""
+    from bytetransformer_b200 import encoder as E
+    table = torch.randn(32, 4, device=cuda_device, requires_grad=True)
+    alive = E.relative_position_bias(table, 20, 20)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(graph):
+            E.relative_position_bias(table, 20, 20).sum().backward()
+    torch.cuda.synchronize()
+    del graph
+    alive.sum().backward()
+    want = E.relative_position_bias_grad(torch.ones(4, 20, 20, dtype=torch.float16, device=cuda_device), 32)
+    assert torch.equal(table.grad, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        bias = E.relative_position_bias(table, 20, 20)
+        got = E.relative_position_bias_grad(bias.detach(), 32)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(bias, alive) and torch.equal(got, E.relative_position_bias_grad(alive.detach(), 32))
