@@ -246,7 +246,7 @@ __device__ __forceinline__ void watch(__half2& t, uint32_t w) {
   t = __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&w)), t);
 }
 __device__ __forceinline__ void watch_row(__half2& t, const __half* row) {
-#pragma unroll 1
+#pragma unroll 4
   for (int x = 0; x < kHeadDim; x += 8) {
     const uint4 w = *reinterpret_cast<const uint4*>(row + x);
     watch(t, w.x);
@@ -301,7 +301,7 @@ __device__ __forceinline__ void redo_row(const WindowArgs& a, const Keys& keys, 
     if (mine) {
       const __half* k = row_of(a.k, a.k_stride, u);
       float dot = 0.f;
-#pragma unroll 1
+#pragma unroll 4
       for (int x = 0; x < kHeadDim; x += 8) {
         const uint4 qw = *reinterpret_cast<const uint4*>(q + x), kw = *reinterpret_cast<const uint4*>(k + x);
         const uint32_t qs[4] = {qw.x, qw.y, qw.z, qw.w}, ks[4] = {kw.x, kw.y, kw.z, kw.w};
@@ -324,12 +324,20 @@ __device__ __forceinline__ void redo_row(const WindowArgs& a, const Keys& keys, 
     l = fmaf(l, f, w);
     o0 *= f;
     o1 *= f;
-    for (; left != 0u; left &= left - 1u) {
-      const int t = __ffs(left) - 1;
-      const float wt = __shfl_sync(0xffffffffu, w, t);
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(row_of(a.v, a.v_stride, u0 + t) + 2 * lane));
-      o0 = fmaf(wt, v.x, o0);
-      o1 = fmaf(wt, v.y, o1);
+#pragma unroll 1
+    for (int t0 = 0; t0 < 32; t0 += 8, left >>= 8) {  // (eight loads under way at a time)
+      if ((left & 0xffu) == 0u) continue;
+      uint32_t v[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        v[t] = (left >> t) & 1u ? *reinterpret_cast<const uint32_t*>(row_of(a.v, a.v_stride, u0 + t0 + t) + 2 * lane) : 0u;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const float wt = __shfl_sync(0xffffffffu, w, t0 + t);  // (0 where the key is not seen)
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[t]));
+        o0 = fmaf(wt, f.x, o0);
+        o1 = fmaf(wt, f.y, o1);
+      }
     }
   }
 #pragma unroll
