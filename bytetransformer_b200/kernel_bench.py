@@ -12,7 +12,7 @@ Cases and their reference counterparts: offsets (remove_padding.h:36-101), pack 
 (remove_padding.h:104-121, layernorm.h:430-446), layernorm / layernorm_restore (layernorm.h:410-446),
 gelu (gemm_bias_act.cu:32-66), softmax (softmax.h:191-297), embedding (layernorm.h:219-240), pooler,
 mha_s64 / mha_s256 (attention_fused.cu:295-414, attention_fused_long.cu:171-312); without a counterpart there: relative_bias /
-relative_bias_grad, rmsnorm / rmsnorm_e4m3, window / window_token.
+relative_bias_grad, rmsnorm / rmsnorm_e4m3, window / window_token{,_cluster,_join}.
 """
 from __future__ import annotations
 
@@ -25,7 +25,8 @@ import numpy as np
 import torch
 
 ALL_CASES = ["offsets", "pack", "restore", "layernorm", "layernorm_restore", "gelu", "softmax", "embedding", "pooler",
-             "mha_s64", "mha_s256", "relative_bias", "relative_bias_grad", "rmsnorm", "rmsnorm_e4m3", "window", "window_token"]
+             "mha_s64", "mha_s256", "relative_bias", "relative_bias_grad", "rmsnorm", "rmsnorm_e4m3", "window", "window_token",
+             "window_token_cluster", "window_token_join"]
 
 
 def _peaks():
@@ -209,13 +210,17 @@ def main():
         pairs = sum(min(p, left) + 1 + min(4, max(0, p - left)) for p in range(Lw))
         report("window", "window_mha_kernel", us, flops=4.0 * 64 * nh * pairs, note=f"one sequence of {Lw}, {left} keys back, 4 first ones, {nh} heads")
         del qkv, q, k, v
-    if "window_token" in cases:
-        Bt, Lt = 64, 4096
-        cache = torch.randn(Bt * Lt, 2 * 4 * 64, dtype=torch.float16, device=dev)
-        q = torch.randn(Bt, 16 * 64, dtype=torch.float16, device=dev)
-        off = torch.arange(Bt + 1, dtype=torch.int32, device=dev)
-        us = _time(lambda: E.window_attention(q, cache[:, :256], cache[:, 256:], off, off * Lt, 1, Lt), args.iters, args.warmup)
-        report("window_token", "window_few_kernel + join", us, 2 * cache.numel(), note=f"one token for each of {Bt} sequences of {Lt} keys, 16 heads over 4")
+    # one range of keys for each item; ranges that a cluster puts together; ranges that a second kernel does
+    for case, Bt, Lt, heads, kvh in (("window_token", 64, 4096, 16, 4), ("window_token_cluster", 16, 1027, 4, 1),
+                                     ("window_token_join", 4, 32768, 8, 2)):
+        if case in cases:
+            cache = torch.randn(Bt * Lt, 2 * kvh * 64, dtype=torch.float16, device=dev)
+            q = torch.randn(Bt, heads * 64, dtype=torch.float16, device=dev)
+            off = torch.arange(Bt + 1, dtype=torch.int32, device=dev)
+            us = _time(lambda: E.window_attention(q, cache[:, :kvh * 64], cache[:, kvh * 64:], off, off * Lt, 1, Lt), args.iters, args.warmup)
+            report(case, "window_few_kernel" + (" + join" if case == "window_token_join" else ""), us, 2 * cache.numel(),
+                   note=f"one token for each of {Bt} sequences of {Lt} keys, {heads} heads over {kvh} (the call from Python, host included)")
+            del cache
     if enc is not None:
         st_word = enc.device_status()
         enc.close()
