@@ -12,8 +12,8 @@
 //
 // What both kernels live on: a bias is constant along diagonals.  Both are bound by memory: the forward writes
 // heads * q_len * k_len elements and reads nothing to speak of, the gradient reads as many and writes a table.
-// Measured on B200: 16 heads, 1024 x 1024 fp16 7.4 us (4.6 TB/s of stores into L2; filling the same with a constant takes 9.1); the
-// gradient of 16 sequences of that 94 us (5.7 TB/s, 0.88 of a plain copy), of 8 x 12 heads x 509 x 509 16.4 us.
+// Measured on B200: 16 heads, 1024 x 1024 fp16 7.3 us (4.6 TB/s of stores into L2; filling the same with a constant takes 9.1), fp32 13.0; the
+// gradient of 16 sequences of that 94 us (5.7 TB/s, 0.88 of a plain copy; fp32 160 us, 6.7 TB/s), of 8 x 12 heads x 509 x 509 16.4 us.
 #include <math.h>
 
 #include "common.cuh"
@@ -60,7 +60,7 @@ struct Whole {
   }
 };
 
-bool bucket_borders(Borders* b, int num_buckets, int max_distance, int bidirectional) {
+void bucket_borders(Borders* b, int num_buckets, int max_distance, int bidirectional) {
   b->sides = bidirectional ? 2 : 1;
   b->count = num_buckets / b->sides;
   b->exact = b->count / 2;
@@ -86,7 +86,6 @@ bool bucket_borders(Borders* b, int num_buckets, int max_distance, int bidirecti
     }
     b->first[e + j] = n;
   }
-  return true;
 }
 
 // Bucket of distance d by the borders in shared memory: the logarithm to a few bits, then the borders decide.
@@ -442,7 +441,7 @@ GradSplit grad_split(int batch, int heads, int q_len, int k_len, int elem_bytes)
   // Chunks of 128 rows waste least (a chunk of R rows walks R diagonals more than the matrix has columns), but every CTA
   // walks its rows one after the other: calls of few rows take shorter ones, down to 16, while there are fewer than two CTAs to an
   // SM.  us with that line at 1 / 2 / 4 / 8 CTAs to an SM: 8 x 12 heads x 197 x 197 12.7 / 9.8 / 11.3 / 13.7; 16 heads, 1024 x 1024 11.5 / 11.9 /
-  // 16.4 / 16.4; 2 x 16 heads x 384 x 384 9.1 / 7.7 / 9.9 / 9.9.
+  // 16.4 / 16.4; 2 x 16 heads x 384 x 384 9.1 / 7.7 / 9.9 / 9.9.  (148 SMs, a B200's: the workspace is asked for without a device.)
   s.chunk_rows = kGradRows;
   while (s.chunk_rows > 16 && static_cast<long long>(batch) * heads * ((q_len + s.chunk_rows - 1) / s.chunk_rows) < 2 * 148) s.chunk_rows /= 2;
   s.chunks = (q_len + s.chunk_rows - 1) / s.chunk_rows;
@@ -463,7 +462,7 @@ cudaError_t launch_grad(const GradArgs& a, cudaStream_t stream) {
 template <typename T, typename TableT>
 cudaError_t launch_bias(BiasArgs a, cudaStream_t stream) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  // (16 heads, 1024 x 1024 fp16, us by tile: 64 x 1024 13.9, 64 x 512 9.0, 32 x 512 7.4, 64 x 256 7.0, 16 x 256 11.8: enough CTAs that some
+  // (16 heads, 1024 x 1024 fp16, us by tile: 64 x 1024 12.8, 64 x 512 9.3, 32 x 512 7.7, 64 x 256 7.3, 16 x 256 12.0: enough CTAs that some
   // store while others lay out their diagonals)
   a.cols = a.k_len <= 256 + V ? a.k_len : 256;
   a.rows = a.q_len < 64 ? a.q_len : 64;

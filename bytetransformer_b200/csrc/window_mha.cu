@@ -40,7 +40,7 @@ constexpr int kKeys = 64;   // keys of a tile
 constexpr int kHeadDim = 64;
 constexpr int kQTile = kRows * kHeadDim * 2;   // 16 KiB
 constexpr int kKvTile = kKeys * kHeadDim * 2;  // 8 KiB
-constexpr int kThreads = 384;  // two groups of four softmax warps; loads, MMAs of either group, bias
+constexpr int kThreads = 384;  // two groups of four softmax warps; loads, MMAs of either group; a warp that only makes the four whole
 constexpr int kSlots = 4;  // items between the loader and the other roles
 constexpr int kSeam = 32;  // keys of a box of the tile with the seam
 constexpr float kOneBias = 1048576.0f;  // a bias that is one for many keys is kept out of their scores below this (log2 units)
@@ -259,7 +259,7 @@ __device__ __forceinline__ bool not_finite(__half2 t) { return !(__low2float(t) 
 // Where values of keys that a row does not see are infinities or NaN, a product with their weights of zero leaves NaN in the row.
 // A row that came out so is looked at again, by a whole warp: if any key or value that it does not see, of those that its item
 // multiplied, holds such a number, the row is done anew over the keys that it sees alone.  Slow (32 keys at a time, without
-// matrix instructions), but nothing with finite inputs comes here.
+// matrix instructions: 190 us for a row of 2,047 keys, 560 before eight loads went at a time), but nothing with finite inputs comes here.
 template <bool BIAS>
 __device__ __forceinline__ void redo_row(const WindowArgs& a, const Keys& keys, const Item& it, int i, int head) {
   const int lane = static_cast<int>(threadIdx.x & 31u);
@@ -388,8 +388,8 @@ struct Layout {
 template <bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
 window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k16,
-                  const __grid_constant__ CUtensorMap tm_v16, const WindowArgs args) {
+                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_k_seam,
+                  const __grid_constant__ CUtensorMap tm_v_seam, const WindowArgs args) {
   using L = Layout;
   constexpr int kStages = L::kStages, kQStages = L::kStages;
   constexpr int kLoadTimeout = kStatusMhaLoadTimeout, kMmaTimeout = kStatusMhaMmaTimeout, kSoftmaxTimeout = kStatusMhaSoftmaxTimeout;
@@ -554,11 +554,11 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           };
           ok = wait_role(&k_empty[slot], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
           if (!ok) break;
-          if (elect_one()) fetch(smem + L::kK + slot * kKvTile, &tm_k, &tm_k16, &k_full[slot]);
+          if (elect_one()) fetch(smem + L::kK + slot * kKvTile, &tm_k, &tm_k_seam, &k_full[slot]);
           __syncwarp();
           ok = wait_role(&v_empty[slot], phase ^ 1u, abort_flag, args.status, kLoadTimeout);
           if (!ok) break;
-          if (elect_one()) fetch(smem + L::kV + slot * kKvTile, &tm_v, &tm_v16, &v_full[slot]);
+          if (elect_one()) fetch(smem + L::kV + slot * kKvTile, &tm_v, &tm_v_seam, &v_full[slot]);
           __syncwarp();
         }
         if (!ok) break;
@@ -941,7 +941,8 @@ cudaError_t launch_window(const CUtensorMap (&tm)[5], WindowArgs a, int sms, cud
 // its virtual keys) and all rows that need them; each of its four warps walks every fourth 32 keys with a softmax of its
 // own, on mma.sync (16 x 8 x 16: a tcgen05 tile would be one eighth full at best).  A warp has a ring of its own of 32 keys and
 // values, fetched by TMA a step ahead; no warp waits for another before the range ends.  Bound by HBM: 32 sequences of 8192 keys, 32 heads
-// over 8, 81.7 us (6.6 TB/s); 64 of 4100 keys, 16 heads over 4, 44.2 us (with loads straight into the operands' registers 98 and 55).
+// over 8, 81.7 us (6.6 TB/s); 64 of 4100 keys, 16 heads over 4, 44.2 us (with loads straight into the operands' registers 98 and 55;
+// 45.0 with the look at rows that are not finite, with the bias 64.4).
 // Rings of 2 stages and three CTAs to an SM, 3 and two, 4 and one, of the latter 44.2 / 46.2 / 68.2 us.
 constexpr int kFewRows = 16;
 constexpr int kFewWarps = 4;
@@ -1351,9 +1352,12 @@ struct FewSplit {
 // Three CTAs are resident to an SM, but two of them already keep the memory busy: waves are counted by two.  us per call with
 // waves of 296 / 370 / 444 / 592: 64 sequences of 4100 keys, 16 heads over 4, 44.2 / 51.3 / 50.3 / 56.8; 32 of 8192, 32 over 8, 81.7 / 91.1 /
 // 88.6 / 105; 40 of 3000, 8 heads, 45.4 / 41.4 / 45.2 / 47.4; 8 of 4096, 12 heads, 21.5 / 21.5 / 21.0 / 25.2.
-// Clusters save the second kernel, but their CTAs come and go together: where all are resident at once 16 sequences of 1027
-// keys, one key/value head 7.2 us (second kernel: 7.8), 4 of 700, 2 heads 6.4 (7.5); where they are not, the 64 sequences of 4100
-// keys above 71 (55; all with the registers' loads that the rings replaced).
+// Clusters save the second kernel, but their CTAs come and go together, so only calls whose CTAs are all resident at once take them.
+// us with clusters (second kernel): 16 sequences of 1027 keys, one key/value head, 128 CTAs 6.4 (6.7); 4 of 700, 2 heads, 40 CTAs 5.4
+// (6.3); 60 of 1000, 240 CTAs 7.6 (8.4); 110 of 1000, 220 CTAs 8.6 (10.7); 8 of 4096, 12 heads, 288 CTAs 21.9 (22.8); 74 of 2000, 296
+// CTAs 11.9 (11.6).  Beyond the limit: 150 of 2000, 450 CTAs 23.5 (21.9); 48 of 1024, 4 heads, 576 CTAs 18.8 (17.6); 40 of 3000,
+// 8 heads, 1280 CTAs 49.9 (48.1); 444 of 2000, 888 CTAs 43.5 (45.9).
+// 148 SMs, a B200's: the workspace is asked for without a device, and the call has to come to the same split.
 FewSplit few_split(int batch, int kv_heads, int group, int max_q, int max_k, int left, int sinks) {
   FewSplit f;
   if (static_cast<long long>(max_q) * group > kFewRows || batch > 65535 || kv_heads > 65535) return f;
