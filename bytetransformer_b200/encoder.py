@@ -519,28 +519,28 @@ def _half_or_float(t: torch.Tensor, name: str, device=None) -> int:
     return _FP32[t.dtype]
 
 
-def _check_sizes(*sizes):
-    """The library's sizes are 32 bits wide: what does not fit is refused before it is cut off."""
-    if max(sizes) >= 1 << 31 or min(sizes) < 0:
-        raise RuntimeError("sizes must be below 2^31 and not negative")
+# The library's sizes are 32 bits wide: what does not fit is refused before it is cut off.
+_SIZE_LIMIT = 1 << 31
+_TOO_LARGE = "sizes must be below 2^31 and not negative"
 
 
-def _check_distances(q_len, k_len, max_distance, q_start):
-    """The same for lengths and positions, whose sums have to fit too."""
+def _check_distances(buckets, heads, q_len, k_len, max_distance, q_start):
+    """Sizes of a bias; those that are added to one another leave room for the sums."""
+    if not 0 <= buckets < _SIZE_LIMIT > heads:
+        raise RuntimeError(_TOO_LARGE)
     if not (0 <= q_len <= 1 << 29 and 0 <= k_len <= 1 << 29 and -(1 << 29) <= q_start <= 1 << 29 and 0 < max_distance <= 1 << 20):
         raise RuntimeError("lengths and q_start must be at most 2^29, max_distance at most 2^20")
 
 
-def _relative_bias(table, q_len, k_len, max_distance, bidirectional, q_start, out_dtype):
+def _relative_bias(table, fp32, buckets, heads, q_len, k_len, max_distance, bidirectional, q_start, out_dtype):
     """The launch of relative_position_bias, whose arguments have been looked at."""
-    buckets, heads = table.shape
     if q_len == 0 or k_len == 0:
         return torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
     lib = _abi.load()
     with _On(table.device) as stream:
         out = torch.empty(heads, q_len, k_len, dtype=out_dtype, device=table.device)
-        rc = lib.bt_relative_position_bias(table.data_ptr(), _FP32[table.dtype], buckets, int(max_distance),
-                                           int(bool(bidirectional)), heads, q_len, k_len, int(q_start), out.data_ptr(),
+        rc = lib.bt_relative_position_bias(table.data_ptr(), fp32, buckets, int(max_distance), int(bool(bidirectional)),
+                                           heads, q_len, k_len, int(q_start), out.data_ptr(),
                                            int(out_dtype == torch.float32), stream)
     if rc != _abi.BT_OK:
         raise _abi.BtError(rc, "bt_relative_position_bias")
@@ -552,7 +552,7 @@ class _RelativeBias(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, *how):
-        ctx.table, ctx.how = (table.shape[0], table.dtype), how
+        ctx.table_dtype, ctx.how = table.dtype, how
         return _relative_bias(table, *how)
 
     @staticmethod
@@ -562,14 +562,13 @@ class _RelativeBias(torch.autograd.Function):
             # autograd itself does not survive a capture that meets leaves of a graph recorded outside it
             raise RuntimeError("the backward pass of relative_position_bias cannot be captured: capture "
                                "relative_position_bias_grad")
-        buckets, dtype = ctx.table
-        _, _, max_distance, bidirectional, q_start, _ = ctx.how
+        _, buckets, _, _, _, max_distance, bidirectional, q_start, _ = ctx.how
         grad = grad.contiguous()
         if grad.data_ptr() % 16 != 0:  # (part of something larger)
             grad = grad.clone()
         got = relative_position_bias_grad(grad, buckets, max_distance=max_distance, bidirectional=bidirectional,
                                           q_start=q_start)
-        return (got.to(dtype),) + (None,) * len(ctx.how)
+        return (got.to(ctx.table_dtype),) + (None,) * len(ctx.how)
 
 
 def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_distance: int = 128,
@@ -581,16 +580,16 @@ def relative_position_bias(table: torch.Tensor, q_len: int, k_len: int, *, max_d
     A table that requires its gradient gets it through autograd, by relative_position_bias_grad, in the table's type;
     that backward pass is refused in a stream capture (relative_position_bias_grad itself is not).  The encoder and
     window_attention are forward passes only: what they make of the bias has no history."""
-    _half_or_float(table, "table")
+    fp32 = _half_or_float(table, "table")
     if table.dim() != 2:
         raise RuntimeError("table must be [num_buckets, heads]")
     if out_dtype not in (torch.float16, torch.float32):
         raise RuntimeError("out_dtype must be torch.float16 or torch.float32")
-    _check_sizes(*table.shape)
-    _check_distances(q_len, k_len, max_distance, q_start)
+    buckets, heads = table.shape
+    _check_distances(buckets, heads, q_len, k_len, max_distance, q_start)
     if table.requires_grad and torch.is_grad_enabled():
-        return _RelativeBias.apply(table, q_len, k_len, max_distance, bidirectional, q_start, out_dtype)
-    return _relative_bias(table, q_len, k_len, max_distance, bidirectional, q_start, out_dtype)
+        return _RelativeBias.apply(table, fp32, buckets, heads, q_len, k_len, max_distance, bidirectional, q_start, out_dtype)
+    return _relative_bias(table, fp32, buckets, heads, q_len, k_len, max_distance, bidirectional, q_start, out_dtype)
 
 
 @functools.lru_cache(maxsize=256)
@@ -611,8 +610,9 @@ def relative_position_bias_grad(grad: torch.Tensor, num_buckets: int, *, max_dis
         raise RuntimeError("grad must be [heads, q_len, k_len] or [batch, heads, q_len, k_len]")
     batch = int(grad.shape[0]) if grad.dim() == 4 else 1
     heads, q_len, k_len = grad.shape[-3:]
-    _check_sizes(num_buckets, batch, heads)
-    _check_distances(q_len, k_len, max_distance, q_start)
+    if batch >= _SIZE_LIMIT:
+        raise RuntimeError(_TOO_LARGE)
+    _check_distances(num_buckets, heads, q_len, k_len, max_distance, q_start)
     if grad.numel() == 0:
         return torch.zeros(num_buckets, heads, dtype=torch.float32, device=grad.device)
     lib = _abi.load()
@@ -657,7 +657,8 @@ def add_residual_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], gamm
     fp16.  Rows from *m_dev on are left unwritten."""
     x_fp32, gamma_fp32 = _rmsnorm_args(x, residual, gamma, m_dev)
     rows, hidden = x.shape
-    _check_sizes(rows, hidden)
+    if rows >= _SIZE_LIMIT or hidden >= _SIZE_LIMIT:
+        raise RuntimeError(_TOO_LARGE)
     lib = _abi.load()
     with _On(x.device) as stream:
         out = torch.empty(rows, hidden, dtype=torch.float16, device=x.device)
@@ -681,7 +682,8 @@ def add_residual_rmsnorm_e4m3(x: torch.Tensor, residual: Optional[torch.Tensor],
     if group not in (0, 128):
         raise RuntimeError("group must be 0 (a scale per row) or 128 (a scale per 128 columns)")
     rows, hidden = x.shape
-    _check_sizes(rows, hidden)
+    if rows >= _SIZE_LIMIT or hidden >= _SIZE_LIMIT:
+        raise RuntimeError(_TOO_LARGE)
     lib = _abi.load()
     with _On(x.device) as stream:
         out = torch.empty(rows, hidden, dtype=torch.float8_e4m3fn, device=x.device)
@@ -711,11 +713,6 @@ def _rows(t: torch.Tensor, name: str, device) -> int:
     if t.device != device:
         raise RuntimeError(f"{name} is on {t.device}, the other tensors are on {device}")
     return cols // 64
-
-
-def _pitch(t: torch.Tensor) -> int:
-    """Elements from a row to the next.  The stride of a single row says nothing, whatever it is."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _ints(t: torch.Tensor, name: str, device) -> int:
@@ -764,9 +761,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
             raise RuntimeError("bias_left must be a place in distance_bias")
     if out is not None and (_rows(out, "out", device) != heads or out.shape[0] != rows):
         raise RuntimeError("out must have q's shape")
-    if max(max_q_len, max_k_len) >= 1 << 30 or min(max_q_len, max_k_len, sinks) < 0:
+    if not (0 <= max_q_len < 1 << 30 and 0 <= max_k_len < 1 << 30 and sinks >= 0):
         raise RuntimeError("max_q_len and max_k_len must be below 2^30, they and sinks not negative")
-    _check_sizes(batch, rows, k_rows, heads, n_bias)
+    if batch >= _SIZE_LIMIT or rows >= _SIZE_LIMIT or k_rows >= _SIZE_LIMIT or heads >= _SIZE_LIMIT or n_bias >= _SIZE_LIMIT:
+        raise RuntimeError(_TOO_LARGE)
     # bounds that no distance reaches, however large, are none (the library's are 32 bits wide)
     left = -1 if left < 0 or left >= max_k_len else left
     right = -1 if right < 0 or right >= 1 << 30 else right
@@ -782,8 +780,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
             n = _window_workspace(batch, heads, kv_heads, max_q_len, max_k_len, left, sinks)
             if n:
                 ws = torch.empty(n, dtype=torch.int8, device=device)
+        # elements from a row to the next; the stride of a single row says nothing, whatever it is
+        q_row, out_row = (q.stride(0), out.stride(0)) if rows > 1 else (heads * 64, heads * 64)
+        k_row, v_row = (k.stride(0), v.stride(0)) if k_rows > 1 else (kv_heads * 64, kv_heads * 64)
         a = _abi.bt_window_attention_args(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _pitch(q), _pitch(k), _pitch(v), _pitch(out),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q_row, k_row, v_row, out_row,
             q_offsets.data_ptr(), k_offsets.data_ptr(), k_lens.data_ptr() if k_lens is not None else None,
             batch, heads, kv_heads, rows, k_rows, max_q_len, max_k_len, left, right, sinks, scale,
             distance_bias.data_ptr() if distance_bias is not None else None, n_bias, bias_left if n_bias else 0,
