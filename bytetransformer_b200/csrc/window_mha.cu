@@ -257,9 +257,11 @@ __device__ __forceinline__ void watch_row(__half2& t, const __half* row) {
 }
 __device__ __forceinline__ bool not_finite(__half2 t) { return !(__low2float(t) < INFINITY) || !(__high2float(t) < INFINITY); }
 // Where values of keys that a row does not see are infinities or NaN, a product with their weights of zero leaves NaN in the row.
-// A row that came out so is looked at again, by a whole warp: if any key or value that it does not see, of those that its item
-// multiplied, holds such a number, the row is done anew over the keys that it sees alone.  Slow (32 keys at a time, without
-// matrix instructions: 190 us for a row of 2,047 keys, 560 before eight loads went at a time), but nothing with finite inputs comes here.
+// And where scores are so large (from 2^24 on) that a reference in single precision is off by whole steps of the exponent, weights may pass fp16's
+// range.  A row that came out so is looked at again, by a whole warp: if any key or value that it does not see, of those that its item
+// multiplied, holds such a number, or nothing that it does see, the row is done anew over the keys that it sees alone.  Slow (32 keys at a time, without
+// matrix instructions: 190 us for a row of 2,047 keys, 560 before eight loads went at a time), but nothing with finite inputs and scores below
+// 10^7 comes here.
 template <bool BIAS>
 __device__ __forceinline__ void redo_row(const WindowArgs& a, const Keys& keys, const Item& it, int i, int head) {
   const int lane = static_cast<int>(threadIdx.x & 31u);
@@ -278,18 +280,25 @@ __device__ __forceinline__ void redo_row(const WindowArgs& a, const Keys& keys, 
   auto row_of = [&](const __half* base, long long stride, int u) {
     return base + (static_cast<long long>(it.k_row) + key_of(u)) * stride + kv * kHeadDim;
   };
-  bool redo = false;
-#pragma unroll 1
-  for (int u = lane; u - lane < keys.total && !redo; u += 32) {
-    __half2 t = __half2half2(__ushort_as_half(0));
-    if (u < keys.total && !seen(u)) {
-      watch_row(t, row_of(a.k, a.k_stride, u));
-      watch_row(t, row_of(a.v, a.v_stride, u));
-    }
-    redo = __any_sync(0xffffffffu, not_finite(t));
-  }
-  if (!redo) return;
   const __half* q = a.q + static_cast<long long>(it.q_row + i) * a.q_stride + head * kHeadDim;
+  auto not_finite_among = [&](bool what_it_sees) {
+    bool found = false;
+#pragma unroll 1
+    for (int u = lane; u - lane < keys.total && !found; u += 32) {
+      __half2 t = __half2half2(__ushort_as_half(0));
+      if (u < keys.total && seen(u) == what_it_sees) {
+        watch_row(t, row_of(a.k, a.k_stride, u));
+        watch_row(t, row_of(a.v, a.v_stride, u));
+      }
+      found = __any_sync(0xffffffffu, not_finite(t));
+    }
+    return found;
+  };
+  if (!not_finite_among(false)) {
+    __half2 t = __half2half2(__ushort_as_half(0));
+    watch_row(t, q);
+    if (__any_sync(0xffffffffu, not_finite(t)) || not_finite_among(true)) return;
+  }
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;  // dimensions 2 lane, 2 lane + 1
 #pragma unroll 1
   for (int u0 = 0; u0 < keys.total; u0 += 32) {
@@ -671,7 +680,10 @@ window_mha_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       float f0 = m == -INFINITY ? 0.f : ex2(m - top);
       float f1 = theirs.x == -INFINITY ? 0.f : ex2(theirs.x - top);
       const float sum = fmaf(theirs.y, f1, l * f0);
-      const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // (a row that sees no key: zeros)
+      // A row that sees no key: zeros.  Any other has a key whose weight is 1 or more, but for references beyond 2^24 or so: their
+      // rounding is in all of the row's weights alike, and where these leave fp16's range the sum says so, or the products are not
+      // finite.  Such a row is done anew.
+      const float inv = sum >= 0.5f ? 1.0f / sum : (top == -INFINITY && sum == 0.f ? 0.f : NAN);
       f0 *= inv;
       f1 *= inv;
       __half* out = args.out + static_cast<long long>(it.q_row + quarter * 32) * args.out_stride + it.head * kHeadDim + (lane & 3) * 8;

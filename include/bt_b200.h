@@ -361,9 +361,9 @@ int bt_add_residual_rmsnorm_e4m3(const void* x, int x_fp32, const void* residual
  *   data pointers 16-byte aligned; q_offsets, k_offsets int32[batch+1], k_lens int32[batch], on the device.  max_q_len,
  *   max_k_len: upper bounds of Lq and Lk.  Rows of q and out from q_offsets[batch] on are neither read into a result nor written.
  *   Keys and values that a query does not see, a sequence's own or others', do not matter to it, also where they are infinities
- *   or NaN.  (Rows beside which they are get done a second time without matrix instructions, by a warp that takes up to 32 of them one
- *   after the other, 0.09 us for each key: one such value among 8,192 keys, 2,047 back, makes 6 ms of a call's 0.1.)
- *   out may not overlap q, k or v.
+ *   or NaN.  (Rows beside which they are, and rows whose scores pass 10^7 so that fp16 may not hold their weights, get done a second time
+ *   without matrix instructions, by a warp that takes up to 32 of them one after the other, 0.1 us for each key: one such value among
+ *   8,192 keys, 2,047 back, makes 7 ms of a call's 0.1.)  out may not overlap q, k or v.
  *   Offsets or lengths that do not describe rows of the buffers make the sequence a no-op and set the device's status
  *   word, as in bt_attention (bt_device_status of any handle of the device).
  *   The current device is the one used; the first call on it looks its properties up and must be outside a stream capture. */

@@ -633,3 +633,54 @@ def test_a_batch_without_queries(cuda_device):
     assert E.window_attention(q, k, v, none, off, 0, 30, out=out) is out and (out == 7).all()
     assert (E.window_attention(q, k, v, none, off, 1, 30, out=out) == 7).all()
     assert E.window_attention(q, k, v, none, off, 0, 30).shape == q.shape
+
+
+@pytest.mark.parametrize("size", [1.0, 30.0, 1000.0, 60000.0])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("q_len", [0, 1])
+def test_scores_up_to_the_largest_that_halves_can_make(cuda_device, size, sign, with_bias, q_len):
+    """Scores of up to 3e10, where a step of single precision is 2,048, all of one sign and either equal or so far apart that a row
+    takes the values of the keys with the largest, weighed by their biases.  q_len 1: one query for each sequence.  The weights of those
+    keys and their sum are rounded to fp16 in the one place: half a step of each, and of the result.  A bias loses half a step of its sum
+    with the score, twice as the sum of weights has it too; where that leaves nothing of it, the result lies between those values."""
+    from bytetransformer_b200 import encoder as E
+    lens, heads = [700, 129, 64], 2
+    g = torch.Generator().manual_seed(71)
+    q, k, v, off = packed(lens, heads, heads, cuda_device, seed=71)
+    T = sum(lens)
+    signs = torch.randint(0, 2, (heads * D,), generator=g).mul(2).sub(1).half().to(cuda_device)
+    ramp = (64 + 84 * torch.randperm(T, generator=g)[:T].float()).clamp(max=60000).half().to(cuda_device)
+    q = (signs * sign * size).expand(T, -1).contiguous()
+    k = ramp[:, None] * signs
+    bias = torch.randn(heads, 65, device=cuda_device) if with_bias else None
+    lost = 64 * size * 60000 * 0.125 * 2.0 ** -23 if with_bias else 0.0
+    ends, ones = off.tolist(), torch.arange(4, dtype=torch.int32, device=cuda_device)
+    last = [e - 1 for e in ends[1:]]
+    for left, right in [(-1, -1), (-1, 0), (100, 30)]:
+        if q_len:
+            got = E.window_attention(q[last], k, v, ones, off, 1, 700, left=left, right=right, distance_bias=bias, bias_left=32)
+        else:
+            got = E.window_attention(q, k, v, off, off, 700, 700, left=left, right=right, distance_bias=bias, bias_left=32)
+        for b, (first, end) in enumerate(zip(ends, ends[1:])):
+            p = torch.arange(end - first, device=cuda_device)[:, None]
+            d = p.t() - p
+            seen = ((d <= right) | (right < 0)) & ((d >= -left) | (left < 0))
+            for h in range(heads):
+                c = slice(h * D, h * D + D)
+                score = (64 * 0.125 * size * sign * ramp[first:end].double()).expand(end - first, -1)
+                if with_bias:
+                    score = score + bias[h].double()[(d + 32).clamp(0, 64)]
+                w = torch.softmax(score.masked_fill(~seen, -math.inf), 1)
+                vv = v[first:end, c].double()
+                want, whole = w @ vv, w @ vv.abs()
+                if lost < 0.25:
+                    off_by = whole * (2.0 ** -11 + 2 * lost * ((w > 0).sum(1, keepdim=True) > 1))
+                else:
+                    high = torch.where((w > 0)[:, :, None], vv[None], -math.inf).amax(1)
+                    low = torch.where((w > 0)[:, :, None], vv[None], math.inf).amin(1)
+                    want, off_by = (high + low) / 2, (high - low) / 2 + torch.maximum(high.abs(), low.abs()) * 2.0 ** -11
+                off_by = off_by * 1.01 + want.abs() * 2.0 ** -11 + 2.0 ** -25
+                mine = got[b:b + 1, c] if q_len else got[first:end, c]
+                ok = (mine.double() - want[-len(mine):]).abs() <= off_by[-len(mine):]
+                assert ok.all(), (left, right, b, h, int((~ok).sum()), int((~torch.isfinite(mine)).sum()))
